@@ -264,8 +264,7 @@ def _attend(s):
     out = torch.matmul(x, v).reshape(n, c["q_heads"], d).to(s["q"].dtype)
     if not c["track"]:
         return {"out": out}
-    w = s["weights"].transpose(0, 1)  # [kv_heads, pages, page]
-    w = w.flatten(1)
+    w = s["weights"].transpose(0, 1).clone().flatten(1)  # [kv_heads, slots]
     rows = (s["table"].long()[:, :, None] * c["page"] + torch.arange(c["page"], device="cuda")).flatten(1)[inside]
     w[:, rows] = w[:, rows] + x.sum(2).transpose(0, 1)[:, inside]
     s["weights"].copy_(w.view(hk, -1, c["page"]).transpose(0, 1))
