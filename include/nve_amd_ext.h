@@ -185,6 +185,144 @@ NVE_C_API nve_status_t nve_amd_pooling_backprop(
     nve_data_type_t grad_type, int64_t embedding_width, void* unique_keys_out, void* grads_out,
     int64_t* num_unique_out, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Paged key-value cache of an attention layer (serving; no counterpart in the
+ * reference).  A page holds page_size slots of num_heads key / value heads:
+ * k and v are [num_pages, num_heads, page_size, head_dim] of dtype (FLOAT32,
+ * FLOAT16, BFLOAT16 or E4M3), 16-byte aligned.  E4M3 rows have one f32 scale
+ * each (value = e4m3(code) * scale) in k_scale and v_scale [num_pages,
+ * num_heads, page_size]; NULL for the other types.  weights (f32) and index
+ * (int32) have the scales' shape: the attention weight a slot has received so
+ * far, and its token's place in its sequence; either may be NULL where a call
+ * does not need it.  page_size is a power of two from 8 to 1024, head_dim a
+ * multiple of 8 from 8 to 256.
+ * A sequence is a row of block_tables: its slot t lies in page
+ * block_tables[s * table_stride + t / page_size], row t % page_size.  Page ids
+ * outside [0, num_pages) are neither read nor written: their slots count as
+ * absent.  A length below 0 counts as 0, one above max_pages * page_size (or
+ * above a call's max_length) as that bound.  All pointers are device memory;
+ * strides are in elements, and the last dimension is contiguous. */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  float* weights;
+  int32_t* index;
+  int64_t num_pages;
+  int32_t num_heads;
+  int32_t page_size;
+  int32_t head_dim;
+  nve_data_type_t dtype;
+} nve_amd_kv_pages_t;
+
+/* New tokens enter the cache.  Token t's keys and values (num_heads heads of
+ * `dtype`, the pages' type, or FLOAT16 / BFLOAT16 for E4M3 pages) are written to
+ * slot slots[t] = page * page_size + row (a slot outside the cache is skipped;
+ * no slot may appear twice), index[t] to the slot's index (with pages->index;
+ * index NULL: positions[0][t], or 0 without positions), 0 to its weight (with
+ * pages->weights).  E4M3 rows: scale = max(largest magnitude, 1e-30) / 448,
+ * code = value / scale rounded to nearest even.
+ * rot_dim > 0: the first rot_dim values of every key head, and of every head of
+ * q, are rotated first.  Pair i (of rot_dim / 2) is values i and i +
+ * rot_dim / 2, or 2i and 2i + 1 if interleaved; it belongs to one of num_axes
+ * axes, the first sections[0] pairs to axis 0, the next sections[1] to axis 1
+ * and so on, and turns by row p = positions[axis * axis_stride + t] of cos_sin
+ * [max_position, rot_dim] (f32: the cosines of the pairs, then their sines):
+ *   (a, b) -> (a cos - b sin, b cos + a sin)
+ * in f32, rounded once.  A position outside [0, max_position) leaves its pairs
+ * as they are.  q (may be NULL): [num_tokens, num_q_heads, head_dim] of `dtype`,
+ * rotated into q_out, which may be q itself. */
+typedef struct {
+  int64_t num_tokens;
+  const int64_t* slots;
+  nve_data_type_t dtype;
+  const void* k;
+  int64_t k_token_stride, k_head_stride;
+  const void* v;
+  int64_t v_token_stride, v_head_stride;
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  void* q_out;
+  int64_t q_out_token_stride, q_out_head_stride;
+  int32_t num_q_heads;
+  const int32_t* index;
+  const int32_t* positions;
+  int64_t axis_stride;
+  const float* cos_sin;
+  int64_t max_position;
+  int32_t rot_dim;
+  int32_t interleaved;
+  int32_t num_axes;
+  int32_t sections[4];
+} nve_amd_kv_append_t;
+NVE_C_API nve_status_t nve_amd_kv_append(const nve_amd_kv_pages_t* pages,
+                                         const nve_amd_kv_append_t* call, void* stream);
+
+/* Attention of one new token per sequence over its slots t < lengths[s]:
+ *   x_t = scale * q . k_t,  p = softmax(x),  out = sum_t p_t v_t
+ * q and out: [num_seqs, num_q_heads, head_dim] of `dtype` (the pages' type, or
+ * FLOAT16 / BFLOAT16 for E4M3 pages); query head h reads key head
+ * h / (num_q_heads / num_heads).  lse (may be NULL): [num_seqs, num_q_heads],
+ * log sum_t exp(x_t).  Where no slot has a score above -infinity (a length of
+ * zero, say) out is 0 and lse -infinity.  What lies in a page's rows at or past
+ * the length is not used, whatever it is.  accumulate:
+ * p_t, summed over the query heads of a key head, is added to pages->weights;
+ * no page may then belong to two sequences of the call.  max_length: the
+ * longest length that occurs, if the caller knows it (0: the table's extent);
+ * it only sizes the launch.  workspace: device memory of
+ * nve_amd_kv_attend_workspace_size bytes, 16-byte aligned. */
+typedef struct {
+  int64_t num_seqs;
+  int32_t num_q_heads;
+  nve_data_type_t dtype;
+  const void* q;
+  int64_t q_seq_stride, q_head_stride;
+  void* out;
+  int64_t out_seq_stride, out_head_stride;
+  float* lse;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int64_t max_pages;
+  const int32_t* lengths;
+  int64_t max_length;
+  float scale;
+  int32_t accumulate;
+} nve_amd_kv_attend_t;
+NVE_C_API nve_status_t nve_amd_kv_attend_workspace_size(const nve_amd_kv_pages_t* pages,
+                                                        const nve_amd_kv_attend_t* call,
+                                                        uint64_t* bytes);
+NVE_C_API nve_status_t nve_amd_kv_attend(const nve_amd_kv_pages_t* pages,
+                                         const nve_amd_kv_attend_t* call, void* workspace,
+                                         uint64_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight.  Every sequence of more than
+ * `budget` slots keeps `budget` of them, chosen for each key head by itself:
+ * dropped are the first ones in the order (protected, weight, slot), where a
+ * slot is protected if its index is below `sinks` or among the `recent` places
+ * up to the head's newest index, a NaN weight is the greatest and slots of
+ * absent pages come first.  The j-th dropped slot below `budget` then takes the
+ * row (k, v, scales, weight, index) of the j-th kept slot at or past it;
+ * nothing else is written.  new_lengths[s] = min(lengths[s], budget).  No page
+ * may belong to two sequences of the call.  workspace: device memory of
+ * nve_amd_kv_evict_workspace_size bytes, 16-byte aligned. */
+typedef struct {
+  int64_t num_seqs;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int64_t max_pages;
+  const int32_t* lengths;
+  int32_t* new_lengths;
+  int64_t budget;
+  int64_t sinks;
+  int64_t recent;
+} nve_amd_kv_evict_t;
+NVE_C_API nve_status_t nve_amd_kv_evict_workspace_size(const nve_amd_kv_pages_t* pages,
+                                                       const nve_amd_kv_evict_t* call,
+                                                       uint64_t* bytes);
+NVE_C_API nve_status_t nve_amd_kv_evict(const nve_amd_kv_pages_t* pages,
+                                        const nve_amd_kv_evict_t* call, void* workspace,
+                                        uint64_t workspace_bytes, void* stream);
+
 /* Log level (include/logging.hpp:34-203): messages at or below the level are
  * written, errors to stderr and the rest to stdout.  Levels: 0 critical,
  * 10 error, 20 warning, 30 perf, 40 info, 100 verbose.  The initial level is

@@ -13,6 +13,7 @@
 #include "dedup.hpp"
 #include "host_layer.hpp"
 #include "kernels/noalloc_launch.hpp"
+#include "kv_cache.hpp"
 #include "layers.hpp"
 #include "trace.hpp"
 
@@ -1000,6 +1001,51 @@ nve_status_t nve_amd_dedup_gather_noalloc(nve_key_type_t key_type, int64_t num_k
   dedup_gather_run(key_bytes_of(key_type), num_keys, keys, static_cast<const uint8_t*>(table), num_rows,
                    row_size_in_bytes, output, output_stride, ses.device_scratch(), need, (hipStream_t)stream);
   NVE_HIP(ses.end());
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
+nve_status_t nve_amd_kv_append(const nve_amd_kv_pages_t* pages, const nve_amd_kv_append_t* call,
+                               void* stream) {
+  C_TRY
+  NVE_TRACE("nve_amd_kv_append");
+  kv_append_run(pages, call, (hipStream_t)stream);
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
+nve_status_t nve_amd_kv_attend_workspace_size(const nve_amd_kv_pages_t* pages,
+                                              const nve_amd_kv_attend_t* call, uint64_t* bytes) {
+  C_TRY
+  NVE_CHECK_ARG(bytes != nullptr, "bytes must not be NULL");
+  *bytes = kv_attend_workspace_bytes(pages, call);
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
+nve_status_t nve_amd_kv_attend(const nve_amd_kv_pages_t* pages, const nve_amd_kv_attend_t* call,
+                               void* workspace, uint64_t workspace_bytes, void* stream) {
+  C_TRY
+  NVE_TRACE("nve_amd_kv_attend");
+  kv_attend_run(pages, call, workspace, workspace_bytes, (hipStream_t)stream);
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
+nve_status_t nve_amd_kv_evict_workspace_size(const nve_amd_kv_pages_t* pages,
+                                             const nve_amd_kv_evict_t* call, uint64_t* bytes) {
+  C_TRY
+  NVE_CHECK_ARG(bytes != nullptr, "bytes must not be NULL");
+  *bytes = kv_evict_workspace_bytes(pages, call);
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
+nve_status_t nve_amd_kv_evict(const nve_amd_kv_pages_t* pages, const nve_amd_kv_evict_t* call,
+                              void* workspace, uint64_t workspace_bytes, void* stream) {
+  C_TRY
+  NVE_TRACE("nve_amd_kv_evict");
+  kv_evict_run(pages, call, workspace, workspace_bytes, (hipStream_t)stream);
   return NVE_SUCCESS;
   C_CATCH
 }

@@ -84,6 +84,36 @@ class HostTableConfig(ctypes.Structure):
                 ("invalid_key", I64)]
 
 
+class KvPages(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("weights", P), ("index", P),
+                ("num_pages", I64), ("num_heads", I32), ("page_size", I32), ("head_dim", I32),
+                ("dtype", I32)]
+
+
+class KvAppend(ctypes.Structure):
+    _fields_ = [("num_tokens", I64), ("slots", P), ("dtype", I32),
+                ("k", P), ("k_token_stride", I64), ("k_head_stride", I64),
+                ("v", P), ("v_token_stride", I64), ("v_head_stride", I64),
+                ("q", P), ("q_token_stride", I64), ("q_head_stride", I64),
+                ("q_out", P), ("q_out_token_stride", I64), ("q_out_head_stride", I64),
+                ("num_q_heads", I32), ("index", P), ("positions", P), ("axis_stride", I64),
+                ("cos_sin", P), ("max_position", I64), ("rot_dim", I32), ("interleaved", I32),
+                ("num_axes", I32), ("sections", I32 * 4)]
+
+
+class KvAttend(ctypes.Structure):
+    _fields_ = [("num_seqs", I64), ("num_q_heads", I32), ("dtype", I32),
+                ("q", P), ("q_seq_stride", I64), ("q_head_stride", I64),
+                ("out", P), ("out_seq_stride", I64), ("out_head_stride", I64), ("lse", P),
+                ("block_tables", P), ("table_stride", I64), ("max_pages", I64), ("lengths", P),
+                ("max_length", I64), ("scale", ctypes.c_float), ("accumulate", I32)]
+
+
+class KvEvict(ctypes.Structure):
+    _fields_ = [("num_seqs", I64), ("block_tables", P), ("table_stride", I64), ("max_pages", I64),
+                ("lengths", P), ("new_lengths", P), ("budget", I64), ("sinks", I64), ("recent", I64)]
+
+
 # name -> (restype, argtypes); status-returning calls use I32
 SIGNATURES = {
     "nve_get_last_error": (I32, [ctypes.POINTER(ctypes.c_char_p)]),
@@ -161,6 +191,13 @@ SIGNATURES = {
     "nve_amd_backprop_workspace_size": (I32, [I64, I64, I64, ctypes.POINTER(U64)]),
     "nve_amd_pooling_backprop": (I32, [ctypes.c_int, I64, P, ctypes.c_int, ctypes.c_int, P, I64, I64, P, I32,
                                        P, I32, I64, P, P, PI64, P, U64, P]),
+    "nve_amd_kv_append": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvAppend), P]),
+    "nve_amd_kv_attend_workspace_size": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvAttend),
+                                               ctypes.POINTER(U64)]),
+    "nve_amd_kv_attend": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvAttend), P, U64, P]),
+    "nve_amd_kv_evict_workspace_size": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvEvict),
+                                              ctypes.POINTER(U64)]),
+    "nve_amd_kv_evict": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvEvict), P, U64, P]),
 }
 
 _lib = None

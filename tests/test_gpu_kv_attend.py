@@ -1,0 +1,311 @@
+"""Attention of one new token over the paged key-value cache (nve_ops::kv_attend)
+against softmax attention in 64 bits: every type, head layouts, page sizes,
+lengths around the kernels' tile sizes, long sequences, what lies past a length,
+absent pages, strides, streams and graphs.  The bounds follow from the formula
+(kv_reference.attend)."""
+import math
+
+import numpy as np
+import pytest
+
+import kv_reference as R
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def setup(dtype, cache, lengths, q_heads, heads, dim, page, seed=0, spread=1.0, q_spread=1.0, extra=2, spare=3):
+    rng = np.random.default_rng(seed)
+    num_pages = sum(-(-n // page) for n in lengths) + spare
+    k, ks = R.make_pages(cache, num_pages, heads, page, dim, rng, spread)
+    v, vs = R.make_pages(cache, num_pages, heads, page, dim, rng)
+    table = R.tables(lengths, page, num_pages, rng, extra)
+    q = torch.from_numpy(rng.normal(0, q_spread, size=(len(lengths), q_heads, dim)).astype(np.float32))
+    return {"q": q.to(R.TORCH[dtype]), "k": k, "v": v, "ks": ks, "vs": vs, "table": table,
+            "lengths": np.asarray(lengths, np.int32), "dtype": dtype, "cache": cache, "page": page,
+            "weights": torch.from_numpy(rng.random((num_pages, heads, page)).astype(np.float32))}
+
+
+def poison_unused(s):
+    """NaN and infinities in every row no sequence holds."""
+    P, H, page, _ = s["k"].shape
+    used = np.zeros((P, page), bool)
+    for i, n in enumerate(s["lengths"]):
+        _, p, o = R.slots_of(s["table"][i], int(n), page, P)
+        used[p, o] = True
+    free = ~torch.from_numpy(used)
+    for name, bad in (("k", math.nan), ("v", math.inf)):
+        x = s[name].to(torch.float32)
+        x.transpose(1, 2)[free] = bad if s["cache"] != "e4m3" else math.nan
+        s[name] = x.to(s[name].dtype)
+    for name in ("ks", "vs"):
+        if s[name] is not None:
+            s[name].transpose(1, 2)[free] = math.inf
+
+
+def cuda(x):
+    return None if x is None else (torch.from_numpy(x) if isinstance(x, np.ndarray) else x).cuda()
+
+
+def call(s, scale, accumulate=True, **kw):
+    from pynve.torch import nve_kv
+
+    w = cuda(s["weights"]) if accumulate else None
+    out, lse = nve_kv.kv_attend(kw.pop("q", None) if "q" in kw else cuda(s["q"]), cuda(s["k"]), cuda(s["v"]),
+                                cuda(s["table"]), cuda(s["lengths"]), scale=scale, k_scale=cuda(s["ks"]),
+                                v_scale=cuda(s["vs"]), weights=w, return_lse=True, **kw)
+    torch.cuda.synchronize()
+    return out.cpu(), lse.cpu(), None if w is None else w.cpu()
+
+
+def check(s, scale, got, limit=None):
+    out, lse, w = got
+    lengths = s["lengths"] if limit is None else np.minimum(s["lengths"], limit)
+    ro, rl, ra, bo, bl, ba = R.attend(s["q"], R.values64(s["k"], s["ks"]), R.values64(s["v"], s["vs"]), s["table"],
+                                      lengths, scale, s["dtype"], s["cache"])
+    err = np.abs(out.to(torch.float32).double().numpy() - ro)
+    assert np.isfinite(err).all() and (err <= bo).all(), f"out: {np.max(err - bo)} over, {np.max(err)} off"
+    empty = np.isneginf(rl)
+    l64 = lse.double().numpy()
+    assert np.array_equal(np.isneginf(l64), empty)
+    assert (np.abs(l64 - rl)[~empty] <= bl[~empty]).all()
+    if w is not None:
+        w0 = s["weights"].double().numpy()
+        touched = ra > 0
+        e = np.abs(w.double().numpy() - (w0 + ra))
+        assert (e[touched] <= (ba + 2.0**-23 * (w0 + ra))[touched]).all(), f"weights {np.nanmax(e[touched])} off"
+        assert torch.equal(w[torch.from_numpy(~touched)], s["weights"][torch.from_numpy(~touched)])
+
+
+TYPES = [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3"), ("bf16", "e4m3")]
+
+
+@pytest.mark.parametrize("q_heads,heads,dim,page", [(8, 2, 128, 16), (3, 3, 64, 8), (12, 1, 80, 32), (16, 2, 256, 64),
+                                                    (10, 2, 8, 8), (20, 1, 96, 128), (34, 2, 136, 16), (7, 1, 40, 1024),
+                                                    (70, 1, 128, 16)])
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_types_and_layouts(dtype, cache, q_heads, heads, dim, page):
+    s = setup(dtype, cache, [0, 1, 9, 31, 32, 33, 64, 100, 257, 700], q_heads, heads, dim, page, seed=dim + page)
+    poison_unused(s)
+    check(s, dim**-0.5, call(s, dim**-0.5))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_every_short_length(dtype, cache):
+    s = setup(dtype, cache, list(range(0, 70)) + [127, 128, 129, 255, 256, 257, 511, 512, 513], 8, 2, 64, 16, seed=3)
+    poison_unused(s)
+    check(s, 0.125, call(s, 0.125))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("lengths", [[20011], [5000, 1, 0, 16384, 16385, 3]])
+def test_long_sequences(dtype, cache, lengths):
+    """Few rows, long caches: the length is split and joined."""
+    s = setup(dtype, cache, lengths, 8, 2, 64, 16, seed=11, q_spread=3.0)
+    poison_unused(s)
+    check(s, 0.125, call(s, 0.125))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_many_sequences(dtype, cache):
+    rng = np.random.default_rng(0)
+    s = setup(dtype, cache, [int(n) for n in rng.integers(0, 90, size=300)], 4, 2, 64, 16, seed=12)
+    check(s, 0.125, call(s, 0.125))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_one_slot_is_copied(dtype, cache, accumulate):
+    """A softmax over one slot is 1: the output is the value row itself."""
+    s = setup(dtype, cache, [1, 1, 1], 6, 3, 128, 16, seed=4, q_spread=30.0)
+    out, lse, w = call(s, 0.2, accumulate)
+    for i in range(3):
+        v = R.values64(s["v"], s["vs"])[s["table"][i, 0], :, 0].astype(np.float32)
+        want = torch.from_numpy(np.repeat(v, 2, axis=0)).to(R.TORCH[dtype])
+        if cache == "e4m3":  # the scale meets the weight before the code does: 16 bits of it are kept
+            assert (out[i].float() - want.float()).abs().max() <= want.float().abs().max() * (2.0**-15 + R.HALF_ULP[dtype] * 2)
+        else:
+            assert torch.equal(out[i], want)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_wide_scores(dtype, cache):
+    """Scores of some hundreds: one slot takes nearly all the weight, most of the others none."""
+    s = setup(dtype, cache, [1000, 37, 4097], 8, 2, 64, 16, seed=5, spread=4.0, q_spread=8.0)
+    check(s, 1.0, call(s, 1.0))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_flat_tail_is_not_lost(dtype, cache):
+    """One slot far above 20,000 equal ones that together weigh as much: 2e4 e^-10 = 0.91."""
+    s = setup(dtype, cache, [20001], 2, 1, 64, 16, seed=6)
+    q = torch.zeros_like(s["q"])
+    q[..., 0] = 1.0
+    k = torch.zeros(s["k"].shape)
+    top = (int(s["table"][0, 700]), 0, 3)
+    k[top][0] = 10.0
+    if cache == "e4m3":
+        s["ks"] = torch.ones_like(s["ks"])
+    s["q"], s["k"] = q, k.to(s["k"].dtype)
+    check(s, 1.0, call(s, 1.0))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES[:3])
+def test_scores_of_minus_infinity(dtype, cache):
+    """-infinity scores weigh nothing; where there are no others the row is empty."""
+    s = setup(dtype, cache, [50, 600, 33], 4, 2, 64, 16, seed=7)
+    s["q"][..., 0] = 1.0
+    for i, n in enumerate(s["lengths"]):
+        _, p, o = R.slots_of(s["table"][i], int(n), 16, s["k"].shape[0])
+        off = np.arange(n) >= 0 if i == 2 else np.arange(n) % 40 < 35
+        s["k"][torch.from_numpy(p[off]), :, torch.from_numpy(o[off]), 0] = -math.inf
+    out, lse, w = call(s, 0.3)
+    assert torch.equal(out[2], torch.zeros_like(out[2]))
+    check(s, 0.3, (out, lse, w))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_absent_pages(dtype, cache):
+    """Page numbers outside the cache inside a length: their slots are left out."""
+    s = setup(dtype, cache, [300, 17, 40], 4, 2, 64, 16, seed=8)
+    s["table"][0, 3], s["table"][0, 7], s["table"][0, 18] = -1, s["k"].shape[0], 2**31 - 1
+    s["table"][1, :] = -5
+    check(s, 0.125, call(s, 0.125))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_length_bounds(dtype, cache):
+    """Negative lengths count as 0, those above the table (or max_length) as that bound."""
+    s = setup(dtype, cache, [64, 48, 5], 4, 2, 64, 16, seed=9, extra=0)
+    full = call(s, 0.125, max_length=64)
+    check(s, 0.125, full)
+    s["lengths"] = np.asarray([2**31 - 1, 48, -7], np.int32)
+    got = call(s, 0.125)
+    s["lengths"] = np.asarray([64, 48, 0], np.int32)
+    check(s, 0.125, got)
+    check(s, 0.125, call(s, 0.125, max_length=33), limit=33)
+
+
+def test_no_sequences_and_no_pages():
+    s = setup("f16", "f16", [], 4, 2, 64, 16)
+    assert call(s, 0.125)[0].shape == (0, 4, 64)
+    s = setup("f16", "f16", [0, 0], 4, 2, 64, 16, extra=0, spare=0)
+    out, lse, _ = call(s, 0.125)
+    assert torch.equal(out, torch.zeros_like(out)) and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_strides(dtype, cache):
+    """q as a slice of a wider projection at an odd element offset; a block table wider than it is read."""
+    s = setup(dtype, cache, [100, 31, 450], 6, 2, 72, 8, seed=10)
+    base = torch.zeros((3, 9, 75), dtype=s["q"].dtype)
+    base[:, 1:7, 3:75] = s["q"]
+    out, lse, w = call(s, 0.1, q=base.cuda()[:, 1:7, 3:75])
+    check(s, 0.1, (out, lse, w))
+    wide = cuda(s["table"]).repeat(1, 2)
+    from pynve.torch import nve_kv
+
+    again = nve_kv.kv_attend(cuda(s["q"]), cuda(s["k"]), cuda(s["v"]), wide[:, :s["table"].shape[1]],
+                             cuda(s["lengths"]), scale=0.1, k_scale=cuda(s["ks"]), v_scale=cuda(s["vs"]))
+    assert torch.equal(again.cpu(), out)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_the_same_every_time(dtype, cache):
+    s = setup(dtype, cache, [3000, 20, 9000], 8, 2, 128, 16, seed=13)
+    a, b = call(s, 0.1), call(s, 0.1)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_rows_past_32_bits():
+    """Pages whose elements lie past 2^31 of the cache's start."""
+    from pynve.torch import nve_kv
+
+    heads, page, dim = 8, 16, 128
+    num_pages = 2**31 // (heads * page * dim) + 40
+    k = torch.zeros((num_pages, heads, page, dim), dtype=torch.float16, device="cuda")
+    v = torch.zeros_like(k)
+    s = setup("f16", "f16", [500], 8, heads, dim, page, seed=14)
+    n = s["k"].shape[0]
+    k[-n:], v[-n:] = s["k"].cuda(), s["v"].cuda()
+    table = cuda(s["table"])
+    table = torch.where(table >= 0, table + num_pages - n, table)
+    w = torch.zeros((num_pages, heads, page), device="cuda")
+    w[-n:] = s["weights"].cuda()
+    out, lse = nve_kv.kv_attend(cuda(s["q"]), k, v, table, cuda(s["lengths"]), scale=0.1, weights=w, return_lse=True)
+    check(s, 0.1, (out.cpu(), lse.cpu(), w[-n:].cpu()))
+
+
+def test_another_stream():
+    """Inputs made on one stream, used on another that waits for it."""
+    from pynve.torch import nve_kv
+
+    s = setup("bf16", "bf16", [4000, 900], 8, 2, 128, 16, seed=15)
+    want = call(s, 0.1)
+    side = torch.cuda.Stream()
+    args = [cuda(s[n]) for n in ("q", "k", "v", "table", "lengths")]
+    w = cuda(s["weights"])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out, lse = nve_kv.kv_attend(*args, scale=0.1, weights=w, return_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(lse.cpu(), want[1]) and torch.equal(w.cpu(), want[2])
+
+
+def test_graph_replays():
+    """Captured once, replayed over new queries and lengths, each replay against the eager call."""
+    from pynve.torch import nve_kv
+
+    s = setup("f16", "f16", [3000, 1500, 64], 8, 2, 64, 16, seed=16)
+    q, k, v, table, lengths = (cuda(s[n]) for n in ("q", "k", "v", "table", "lengths"))
+    w = torch.zeros(s["weights"].shape, device="cuda")
+    nve_kv.kv_attend(q, k, v, table, lengths, scale=0.125, weights=w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = nve_kv.kv_attend(q, k, v, table, lengths, scale=0.125, weights=w)
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, device="cuda"))
+        lengths.copy_(torch.tensor([3000 - 700 * i, 1500 - i, 16 * i], dtype=torch.int32))
+        w.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        w2 = torch.zeros_like(w)
+        want = nve_kv.kv_attend(q, k, v, table, lengths, scale=0.125, weights=w2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(w, w2)
+
+
+def test_refusals():
+    from pynve.torch import nve_kv
+
+    s = setup("f16", "f16", [20, 5], 4, 2, 64, 16)
+    base = {n: cuda(s[n]) for n in ("q", "k", "v", "table", "lengths")}
+
+    def run(**change):
+        kw = {n: change.pop(n) for n in ("k_scale", "v_scale", "weights", "max_length", "scale") if n in change}
+        a = {**base, **change}
+        return nve_kv.kv_attend(a["q"], a["k"], a["v"], a["table"], a["lengths"], **kw)
+
+    run()
+    bad_values = [{"q": base["q"][:, :3]}, {"q": base["q"][:1]}, {"q": base["q"][..., :56]}, {"q": base["q"][0]},
+                  {"q": base["q"].transpose(1, 2)}, {"q": base["q"].cpu()}, {"table": base["table"][:1]},
+                  {"table": base["table"].cpu()}, {"lengths": base["lengths"][:1]}, {"v": base["v"][:2]},
+                  {"k": base["k"].transpose(1, 2)}, {"weights": torch.zeros(3, device="cuda")}, {"max_length": -1},
+                  {"scale": math.nan}, {"k_scale": cuda(s["weights"]), "v_scale": cuda(s["weights"])},
+                  {"k": base["k"][:, :, :4].contiguous(), "v": base["v"][:, :, :4].contiguous()},
+                  {"k": base["k"][:, :, :12].contiguous(), "v": base["v"][:, :, :12].contiguous()},
+                  {"k": base["k"][..., :60].contiguous(), "v": base["v"][..., :60].contiguous(), "q": base["q"][..., :60]},
+                  {"k": base["k"].to(torch.float8_e4m3fn), "v": base["v"].to(torch.float8_e4m3fn)},
+                  {"q": base["q"].float()}]
+    for change in bad_values:
+        with pytest.raises(ValueError):
+            run(**change)
+    for change in [{"table": base["table"].long()}, {"lengths": base["lengths"].long()}, {"q": base["q"].double()},
+                   {"k": base["k"].float()}, {"weights": cuda(s["weights"]).half()}]:
+        with pytest.raises((TypeError, ValueError)):
+            run(**change)
+    with pytest.raises(RuntimeError, match="gradient"):
+        run(q=base["q"].clone().requires_grad_())
+    with torch.no_grad():
+        run(q=base["q"].clone().requires_grad_())
