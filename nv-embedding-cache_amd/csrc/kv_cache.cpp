@@ -39,6 +39,8 @@ KvPages pages_of(const nve_amd_kv_pages_t* p) {
   } else {
     NVE_CHECK_ARG(!p->k_scale && !p->v_scale, "only e4m3 pages have scales");
   }
+  NVE_CHECK_ARG((int64_t)p->num_heads * p->page_size * p->head_dim * value_elem_bytes(dt) <= kMaxGrid,
+                "a page of all heads must be smaller than 2 GiB");
   KvPages c{};
   c.k = static_cast<uint8_t*>(p->k);
   c.v = static_cast<uint8_t*>(p->v);
