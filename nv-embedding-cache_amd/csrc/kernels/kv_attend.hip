@@ -52,119 +52,110 @@ using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
-constexpr int kThreads = 256;
-constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // f32 has 4 slots per lane and step, the other types 8.
 constexpr int step_slots(int qt) { return qt == kF32 ? 16 : 32; }
-constexpr int tile_slots(int qt) { return kWaves * step_slots(qt); }
 
 // ---------------------------------------------------------------------------
-// the workgroups' shares
+// the workgroups' tiles
 // ---------------------------------------------------------------------------
+// A unit is a (sequence, key head); a piece a run of its tiles in one workgroup.
 struct Plan {
-  int64_t units_per_seq;  // key heads * query tiles
   int32_t query_tiles, group, tile;
-  int64_t padded;   // slots of a row of scores
-  float* scores;    // [seqs * q_heads, padded], log2 units (accumulate)
-  float* sums;      // [units, 16]: log2 of the softmax's sum (accumulate)
-  float* slot_ml;   // [2 * workgroups, 2, 16]
-  float* slot_rows; // [2 * workgroups, 16, dim padded]
+  int32_t chunk, pieces;  // grid mode: tiles of a piece, pieces of a unit at most
+  int32_t workgroups;     // stream mode
+  int64_t padded;         // slots of a row of scores
+  float* scores;          // [seqs * q_heads, padded], log2 units (accumulate)
+  float* slot_ml;         // [slots, query_tiles, 2, 16]
+  float* slot_rows;       // [slots, query_tiles, 16, dim padded]
+  struct Slot* slots;     // [2 * workgroups] (stream mode)
 };
+
+struct Piece {
+  int seq, head, tiles;  // the unit and its number of tiles
+  int first, last;       // [first, last) of them
+  int64_t len;           // the sequence's
+};
+
+// What a stream workgroup leaves of the first and the last piece of its share.
+struct Slot {
+  int32_t valid, unit_tile, total;
+  Piece piece;
+};
+
+// The same in every lane, and so in a scalar register: what describes a share must not
+// take vector registers from the loop over its tiles.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Tiles of a sequence; one at least, so that an empty one is visited.
-__device__ __forceinline__ int64_t tiles_of(const KvAttend& a, const Plan& p, int64_t s) {
-  const int64_t n = kv_length(a.lengths, s, a.max_length);
-  return n <= p.tile ? 1 : (n + p.tile - 1) / p.tile;
+__device__ __forceinline__ int tiles_of(const Plan& p, int64_t len) {
+  return len <= p.tile ? 1 : (int)((len + p.tile - 1) / p.tile);
 }
 
-struct Share {
-  int64_t total;         // tiles of the call
-  int64_t workers;       // workgroups that have a share: no share is empty
-  int64_t begin, end;    // this workgroup's
-  int64_t seq, seq_tile; // the sequence `begin` lies in, and the call's tile where it starts
+// Stream mode: all tiles of the call, end to end, in shares that differ by one tile at most.
+struct Shares {
+  int total, workers;  // no share is empty
+  int base, more;      // the first `more` shares have base + 1 tiles
+  __device__ __forceinline__ Shares(int total, int workgroups) : total(total) {
+    workers = total < workgroups ? total : workgroups;
+    base = total / workers;
+    more = total - base * workers;
+  }
+  __device__ __forceinline__ int begin(int w) const { return w * base + (w < more ? w : more); }
+  __device__ __forceinline__ int of(int tile) const {  // the share a tile is in
+    const int long_end = more * (base + 1);
+    return tile < long_end ? tile / (base + 1) : more + (tile - long_end) / base;
+  }
 };
 
-__device__ __forceinline__ int64_t share_begin(const Share& s, int64_t w) { return w * s.total / s.workers; }
-// the workgroup that has a tile
-__device__ __forceinline__ int64_t share_of(const Share& s, int64_t tile) {
-  return ((tile + 1) * s.workers - 1) / s.total;
-}
+struct Start {
+  int total;
+  int seq, seq_tile;  // the sequence that the share starts in, and the call's tile where that starts
+};
 
-// Every thread sums a run of the sequences; a scan finds where the share starts.
-__device__ __forceinline__ Share find_share(const KvAttend& a, const Plan& p) {
-  __shared__ int64_t wave_total[kWaves];
-  __shared__ int64_t found[2];
+// Every thread sums a run of the sequences; a scan finds where this workgroup's share starts.
+__device__ __forceinline__ Start find_start(const KvAttend& a, const Plan& p) {
+  __shared__ int wave_total[4];
+  __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t per = (a.seqs + kThreads - 1) / kThreads;
-  const int64_t s0 = per * tid < a.seqs ? per * tid : a.seqs;
-  const int64_t s1 = s0 + per < a.seqs ? s0 + per : a.seqs;
-  int64_t own = 0;
-  for (int64_t s = s0; s < s1; ++s) own += tiles_of(a, p, s);
-  int64_t scan = own;
+  const int seqs = (int)a.seqs, per = (seqs + 255) / 256;
+  const int s0 = min(per * tid, seqs), s1 = min(s0 + per, seqs);
+  int own = 0;
+  for (int s = s0; s < s1; ++s) own += tiles_of(p, kv_length(a.lengths, s, a.max_length));
+  int scan = own;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(scan, d);
+    const int o = __shfl_up(scan, d);
     if (lane >= d) scan += o;
   }
   if (lane == 63) wave_total[wave] = scan;
   __syncthreads();
-  int64_t total = 0;
+  int total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < 4; ++w) {
     if (w < wave) scan += wave_total[w];
     total += wave_total[w];
   }
-  Share r;
-  r.total = total * p.units_per_seq;
-  r.workers = r.total < gridDim.x ? r.total : gridDim.x;
-  if (blockIdx.x >= r.workers) {
-    r.begin = r.end = r.total;
-    return r;
-  }
-  r.begin = share_begin(r, blockIdx.x);
-  r.end = share_begin(r, (int64_t)blockIdx.x + 1);
-  int64_t at = (scan - own) * p.units_per_seq;
-  if (r.begin >= at && r.begin < scan * p.units_per_seq) {
-    int64_t s = s0;
-    for (; s < s1; ++s) {
-      const int64_t n = tiles_of(a, p, s) * p.units_per_seq;
-      if (r.begin < at + n) break;
+  Start r;
+  r.total = uniform(total * a.pages.heads);
+  const Shares shares(r.total, p.workgroups);
+  const int begin = (int)blockIdx.x < shares.workers ? shares.begin(blockIdx.x) : r.total;
+  int at = (scan - own) * a.pages.heads;
+  if (begin >= at && begin < scan * a.pages.heads) {
+    int s = s0;
+    for (; s + 1 < s1; ++s) {
+      const int n = tiles_of(p, kv_length(a.lengths, s, a.max_length)) * a.pages.heads;
+      if (begin < at + n) break;
       at += n;
     }
     found[0] = s;
     found[1] = at;
   }
   __syncthreads();
-  r.seq = found[0];
-  r.seq_tile = found[1];
-  return r;
-}
-
-// A run of one unit's tiles in a workgroup's share.
-struct Piece {
-  int64_t seq, len, tiles;  // the unit's
-  int64_t unit_tile;        // the call's tile where the unit starts
-  int64_t first, last;      // [first, last) of the unit's tiles
-  int64_t unit;
-  int head, query_tile;
-};
-
-__device__ __forceinline__ Piece piece_at(const KvAttend& a, const Plan& p, int64_t tile, int64_t end, int64_t seq,
-                                          int64_t seq_tile) {
-  Piece r;
-  r.seq = seq;
-  r.len = kv_length(a.lengths, seq, a.max_length);
-  r.tiles = r.len <= p.tile ? 1 : (r.len + p.tile - 1) / p.tile;
-  const int64_t u = (tile - seq_tile) / r.tiles;
-  r.unit = seq * p.units_per_seq + u;
-  r.head = (int)(u / p.query_tiles);
-  r.query_tile = (int)(u - (int64_t)r.head * p.query_tiles);
-  r.unit_tile = seq_tile + u * r.tiles;
-  r.first = tile - r.unit_tile;
-  r.last = end - r.unit_tile < r.tiles ? end - r.unit_tile : r.tiles;
+  r.seq = uniform(found[0]);
+  r.seq_tile = uniform(found[1]);
   return r;
 }
 
@@ -223,29 +214,48 @@ __device__ __forceinline__ float high_of(uint32_t w) {
 }
 
 // Two e4m3 codes (the low or high half of w) widened exactly.
-template <int QT, bool HIGH>
-__device__ __forceinline__ uint32_t widen2(uint32_t w) {
-  const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, HIGH);
+template <int QT>
+__device__ __forceinline__ uint32_t widen2(uint32_t w, bool high) {
+  const auto x = high ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
   return pack2<QT>(x[0], x[1]);
 }
 
-// 8 or 16 bytes of a row (any 4-byte alignment).
-template <int WORDS>
-__device__ __forceinline__ void load_words(uint32_t* dst, const uint8_t* src) {
-  using gwords = const __attribute__((address_space(1))) uint32_t*;
-  gwords p = (gwords)(uintptr_t)src;
-  if constexpr (WORDS == 4) {
-    typedef u32x4 __attribute__((aligned(4))) u4;
-    const u32x4 x = *(const __attribute__((address_space(1))) u4*)p;
+// 4 to 16 bytes of a row (any 4-byte alignment).
+template <int N>
+using words = __attribute__((ext_vector_type(N))) uint32_t;
+
+template <int N>
+__device__ __forceinline__ words<N> load_words(const uint8_t* src) {
+  typedef words<N> __attribute__((aligned(4))) any;
+  return *(const __attribute__((address_space(1))) any*)(uintptr_t)src;
+}
+
+// The weights of a piece's slots under `rows` softmaxes whose sums are all[]; four slots a
+// thread, which lie in one page.
+__device__ __forceinline__ void add_weights(const KvAttend& a, const Plan& p, const Piece& u, int query_tile,
+                                            const float* all) {
+  typedef f32x4 __attribute__((aligned(4))) f4;
+  const int64_t t1 = min((int64_t)u.last * p.tile, u.len);
+  const int rows = min(16, p.group - query_tile * 16);
+  const float* scores =
+      p.scores + (u.seq * (int64_t)a.q_heads + (int64_t)u.head * p.group + query_tile * 16) * p.padded;
+  for (int64_t t = (int64_t)u.first * p.tile + 4 * threadIdx.x; t < t1; t += 4 * 256) {
+    const int64_t page = kv_page(a.pages, a.tables + u.seq * a.table_stride, t);
+    if (page < 0) continue;
+    float* to = a.pages.weights + kv_row(a.pages, page, u.head, t);
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int q = 0; q < rows; ++q) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(scores + q * p.padded + t);
+      const float y = all[q] == -INFINITY ? INFINITY : all[q];  // an empty softmax has no weights
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dst[i] = x[i];
-  } else if constexpr (WORDS == 2) {
-    typedef uint64_t __attribute__((aligned(4))) u2;
-    const uint64_t x = *(const __attribute__((address_space(1))) u2*)p;
-    dst[0] = (uint32_t)x;
-    dst[1] = (uint32_t)(x >> 32);
-  } else {
-    dst[0] = *p;
+      for (int i = 0; i < 4; ++i) sum[i] += exp2_of(x[i] - y);
+    }
+    if (t + 4 <= t1) {
+      *reinterpret_cast<f4*>(to) += sum;
+    } else {
+      for (int i = 0; i < (int)(t1 - t); ++i) to[i] += sum[i];
+    }
   }
 }
 
@@ -266,9 +276,12 @@ struct Wave {
   static constexpr int VT = CT == kE4M3 ? kBF16 : QT;  // the type of the second product
   static constexpr int kQWords = QT == kF32 ? DP / 4 : kSteps * 4;
 
-  uint32_t q[kQWords];
-  uint32_t k[kTiles][kPieces * 4];
-  uint32_t v[kSlots][kVWords];
+  static constexpr int kVLoad = !EXACT && CT == kE4M3 ? (kVWords < 2 ? 1 : 2) : kVWords < 4 ? kVWords : 4;
+
+  u32x4 q[kQWords / 4];
+  u32x4 k[kTiles][kPieces];
+  words<kVLoad> v[kSlots][kVWords / kVLoad];
+  f32x4 k_scale[kTiles], v_scale[kTiles];  // e4m3: of this lane's slots
   f32x4 acc[kValues];
   float m, l;  // m: of the query; l: of this lane's slots
 
@@ -280,51 +293,45 @@ struct Wave {
     return step * 32 + g * 8 + i;
   }
 
+  // Queries may start at any element: 16-byte loads of the type's alignment.
   __device__ __forceinline__ void load_queries(const KvAttend& a, int64_t row_offset, bool there, int g) {
+    constexpr int kElem = QT == kF32 ? 4 : 2;
+    typedef u32x4 __attribute__((aligned(2))) any4;
     const int dim = a.pages.dim;
 #pragma unroll
-    for (int w = 0; w < kQWords; ++w) {
+    for (int w = 0; w < kQWords; w += 4) {
       const int d = q_value(w, g);
-      q[w] = 0;
-      if (!there || (!EXACT && d >= dim)) continue;
-      if constexpr (QT == kF32) {
-        q[w] = reinterpret_cast<const uint32_t*>(a.q.p)[row_offset + d];
-      } else {
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q.p) + row_offset + d;
-        q[w] = p[0] | (uint32_t)p[1] << 16;
-      }
+      q[w / 4] = u32x4{0, 0, 0, 0};
+      if (there && (EXACT || d < dim)) q[w / 4] = *reinterpret_cast<const any4*>(a.q.p + (row_offset + d) * kElem);
     }
   }
 
   // A k row's pieces: 16 bytes at 64 i + 16 g.
-  static __device__ __forceinline__ void load_k(uint32_t (&r)[kPieces * 4], const uint8_t* row, int g, int dim) {
+  static __device__ __forceinline__ void load_k(u32x4 (&r)[kPieces], const uint8_t* row, int g, int dim) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int b = i * 64 + g * 16;
       if constexpr (EXACT) {
-        load_words<4>(&r[4 * i], row + b);
+        r[i] = load_words<4>(row + b);
       } else if constexpr (CT == kE4M3) {  // head_dim is a multiple of 8: half a piece
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          r[4 * i + 2 * h] = r[4 * i + 2 * h + 1] = 0;
-          if (b + 8 * h < dim) load_words<2>(&r[4 * i + 2 * h], row + b + 8 * h);
-        }
+        words<2> low = {0, 0}, high = {0, 0};
+        if (b < dim) low = load_words<2>(row + b);
+        if (b + 8 < dim) high = load_words<2>(row + b + 8);
+        r[i] = u32x4{low[0], low[1], high[0], high[1]};
       } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[4 * i + j] = 0;
-        if (b < dim * kBytes) load_words<4>(&r[4 * i], row + b);
+        r[i] = u32x4{0, 0, 0, 0};
+        if (b < dim * kBytes) r[i] = load_words<4>(row + b);
       }
     }
   }
 
   // A v row's values kValues c ..; those past head_dim are not used (the row's first instead).
-  static __device__ __forceinline__ void load_v(uint32_t (&r)[kVWords], const uint8_t* row, int c, int dim) {
+  static __device__ __forceinline__ void load_v(words<kVLoad> (&r)[kVWords / kVLoad], const uint8_t* row, int c, int dim) {
     const int b = c * kValues * kBytes;
-    constexpr int kLoad = EXACT ? (kVWords < 4 ? kVWords : 4) : CT == kE4M3 ? (kVWords < 2 ? 1 : 2) : (kVWords < 4 ? kVWords : 4);
 #pragma unroll
-    for (int i = 0; i < kVWords; i += kLoad) {
-      const int at = b + 4 * i;
-      load_words<kLoad>(&r[i], row + (EXACT || at < dim * kBytes ? at : 0));
+    for (int i = 0; i < kVWords / kVLoad; ++i) {
+      const int at = b + 4 * kVLoad * i;
+      r[i] = load_words<kVLoad>(row + (EXACT || at < dim * kBytes ? at : 0));
     }
   }
 
@@ -333,19 +340,19 @@ struct Wave {
     if constexpr (QT == kF32) {
 #pragma unroll
       for (int w = 0; w < DP / 4; ++w)
-        s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[tile][w]), __uint_as_float(q[w]), s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[tile][w / 4][w % 4]), __uint_as_float(q[w / 4][w % 4]), s,
+                                                  0, 0, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        const u32x4 b = {q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]};
         u32x4 x;
         if constexpr (CT == kE4M3) {
-          const uint32_t w0 = k[tile][2 * i], w1 = k[tile][2 * i + 1];
-          x = u32x4{widen2<QT, false>(w0), widen2<QT, true>(w0), widen2<QT, false>(w1), widen2<QT, true>(w1)};
+          const uint32_t w0 = k[tile][i / 2][i % 2 * 2], w1 = k[tile][i / 2][i % 2 * 2 + 1];
+          x = u32x4{widen2<QT>(w0, false), widen2<QT>(w0, true), widen2<QT>(w1, false), widen2<QT>(w1, true)};
         } else {
-          x = u32x4{k[tile][4 * i], k[tile][4 * i + 1], k[tile][4 * i + 2], k[tile][4 * i + 3]};
+          x = k[tile][i];
         }
-        s = mma<QT>(x, b, s);
+        s = mma<QT>(x, q[i], s);
       }
     }
     return s;
@@ -358,7 +365,7 @@ struct Wave {
       for (int j = 0; j < kValues; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j]), p[r], acc[j], 0, 0, 0);
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j / kVLoad][j % kVLoad]), p[r], acc[j], 0, 0, 0);
     } else {
       u32x4 high, low;
 #pragma unroll
@@ -372,9 +379,9 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < kValues / 2; ++i) {
           if constexpr (CT == kE4M3)
-            w[r][i] = (i & 1) ? widen2<VT, true>(v[r][i / 2]) : widen2<VT, false>(v[r][i / 2]);
+            w[r][i] = widen2<VT>(v[r][i / 2 / kVLoad][i / 2 % kVLoad], i & 1);
           else
-            w[r][i] = v[r][i];
+            w[r][i] = v[r][i / kVLoad][i % kVLoad];
         }
 #pragma unroll
       for (int j = 0; j < kValues; ++j) {
@@ -389,29 +396,31 @@ struct Wave {
   }
 };
 
-template <int QT, int CT, int DP, bool EXACT, bool ACC>
-__global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, const Plan p) {
+// Waves of a SIMD (and workgroups of a CU) that the kernel is built for and stream mode fills.
+constexpr int waves_per_simd(int dp) { return dp == 64 ? 3 : dp == 128 ? 2 : 1; }
+
+template <int QT, int CT, int DP, bool EXACT, bool ACC, bool GRID>
+__global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(const KvAttend a, const Plan p) {
   using W = Wave<QT, CT, DP, EXACT>;
   using T = kv_elem<QT>;
-  constexpr int kStep = W::kStep, kValues = W::kValues;
-  constexpr int kPass = kValues < 8 ? kValues : 8;  // output tiles joined at a time
-  constexpr int kRow = 16 * kPass + 4;              // a query's values in shared memory, padded
+  constexpr int kWaves = 4, kStep = W::kStep, kValues = W::kValues;
+  constexpr int kPass = 4;            // output tiles joined at a time
+  constexpr int kRow = 16 * kPass + 4;  // a query's values in shared memory, padded
   __shared__ float wave_ml[kWaves][2][16];
   __shared__ float rows[kWaves][16 * kRow];
+  __shared__ float all[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
   const KvPages& pages = a.pages;
   const int dim = EXACT ? DP : pages.dim;
   const int row_bytes = dim * W::kBytes, mask = pages.page - 1;
   const uint64_t page_bytes = (uint64_t)pages.heads * pages.page * row_bytes;
   const float to_log2 = a.scale * kLog2e;
-  const Share share = find_share(a, p);
-  int64_t seq = share.seq, seq_tile = share.seq_tile;
   W x;
 
-  for (int64_t tile = share.begin; tile < share.end;) {
-    const Piece u = piece_at(a, p, tile, share.end, seq, seq_tile);
-    const int rows_here = min(16, p.group - u.query_tile * 16);
-    const int64_t q_head = (int64_t)u.head * p.group + u.query_tile * 16 + c;
+  // One piece and 16 of its queries; the slot is where it goes if the unit has others.
+  auto process = [&](const Piece& u, int query_tile, int slot) {
+    const int rows_here = min(16, p.group - query_tile * 16);
+    const int64_t q_head = (int64_t)u.head * p.group + query_tile * 16 + c;
     const bool there = c < rows_here;
     x.load_queries(a, u.seq * a.q.token_stride + q_head * a.q.head_stride, there, g);
 #pragma unroll
@@ -420,8 +429,8 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
     x.l = 0.0f;
 
     const int32_t* table = a.tables + u.seq * a.table_stride;
-    const int steps = (int)(u.last - u.first);
-    const int64_t t_base = u.first * (kWaves * kStep) + wave * kStep;  // this wave's first slot
+    const int steps = u.last - u.first;
+    const int64_t t_base = (int64_t)u.first * (kWaves * kStep) + wave * kStep;  // this wave's first slot
     // Page numbers of 16 steps: lane 4 i + b has that of slots 8 b .. of step i (-1: absent).
     int ids = -1;
     auto load_ids = [&](int step) {
@@ -436,6 +445,10 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
       const uint32_t in_page = (uint32_t)(u.head * pages.page + ((int)t & mask)) * (uint32_t)row_bytes;
       return base + (uint64_t)(uint32_t)max(id, 0) * page_bytes + in_page;
     };
+    auto scale_at = [&](const float* base, int id, int64_t t) {
+      typedef f32x4 __attribute__((aligned(4))) f4;
+      return *reinterpret_cast<const f4*>(base + ((int64_t)max(id, 0) * pages.heads + u.head) * pages.page + (t & mask));
+    };
     // Slots without a row read the first page's instead; their scores and values are dropped below.
     auto load_k = [&](int step) {
       const int64_t t0 = t_base + (int64_t)step * (kWaves * kStep);
@@ -443,6 +456,10 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
       for (int n = 0; n < W::kTiles; ++n) {
         const int id = __shfl(ids, (step & 15) * 4 + n * 2 + (c >> 3));
         W::load_k(x.k[n], row_at(pages.k, id, t0 + n * 16 + c), g, dim);
+        if constexpr (CT == kE4M3) {
+          const int of = __shfl(ids, (step & 15) * 4 + n * 2 + (g >> 1));
+          x.k_scale[n] = scale_at(pages.k_scale, of, t0 + n * 16 + g * 4);
+        }
       }
     };
     auto load_v = [&](int step) {
@@ -450,9 +467,11 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
 #pragma unroll
       for (int n = 0; n < W::kTiles; ++n) {
         const int id = __shfl(ids, (step & 15) * 4 + n * 2 + (g >> 1));
-        const uint8_t* row = row_at(pages.v, id, t0 + n * 16 + g * 4);
+        const int64_t t = t0 + n * 16 + g * 4;
+        const uint8_t* row = row_at(pages.v, id, t);
 #pragma unroll
         for (int r = 0; r < 4; ++r) W::load_v(x.v[n * 4 + r], row + r * row_bytes, c, dim);
+        if constexpr (CT == kE4M3) x.v_scale[n] = scale_at(pages.v_scale, id, t);
       }
     };
 
@@ -467,37 +486,26 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
       // the four page numbers of this step, -1 where a slot has no row
       const uint64_t absent = __ballot(ids < 0) >> ((step & 15) * 4);
       const bool full = t0 + kStep <= u.len && (absent & (kStep == 32 ? 15 : 3)) == 0;
-      float scale_v[W::kSlots];
       float y[W::kSlots];
 #pragma unroll
       for (int n = 0; n < W::kTiles; ++n) {
         const int id = __shfl(ids, (step & 15) * 4 + n * 2 + (g >> 1));
         const int64_t t = t0 + n * 16 + g * 4;
-        f32x4 ks = {1.0f, 1.0f, 1.0f, 1.0f}, vs = ks;
-        if constexpr (CT == kE4M3) {
-          const int64_t at = ((int64_t)max(id, 0) * pages.heads + u.head) * pages.page + (t & mask);
-          typedef f32x4 __attribute__((aligned(4))) f4;
-          ks = *reinterpret_cast<const f4*>(pages.k_scale + at);
-          vs = *reinterpret_cast<const f4*>(pages.v_scale + at);
-        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           y[n * 4 + r] = s[n][r] * to_log2;
-          scale_v[n * 4 + r] = 1.0f;
-          if constexpr (CT == kE4M3) {
-            y[n * 4 + r] *= ks[r];
-            scale_v[n * 4 + r] = vs[r];
-          }
+          if constexpr (CT == kE4M3) y[n * 4 + r] *= x.k_scale[n][r];
         }
         if (!full) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (id < 0 || t + r >= u.len) {
-              y[n * 4 + r] = -INFINITY;
-              scale_v[n * 4 + r] = 0.0f;
+          for (int r = 0; r < 4; ++r) {
+            const bool row = id >= 0 && t + r < u.len;
+            const uint32_t keep = row ? 0xffffffffu : 0u;
+            y[n * 4 + r] = row ? y[n * 4 + r] : -INFINITY;
+            if constexpr (CT == kE4M3) x.v_scale[n][r] = row ? x.v_scale[n][r] : 0.0f;
 #pragma unroll
-              for (int w = 0; w < W::kVWords; ++w) x.v[n * 4 + r][w] = 0;
-            }
+            for (int w = 0; w < W::kVWords / W::kVLoad; ++w) x.v[n * 4 + r][w] &= keep;
+          }
         }
         if constexpr (ACC) {
           if (there && t < u.len)  // rows of scores are padded to whole tiles
@@ -526,7 +534,7 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
       for (int i = 0; i < W::kSlots; ++i) {
         w[i] = exp2_of(y[i] - base);
         x.l += w[i];
-        if constexpr (CT == kE4M3) w[i] *= scale_v[i];
+        if constexpr (CT == kE4M3) w[i] *= x.v_scale[i / 4][i % 4];
       }
       x.add_values(w);
       if (more) load_v(step + 1);
@@ -539,9 +547,9 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
       wave_ml[wave][1][c] = l;
     }
     const bool whole = u.first == 0 && u.last == u.tiles;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (tile == share.begin ? 0 : 1);
     const int q = tid >> 4, r = tid & 15;  // a query, and the output rows r of the tiles
-    const int64_t out_head = (int64_t)u.head * p.group + u.query_tile * 16 + q;
+    const int64_t out_head = (int64_t)u.head * p.group + query_tile * 16 + q;
+    const int64_t at = (int64_t)slot * p.query_tiles + query_tile;
 #pragma unroll
     for (int pass = 0; pass < kValues / kPass; ++pass) {
       if (pass > 0) __syncthreads();
@@ -576,27 +584,65 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
           for (int j = 0; j < kPass; ++j)
             if (EXACT || d0 + j < dim) out[d0 + j] = (T)(sum == 0.0f ? 0.0f : o[j] / sum);
           if (r == 0 && pass == 0) {
-            const float all = sum == 0.0f ? -INFINITY : top - kShift + __builtin_amdgcn_logf(sum);
-            if (a.lse) a.lse[u.seq * a.q_heads + out_head] = all * kLn2;
-            if constexpr (ACC) p.sums[u.unit * 16 + q] = all;
+            const float log_sum = sum == 0.0f ? -INFINITY : top - kShift + __builtin_amdgcn_logf(sum);
+            if (a.lse) a.lse[u.seq * a.q_heads + out_head] = log_sum * kLn2;
+            all[q] = log_sum;
           }
         } else {
-          float* to = p.slot_rows + (slot * 16 + q) * DP + d0;
+          float* to = p.slot_rows + (at * 16 + q) * DP + d0;
 #pragma unroll
           for (int j = 0; j < kPass; ++j) to[j] = o[j];
           if (r == 0 && pass == 0) {
-            p.slot_ml[slot * 32 + q] = top == -INFINITY ? top : top - kShift;
-            p.slot_ml[slot * 32 + 16 + q] = sum;
+            p.slot_ml[at * 32 + q] = top == -INFINITY ? top : top - kShift;
+            p.slot_ml[at * 32 + 16 + q] = sum;
           }
         }
       }
     }
+    if (ACC && whole) {
+      __threadfence_block();  // the other waves' scores
+      __syncthreads();
+      add_weights(a, p, u, query_tile, all);
+    }
     __syncthreads();  // the shared rows are free again
+  };
 
-    tile = u.unit_tile + u.last;
-    if (tile == seq_tile + u.tiles * p.units_per_seq) {
-      seq_tile = tile;
-      ++seq;
+  if constexpr (GRID) {
+    const int unit = blockIdx.y;
+    Piece u;
+    u.seq = unit / pages.heads;
+    u.head = unit - u.seq * pages.heads;
+    u.len = kv_length(a.lengths, u.seq, a.max_length);
+    u.tiles = tiles_of(p, u.len);
+    u.first = blockIdx.x * p.chunk;
+    u.last = min(u.first + p.chunk, u.tiles);
+    if (u.first >= u.tiles) return;
+    for (int qt = 0; qt < p.query_tiles; ++qt) process(u, qt, unit * p.pieces + blockIdx.x);
+  } else {
+    const Start start = find_start(a, p);
+    const Shares shares(start.total, p.workgroups);
+    const int w = blockIdx.x;
+    if (tid == 0) p.slots[2 * w].valid = p.slots[2 * w + 1].valid = 0;
+    if (w >= shares.workers) return;
+    const int begin = shares.begin(w), end = shares.begin(w + 1);
+    int seq = start.seq, seq_tile = start.seq_tile;
+    for (int tile = begin; tile < end;) {
+      Piece u;
+      u.seq = seq;
+      u.len = kv_length(a.lengths, seq, a.max_length);
+      u.tiles = tiles_of(p, u.len);
+      u.head = (tile - seq_tile) / u.tiles;
+      const int unit_tile = seq_tile + u.head * u.tiles;
+      u.first = tile - unit_tile;
+      u.last = min(end - unit_tile, u.tiles);
+      const int slot = 2 * w + (tile == begin ? 0 : 1);
+      if (tid == 0 && !(u.first == 0 && u.last == u.tiles)) p.slots[slot] = Slot{1, unit_tile, start.total, u};
+      for (int qt = 0; qt < p.query_tiles; ++qt) process(u, qt, slot);
+      tile = unit_tile + u.last;
+      if (tile == seq_tile + u.tiles * pages.heads) {
+        seq_tile = tile;
+        ++seq;
+      }
     }
   }
 }
@@ -604,124 +650,129 @@ __global__ __launch_bounds__(kThreads) void kv_attend_kernel(const KvAttend a, c
 // ---------------------------------------------------------------------------
 // the second kernel: joins the pieces of units, adds the attention weights
 // ---------------------------------------------------------------------------
+// A unit's pieces: in grid mode slots in a row, in stream mode the slots of the workgroups
+// that have its tiles (the first one's `head`, then each one's first).
 struct Pieces {
-  int64_t first, last;  // workgroups that have tiles of the unit
-  int64_t first_slot;   // of the first one; the others' is their first
-  __device__ __forceinline__ int64_t slot(int64_t w) const { return w == first ? first_slot : 2 * w; }
+  int count, head, next, step;
+  __device__ __forceinline__ int slot(int i) const { return i == 0 ? head : next + (i - 1) * step; }
 };
 
-__device__ __forceinline__ Pieces pieces_of(const Share& share, int64_t unit_tile, int64_t tiles) {
-  Pieces r;
-  r.first = share_of(share, unit_tile);
-  r.last = share_of(share, unit_tile + tiles - 1);
-  r.first_slot = 2 * r.first + (share_begin(share, r.first) == unit_tile ? 0 : 1);
-  return r;
+// The largest m of a unit's pieces, and log2 of the sum over all of them, for 16 queries.
+__device__ __forceinline__ void total_of(const Plan& p, const Pieces& w, int query_tile, float* tops, float* all) {
+  constexpr int kAhead = 8;
+  const int q = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  float top = -INFINITY, sum = 0.0f;
+  for (int i0 = lane; i0 < w.count; i0 += 16 * kAhead) {
+    float m[kAhead], l[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + 16 * j;
+      m[j] = -INFINITY;
+      l[j] = 0.0f;
+      if (i < w.count) {
+        const float* ml = p.slot_ml + ((int64_t)w.slot(i) * p.query_tiles + query_tile) * 32 + q;
+        m[j] = ml[0];
+        l[j] = ml[16];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float t = fmaxf(top, m[j]);
+      sum = sum * rescale(top, t) + l[j] * rescale(m[j], t);
+      top = t;
+    }
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) {
+    const float m = __shfl_xor(top, d), l = __shfl_xor(sum, d);
+    const float t = fmaxf(top, m);
+    sum = sum * rescale(top, t) + l * rescale(m, t);
+    top = t;
+  }
+  __syncthreads();
+  if (lane == 0) {
+    tops[q] = top;
+    all[q] = sum == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
+  }
+  __syncthreads();
 }
 
-template <int QT, int DP, bool ACC>
-__global__ __launch_bounds__(kThreads) void kv_join_kernel(const KvAttend a, const Plan p) {
+constexpr int kJoinValues = 64;  // output values a joining workgroup has at least
+
+template <int QT, int DP, bool ACC, bool GRID>
+__global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend a, const Plan p) {
   using T = kv_elem<QT>;
-  __shared__ float part[kThreads];
+  __shared__ float part[256];
   __shared__ float tops[16], all[16];
-  const int tid = threadIdx.x;
-  const KvPages& pages = a.pages;
-  const int dim = pages.dim;
-  const Share share = find_share(a, p);
-  int64_t seq = share.seq, seq_tile = share.seq_tile;
-  for (int64_t tile = share.begin; tile < share.end;) {
-    const Piece u = piece_at(a, p, tile, share.end, seq, seq_tile);
-    // m and log2 of the sum of all pieces of a unit of this sequence and head
-    auto totals = [&](int query_tile, const Pieces& w) {
-      const int q = tid >> 4, i0 = tid & 15;
-      float top = -INFINITY;
-      for (int64_t i = w.first + i0; i <= w.last; i += 16) top = fmaxf(top, p.slot_ml[w.slot(i) * 32 + q]);
-#pragma unroll
-      for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-      float sum = 0.0f;
-      for (int64_t i = w.first + i0; i <= w.last; i += 16)
-        sum += p.slot_ml[w.slot(i) * 32 + 16 + q] * rescale(p.slot_ml[w.slot(i) * 32 + q], top);
-#pragma unroll
-      for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-      __syncthreads();
-      if (i0 == 0) {
-        tops[q] = top;
-        all[q] = sum == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
-      }
-      __syncthreads();
-    };
-    if (u.first != 0 || u.last != u.tiles) {
-      const Pieces w = pieces_of(share, u.unit_tile, u.tiles);
-      const int n = (int)(w.last - w.first + 1), me = (int)(blockIdx.x - w.first);
-      const int rows_here = min(16, p.group - u.query_tile * 16);
-      totals(u.query_tile, w);
-      // this workgroup's run of the unit's output values
-      const int e0 = (int)((int64_t)me * rows_here * dim / n), e1 = (int)((int64_t)(me + 1) * rows_here * dim / n);
-      for (int e = e0; e < e1; e += kThreads) {
-        const int width = min(e1 - e, kThreads), ways = kThreads / width;
-        const int way = tid / width, mine = e + tid - way * width;
-        float o = 0.0f;
-        if (way < ways) {
-          const int q = mine / dim, d = mine - q * dim;
-          for (int64_t i = w.first + way; i <= w.last; i += ways)
-            o += p.slot_rows[(w.slot(i) * 16 + q) * DP + d] * rescale(p.slot_ml[w.slot(i) * 32 + q], tops[q]);
-        }
-        __syncthreads();
-        part[tid] = o;
-        __syncthreads();
-        if (way == 0) {
-          for (int i = 1; i < ways; ++i) o += part[i * width + tid];
-          const int q = mine / dim, d = mine - q * dim;
-          const int64_t head = (int64_t)u.head * p.group + u.query_tile * 16 + q;
-          const float sum = all[q] == -INFINITY ? 0.0f : exp2_of(tops[q] - all[q]);
-          reinterpret_cast<T*>(a.out)[u.seq * a.out_seq_stride + head * a.out_head_stride + d] = (T)(o * sum);
+  const int tid = threadIdx.x, dim = a.pages.dim;
+  Piece u;
+  Pieces w;
+  int me;  // which of the unit's pieces this is
+  if constexpr (GRID) {
+    const int unit = blockIdx.y;
+    u.seq = unit / a.pages.heads;
+    u.head = unit - u.seq * a.pages.heads;
+    u.len = kv_length(a.lengths, u.seq, a.max_length);
+    u.tiles = tiles_of(p, u.len);
+    me = blockIdx.x;
+    u.first = me * p.chunk;
+    u.last = min(u.first + p.chunk, u.tiles);
+    w.count = (u.tiles + p.chunk - 1) / p.chunk;
+    w.head = unit * p.pieces;
+    w.next = w.head + 1;
+    w.step = 1;
+    if (w.count == 1 || me >= w.count) return;
+  } else {
+    const Slot s = p.slots[blockIdx.x];
+    if (!s.valid) return;
+    u = s.piece;
+    const Shares shares(s.total, p.workgroups);
+    const int first = shares.of(s.unit_tile), last = shares.of(s.unit_tile + u.tiles - 1);
+    me = (int)blockIdx.x / 2 - first;
+    w.count = last - first + 1;
+    w.head = 2 * first + (shares.begin(first) == s.unit_tile ? 0 : 1);
+    w.next = 2 * (first + 1);
+    w.step = 2;
+  }
+  for (int qt = 0; qt < p.query_tiles; ++qt) {
+    // a run of the output values
+    const int rows_here = min(16, p.group - qt * 16), values = rows_here * dim;
+    const int n = min(w.count, (values + kJoinValues - 1) / kJoinValues);
+    if (!ACC && me >= n) continue;
+    total_of(p, w, qt, tops, all);
+    const int e0 = me < n ? me * values / n : 0, e1 = me < n ? (me + 1) * values / n : 0;
+    const int64_t first_head = (int64_t)u.head * p.group + qt * 16;
+    for (int e = e0; e < e1; e += 256) {
+      const int width = min(e1 - e, 256), ways = 256 / width;
+      const int way = tid / width, mine = e + tid - way * width, q = mine / dim, d = mine - q * dim;
+      float o = 0.0f;
+      if (way < ways) {
+#pragma unroll 8
+        for (int i = way; i < w.count; i += ways) {
+          const int64_t at = (int64_t)w.slot(i) * p.query_tiles + qt;
+          o += p.slot_rows[(at * 16 + q) * DP + d] * rescale(p.slot_ml[at * 32 + q], tops[q]);
         }
       }
-      if (a.lse && me == 0 && tid < rows_here)
-        a.lse[u.seq * a.q_heads + (int64_t)u.head * p.group + u.query_tile * 16 + tid] = all[tid] * kLn2;
       __syncthreads();
-    }
-    if constexpr (ACC) {
-      // the first query tile's unit adds the weights of all query heads, so that no two add to one slot
-      if (u.query_tile == 0) {
-        const int64_t t0 = u.first * p.tile, t1 = min(u.last * p.tile, u.len);
-        for (int qt = 0; qt < p.query_tiles; ++qt) {
-          const int64_t unit_tile = u.unit_tile + qt * u.tiles;
-          const Pieces w = pieces_of(share, unit_tile, u.tiles);
-          if (w.first != w.last) {
-            totals(qt, w);
-          } else {
-            __syncthreads();
-            if (tid < 16) all[tid] = p.sums[(u.unit + qt) * 16 + tid];
-            __syncthreads();
-          }
-          const int rows_here = min(16, p.group - qt * 16);
-          const float* scores = p.scores + (u.seq * a.q_heads + (int64_t)u.head * p.group + qt * 16) * p.padded;
-          for (int64_t t = t0 + tid; t < t1; t += kThreads) {
-            const int64_t page = kv_page(pages, a.tables + u.seq * a.table_stride, t);
-            if (page < 0) continue;
-            float sum = 0.0f;
-            for (int q = 0; q < rows_here; ++q)
-              if (all[q] != -INFINITY) sum += exp2_of(scores[q * p.padded + t] - all[q]);
-            pages.weights[kv_row(pages, page, u.head, t)] += sum;
-          }
-        }
-        __syncthreads();
+      part[tid] = o;
+      __syncthreads();
+      if (way == 0) {
+        for (int i = 1; i < ways; ++i) o += part[i * width + tid];
+        const float f = all[q] == -INFINITY ? 0.0f : exp2_of(tops[q] - all[q]);
+        reinterpret_cast<T*>(a.out)[u.seq * a.out_seq_stride + (first_head + q) * a.out_head_stride + d] = (T)(o * f);
       }
     }
-    tile = u.unit_tile + u.last;
-    if (tile == seq_tile + u.tiles * p.units_per_seq) {
-      seq_tile = tile;
-      ++seq;
-    }
+    if (a.lse && me == 0 && tid < rows_here) a.lse[u.seq * (int64_t)a.q_heads + first_head + tid] = all[tid] * kLn2;
+    if constexpr (ACC) add_weights(a, p, u, qt, all);
   }
 }
 
 // A cache without pages: every sequence is empty.
 template <int QT>
-__global__ __launch_bounds__(kThreads) void kv_empty_kernel(const KvAttend a) {
+__global__ __launch_bounds__(256) void kv_empty_kernel(const KvAttend a) {
   using T = kv_elem<QT>;
   const int64_t s = blockIdx.x;
-  for (int i = threadIdx.x; i < a.q_heads * a.pages.dim; i += kThreads) {
+  for (int i = threadIdx.x; i < a.q_heads * a.pages.dim; i += 256) {
     const int h = i / a.pages.dim, d = i - h * a.pages.dim;
     reinterpret_cast<T*>(a.out)[s * a.out_seq_stride + h * a.out_head_stride + d] = (T)0.0f;
     if (a.lse && d == 0) a.lse[s * a.q_heads + h] = -INFINITY;
@@ -735,53 +786,67 @@ int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 struct Layout {
   Plan plan;
-  unsigned workgroups;
+  bool grid;
+  unsigned units;
   size_t bytes;
 };
+
+constexpr int64_t kGridWorkgroups = 2048;
+constexpr int64_t kGridChunk = 4;
 
 Layout layout_of(const KvAttend& a, void* workspace) {
   Layout r{};
   Plan& p = r.plan;
   p.group = a.q_heads / a.pages.heads;
   p.query_tiles = (p.group + 15) / 16;
-  p.units_per_seq = (int64_t)a.pages.heads * p.query_tiles;
-  p.tile = tile_slots(a.dtype);
+  p.tile = 4 * step_slots(a.dtype);
   const int64_t tiles = std::max<int64_t>(1, (a.max_length + p.tile - 1) / p.tile);
-  const int64_t units = a.seqs * p.units_per_seq;
+  const int64_t units = a.seqs * a.pages.heads;
+  r.units = (unsigned)units;
   p.padded = tiles * p.tile;
   const int dp = padded_dim(a.pages.dim);
-  // resident workgroups: two on each of the 256 CUs
-  const int64_t most = 512;
-  r.workgroups = (unsigned)(units >= most ? most : std::min<int64_t>(most, units * tiles));
+  const int64_t chunk = tiles <= kGridChunk ? tiles : (units * tiles + kGridWorkgroups - 1) / kGridWorkgroups;
+  r.grid = chunk <= kGridChunk && units <= 65535;
+  p.chunk = (int)chunk;
+  p.pieces = (int)((tiles + chunk - 1) / chunk);
+  // what the 256 CUs hold at once
+  p.workgroups = (int)std::min<int64_t>(256 * waves_per_simd(dp), units * tiles);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   auto take = [&](size_t n) {
-    float* x = reinterpret_cast<float*>(at + r.bytes);
+    void* x = at + r.bytes;
     r.bytes += (n + 15) / 16 * 16;
     return x;
   };
-  p.slot_rows = take((size_t)r.workgroups * 2 * 16 * dp * 4);
-  p.slot_ml = take((size_t)r.workgroups * 2 * 32 * 4);
-  if (a.accumulate) {
-    p.sums = take((size_t)units * 16 * 4);
-    p.scores = take((size_t)a.seqs * a.q_heads * p.padded * 4);
-  }
+  const size_t slots = r.grid ? (p.pieces == 1 ? 0 : (size_t)units * p.pieces) : 2 * (size_t)p.workgroups;
+  p.slot_rows = static_cast<float*>(take(slots * p.query_tiles * 16 * dp * 4));
+  p.slot_ml = static_cast<float*>(take(slots * p.query_tiles * 32 * 4));
+  if (!r.grid) p.slots = static_cast<Slot*>(take(slots * sizeof(Slot)));
+  if (a.accumulate) p.scores = static_cast<float*>(take((size_t)a.seqs * a.q_heads * p.padded * 4));
   return r;
+}
+
+template <int QT, int CT, int DP, bool EXACT, bool ACC>
+hipError_t launch_kernels(const KvAttend& a, const Layout& l, hipStream_t stream) {
+  if (l.grid) {
+    const dim3 grid((unsigned)l.plan.pieces, l.units);
+    kv_attend_kernel<QT, CT, DP, EXACT, ACC, true><<<grid, 256, 0, stream>>>(a, l.plan);
+    if (l.plan.pieces > 1) kv_join_kernel<QT, DP, ACC, true><<<grid, 256, 0, stream>>>(a, l.plan);
+  } else {
+    const unsigned n = (unsigned)l.plan.workgroups;
+    kv_attend_kernel<QT, CT, DP, EXACT, ACC, false><<<n, 256, 0, stream>>>(a, l.plan);
+    kv_join_kernel<QT, DP, ACC, false><<<2 * n, 256, 0, stream>>>(a, l.plan);
+  }
+  return hipGetLastError();
 }
 
 template <int QT, int CT, int DP, bool EXACT>
 hipError_t launch_dim(const KvAttend& a, const Layout& l, hipStream_t stream) {
   if (a.pages.num_pages == 0) {
-    kv_empty_kernel<QT><<<(unsigned)a.seqs, kThreads, 0, stream>>>(a);
+    kv_empty_kernel<QT><<<(unsigned)a.seqs, 256, 0, stream>>>(a);
     return hipGetLastError();
   }
-  if (a.accumulate) {
-    kv_attend_kernel<QT, CT, DP, EXACT, true><<<l.workgroups, kThreads, 0, stream>>>(a, l.plan);
-    kv_join_kernel<QT, DP, true><<<l.workgroups, kThreads, 0, stream>>>(a, l.plan);
-  } else {
-    kv_attend_kernel<QT, CT, DP, EXACT, false><<<l.workgroups, kThreads, 0, stream>>>(a, l.plan);
-    kv_join_kernel<QT, DP, false><<<l.workgroups, kThreads, 0, stream>>>(a, l.plan);
-  }
-  return hipGetLastError();
+  return a.accumulate ? launch_kernels<QT, CT, DP, EXACT, true>(a, l, stream)
+                      : launch_kernels<QT, CT, DP, EXACT, false>(a, l, stream);
 }
 
 template <int QT, int CT>

@@ -133,6 +133,9 @@ KvAttend attend_of(const nve_amd_kv_pages_t* pages, const nve_amd_kv_attend_t* p
                 "num_q_heads (", p->num_q_heads, ") must be a multiple of the pages' num_heads (", a.pages.heads, ")");
   NVE_CHECK_ARG(!std::isnan(p->scale), "scale must not be NaN");
   a.max_length = extent(a.pages, p->max_pages, p->max_length);
+  // the kernels count tiles of at least 64 slots in 32 bits
+  NVE_CHECK_ARG((a.max_length / 64 + 1) * p->num_seqs <= kMaxGrid / p->num_q_heads, "Too many slots: ", p->num_seqs,
+                " sequences of up to ", a.max_length);
   if (p->num_seqs > 0) {
     NVE_CHECK_ARG(p->q && p->out && p->lengths, "q, out and lengths must not be NULL");
     if (a.max_length > 0) NVE_CHECK_ARG(p->block_tables != nullptr, "block_tables must not be NULL");

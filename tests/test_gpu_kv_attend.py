@@ -84,10 +84,25 @@ TYPES = [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3"), ("bf
                                                     (10, 2, 8, 8), (20, 1, 96, 128), (34, 2, 136, 16), (7, 1, 40, 1024),
                                                     (70, 1, 128, 16)])
 @pytest.mark.parametrize("dtype,cache", TYPES)
-def test_types_and_layouts(dtype, cache, q_heads, heads, dim, page):
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_types_and_layouts(dtype, cache, q_heads, heads, dim, page, accumulate):
     s = setup(dtype, cache, [0, 1, 9, 31, 32, 33, 64, 100, 257, 700], q_heads, heads, dim, page, seed=dim + page)
     poison_unused(s)
-    check(s, dim**-0.5, call(s, dim**-0.5))
+    check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 56, 112, 248])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_widths_of_long_and_short_sequences(dtype, cache, accumulate, dim):
+    """Every width the kernels are built for, whole and partly filled, over a few lengths beyond one workgroup's."""
+    s = setup(dtype, cache, [3001, 40, 0, 1333, 5], 6, 2, dim, 16, seed=dim)
+    poison_unused(s)
+    check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
+    for i in range(5):  # the same through the path of short tables
+        s["lengths"][i] = min(int(s["lengths"][i]), 500)
+    s["table"] = np.ascontiguousarray(s["table"][:, :32])
+    check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
 
 
 @pytest.mark.parametrize("dtype,cache", TYPES)
@@ -95,6 +110,7 @@ def test_every_short_length(dtype, cache):
     s = setup(dtype, cache, list(range(0, 70)) + [127, 128, 129, 255, 256, 257, 511, 512, 513], 8, 2, 64, 16, seed=3)
     poison_unused(s)
     check(s, 0.125, call(s, 0.125))
+    check(s, 0.125, call(s, 0.125, accumulate=False))
 
 
 @pytest.mark.parametrize("dtype,cache", TYPES)
