@@ -1,15 +1,229 @@
 // kv_append.hip -- new tokens enter the paged key-value cache: rotary positions
 // on queries and keys, keys and values written to their slots.
 //
-// One wave per head row: lane l holds values l, l + 64, ...; a rotated value
-// reads its pair's other value itself, so nothing crosses lanes but an e4m3
-// row's largest magnitude.
+// Every value is read and written once, with 3 flops a rotated value: bound by
+// the bytes.  kv_append_kernel: a head row is a group of lanes (a power of two),
+// 16 values a lane.  A lane that rotates has 8 pairs, both values of each, so
+// that nothing crosses lanes but an e4m3 row's largest magnitude: values 8 j ..
+// and rot / 2 + 8 j .. of the row, or (pairs of neighbours) 16 j ..; the lanes
+// behind them have 16 unrotated values.  A workgroup has whole tokens: it brings
+// their cosines and sines into shared memory once for all their heads, while the
+// first rows' loads are under way.
+// kv_append_any_kernel, for rows that start off 16 bytes and for rotated widths
+// that are no multiple of 16: one value of a row per lane and step.
+#include <algorithm>
+
 #include "kv_common.cuh"
 
 namespace nve_amd {
 
 namespace {
 
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+
+// The largest magnitude by its bits, so that a NaN is the largest of all.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ float e4m3_scale(uint32_t top) {
+  return __uint_as_float(max(top, __float_as_uint(1e-30f))) / 448.0f;
+}
+
+__device__ __forceinline__ void write_slot(const KvAppend& a, int64_t t, int64_t at) {
+  if (a.pages.index) a.pages.index[at] = a.index ? a.index[t] : a.positions ? a.positions[t] : 0;
+  if (a.pages.weights) a.pages.weights[at] = 0.0f;
+}
+
+// The row of [pages, heads, page] that token t's head goes to, or -1.
+__device__ __forceinline__ int64_t row_of(const KvAppend& a, int64_t t, int head) {
+  const int64_t slot = a.slots[t], page = slot >> a.pages.page_bits;
+  if (slot < 0 || page >= a.pages.num_pages) return -1;
+  return kv_row(a.pages, page, head, slot);
+}
+
+__device__ __forceinline__ int axis_of(const KvAppend& a, int pair) {
+  int axis = 0;
+  while (axis + 1 < a.axes && pair >= a.ends[axis]) ++axis;
+  return axis;
+}
+
+// ---------------------------------------------------------------------------
+// 16 values a lane
+// ---------------------------------------------------------------------------
+constexpr int kThreads = 256;
+constexpr int kMaxTable = 2048;  // cosines and sines in shared memory
+
+// 8 values of a row, as they lie in memory: from, widened and (rounded) back.
+template <int DT>
+struct Eight {
+  static constexpr int kWords = DT == kF32 ? 2 : 1;
+  u32x4 w[kWords];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const u32x4*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float* x) const {
+    using T = kv_elem<DT>;
+    T v[8];
+    __builtin_memcpy(v, w, sizeof v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+  }
+  static __device__ __forceinline__ void store(uint8_t* p, const float* x) {
+    using T = kv_elem<DT>;
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (T)x[i];
+    u32x4 w[kWords];
+    __builtin_memcpy(w, v, sizeof v);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<u32x4*>(p)[i] = w[i];
+  }
+};
+
+__device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float scale) {
+  u32x2 w;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] / scale, x[4 * i + 1] / scale, 0, false);
+    w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] / scale, x[4 * i + 3] / scale, v, true);
+  }
+  *reinterpret_cast<u32x2*>(p) = w;
+}
+
+struct AppendPlan {
+  int32_t lanes, lane_bits;  // of a row
+  int32_t tokens;            // of a workgroup
+};
+
+template <int DT, bool E4M3>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppend a, const AppendPlan p) {
+  constexpr int kBytes = value_elem_bytes(DT);
+  __shared__ alignas(16) float table[kMaxTable];
+  __shared__ alignas(8) uint8_t turned[kMaxTable / 2];
+  const int tid = threadIdx.x, dim = a.pages.dim, heads = a.pages.heads, half = a.rot >> 1;
+  const int rows = a.q_heads + 2 * heads;
+  const int64_t t0 = (int64_t)blockIdx.x * p.tokens;
+  const int tokens = (int)min((int64_t)p.tokens, a.tokens - t0);
+  const int lane = tid & (p.lanes - 1), turning = a.rot >> 4;  // lanes that rotate
+  const int step = kThreads >> p.lane_bits;
+
+  // Where a lane's two times 8 values of a row are; `have`: how many of the two exist.
+  struct Place {
+    int first, second, have;
+    bool turn;
+  };
+  auto place = [&](bool value) {
+    Place r;
+    r.turn = !value && lane < turning;
+    if (r.turn && !a.interleaved) {
+      r.first = 8 * lane;
+      r.second = half + 8 * lane;
+    } else {
+      r.first = 16 * lane;  // the unrotated rest starts at rot = 16 * turning
+      r.second = r.first + 8;
+    }
+    r.have = r.turn ? 2 : r.first + 8 < dim ? 2 : r.first < dim ? 1 : 0;
+    return r;
+  };
+  struct Row {
+    int64_t t;
+    int head, kind;  // kind: 0 query, 1 key, 2 value
+  };
+  auto row_at = [&](int r) {
+    Row x;
+    const int token = r / rows;
+    x.t = t0 + token;
+    x.head = r - token * rows;
+    x.kind = x.head < a.q_heads ? 0 : x.head < a.q_heads + heads ? 1 : 2;
+    x.head -= x.kind == 0 ? 0 : x.kind == 1 ? a.q_heads : a.q_heads + heads;
+    return x;
+  };
+  Eight<DT> x0, x1;
+  auto load = [&](int r) {
+    const Row u = row_at(r);
+    const Place at = place(u.kind == 2);
+    const KvRows& in = u.kind == 0 ? a.q : u.kind == 1 ? a.k : a.v;
+    const uint8_t* row = in.p + (u.t * in.token_stride + u.head * in.head_stride) * kBytes;
+    if (at.have > 0) x0.load(row + at.first * kBytes);
+    if (at.have > 1) x1.load(row + at.second * kBytes);
+  };
+
+  int r = tid >> p.lane_bits;
+  const int all = tokens * rows;
+  if (r < all) load(r);
+  for (int e = tid; e < tokens * a.rot; e += kThreads) {
+    const int token = e / a.rot, i = e - token * a.rot, pair = i < half ? i : i - half;
+    const int64_t pos = a.positions[axis_of(a, pair) * a.axis_stride + t0 + token];
+    const bool in = pos >= 0 && pos < a.max_position;
+    table[e] = in ? a.cos_sin[pos * a.rot + i] : 0.0f;
+    if (i < half) turned[token * half + i] = in;
+  }
+  __syncthreads();
+
+  while (r < all) {
+    const Row u = row_at(r);
+    const Place at = place(u.kind == 2);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+    if (at.have > 0) x0.get(x);
+    if (at.have > 1) x1.get(x + 8);
+    const int next = r + step;
+    if (next < all) load(next);
+    if (at.turn) {
+      // pair i of the lane: values i and i + 8, or 2 i and 2 i + 1
+      const f32x4* cos = reinterpret_cast<const f32x4*>(table + (u.t - t0) * a.rot + 8 * lane);
+      const f32x4* sin = reinterpret_cast<const f32x4*>(table + (u.t - t0) * a.rot + 8 * lane + half);
+      const f32x4 c[2] = {cos[0], cos[1]}, s[2] = {sin[0], sin[1]};
+      const uint64_t on = *reinterpret_cast<const uint64_t*>(turned + (u.t - t0) * half + 8 * lane);
+      auto turn = [&](float& v, float& w, int i) {
+        const float co = c[i / 4][i % 4], si = s[i / 4][i % 4];
+        const float y = v * co - w * si, z = w * co + v * si;
+        const bool yes = (on >> (8 * i)) & 1;
+        v = yes ? y : v;
+        w = yes ? z : w;
+      };
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) turn(x[2 * i], x[2 * i + 1], i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) turn(x[i], x[8 + i], i);
+      }
+    }
+    if (u.kind == 0) {
+      uint8_t* out = a.q_out + (u.t * a.q_out_token_stride + u.head * a.q_out_head_stride) * kBytes;
+      if (at.have > 0) Eight<DT>::store(out + at.first * kBytes, x);
+      if (at.have > 1) Eight<DT>::store(out + at.second * kBytes, x + 8);
+    } else {
+      const int64_t to = row_of(a, u.t, u.head);
+      uint8_t* pages = u.kind == 2 ? a.pages.v : a.pages.k;
+      if constexpr (E4M3) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = max(top, magnitude(x[i]));
+        for (int m = p.lanes >> 1; m > 0; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
+        const float scale = e4m3_scale(top);
+        if (to >= 0) {
+          if (at.have > 0) store_codes(pages + to * dim + at.first, x, scale);
+          if (at.have > 1) store_codes(pages + to * dim + at.second, x + 8, scale);
+          if (lane == 0) (u.kind == 2 ? a.pages.v_scale : a.pages.k_scale)[to] = scale;
+        }
+      } else if (to >= 0) {
+        uint8_t* out = pages + to * dim * kBytes;
+        if (at.have > 0) Eight<DT>::store(out + at.first * kBytes, x);
+        if (at.have > 1) Eight<DT>::store(out + at.second * kBytes, x + 8);
+      }
+      if (u.kind == 2 && lane == 0 && to >= 0) write_slot(a, u.t, to);
+    }
+    r = next;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// any alignment, any rotated width
+// ---------------------------------------------------------------------------
 constexpr int kRowsPerBlock = 4;  // waves
 constexpr int kMaxPer = 4;        // values per lane: head_dim <= 256
 
@@ -22,9 +236,7 @@ __device__ __forceinline__ float rotated(const KvAppend& a, const T* row, int64_
   const int pair = a.interleaved ? d >> 1 : (d < half ? d : d - half);
   const bool first = a.interleaved ? (d & 1) == 0 : d < half;
   const int other = a.interleaved ? d ^ 1 : (first ? d + half : d - half);
-  int axis = 0;
-  while (axis + 1 < a.axes && pair >= a.ends[axis]) ++axis;
-  const int64_t p = a.positions[axis * a.axis_stride + t];
+  const int64_t p = a.positions[axis_of(a, pair) * a.axis_stride + t];
   if (p < 0 || p >= a.max_position) return x;
   const float* cs = a.cos_sin + p * a.rot;
   const float c = cs[pair], s = cs[pair + half], y = (float)row[other];
@@ -32,7 +244,7 @@ __device__ __forceinline__ float rotated(const KvAppend& a, const T* row, int64_
 }
 
 template <int DT, bool E4M3>
-__global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_kernel(const KvAppend a) {
+__global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const KvAppend a) {
   using T = kv_elem<DT>;
   const int lane = threadIdx.x & 63;
   const int rows = a.q_heads + 2 * a.pages.heads;
@@ -58,9 +270,8 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_kernel(const KvA
   head -= a.q_heads;
   const bool value = head >= a.pages.heads;
   if (value) head -= a.pages.heads;
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >> a.pages.page_bits >= a.pages.num_pages) return;
-  const int64_t at = kv_row(a.pages, slot >> a.pages.page_bits, head, slot);
+  const int64_t at = row_of(a, t, head);
+  if (at < 0) return;
   const KvRows& in = value ? a.v : a.k;
   const T* row = reinterpret_cast<const T*>(in.p) + t * in.token_stride + head * in.head_stride;
   uint8_t* pages = value ? a.pages.v : a.pages.k;
@@ -71,13 +282,12 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_kernel(const KvA
     x[i] = d >= dim ? 0.0f : value ? (float)row[d] : rotated(a, row, t, d);
   }
   if constexpr (E4M3) {
-    // the largest magnitude by its bits, so that a NaN is the largest of all
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kMaxPer; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int i = 0; i < kMaxPer; ++i) top = max(top, magnitude(x[i]));
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
-    const float scale = __uint_as_float(max(top, __float_as_uint(1e-30f))) / 448.0f;
+    const float scale = e4m3_scale(top);
 #pragma unroll
     for (int i = 0; i < kMaxPer; ++i)
       if (lane + 64 * i < dim)
@@ -89,32 +299,55 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_kernel(const KvA
     for (int i = 0; i < kMaxPer; ++i)
       if (lane + 64 * i < dim) out[lane + 64 * i] = (T)x[i];
   }
-  if (lane == 0 && value) {
-    if (a.pages.index) a.pages.index[at] = a.index ? a.index[t] : a.positions ? a.positions[t] : 0;
-    if (a.pages.weights) a.pages.weights[at] = 0.0f;
+  if (lane == 0 && value) write_slot(a, t, at);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+bool wide(const KvAppend& a) {
+  const int e = value_elem_bytes(a.dtype);
+  auto at16 = [&](const void* p, int64_t token, int64_t head) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && token * e % 16 == 0 && head * e % 16 == 0;
+  };
+  // rows of an e4m3 cache are written 8 bytes at a time, the others' start at 16 bytes with head_dim
+  return a.rot % 16 == 0 && at16(a.k.p, a.k.token_stride, a.k.head_stride) &&
+         at16(a.v.p, a.v.token_stride, a.v.head_stride) &&
+         (a.q_heads == 0 || (at16(a.q.p, a.q.token_stride, a.q.head_stride) &&
+                             at16(a.q_out, a.q_out_token_stride, a.q_out_head_stride)));
+}
+
+template <int DT, bool E4M3>
+hipError_t launch(const KvAppend& a, hipStream_t stream) {
+  const int rows = a.q_heads + 2 * a.pages.heads;
+  if (wide(a)) {
+    AppendPlan p{};
+    const int need = (a.pages.dim + 15) / 16;
+    while ((1 << p.lane_bits) < need) ++p.lane_bits;
+    p.lanes = 1 << p.lane_bits;
+    // whole tokens that fill a workgroup once
+    p.tokens = std::max(1, kThreads / (rows * p.lanes));
+    if (a.rot > 0) p.tokens = std::min(p.tokens, kMaxTable / a.rot);
+    const int64_t n = (a.tokens + p.tokens - 1) / p.tokens;
+    kv_append_kernel<DT, E4M3><<<(unsigned)n, kThreads, 0, stream>>>(a, p);
+  } else {
+    const int64_t n = (a.tokens * rows + kRowsPerBlock - 1) / kRowsPerBlock;
+    kv_append_any_kernel<DT, E4M3><<<(unsigned)n, 64 * kRowsPerBlock, 0, stream>>>(a);
   }
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_kv_append(const KvAppend& a, hipStream_t stream) {
-  const int64_t rows = a.tokens * (a.q_heads + 2 * a.pages.heads);
-  if (rows == 0) return hipSuccess;
-  const dim3 grid((unsigned)((rows + kRowsPerBlock - 1) / kRowsPerBlock)), block(64 * kRowsPerBlock);
+  if (a.tokens == 0) return hipSuccess;
   const bool q8 = a.pages.dtype == kE4M3;
   switch (a.dtype) {
-    case kF32: kv_append_kernel<kF32, false><<<grid, block, 0, stream>>>(a); break;
-    case kF16:
-      if (q8) kv_append_kernel<kF16, true><<<grid, block, 0, stream>>>(a);
-      else kv_append_kernel<kF16, false><<<grid, block, 0, stream>>>(a);
-      break;
-    case kBF16:
-      if (q8) kv_append_kernel<kBF16, true><<<grid, block, 0, stream>>>(a);
-      else kv_append_kernel<kBF16, false><<<grid, block, 0, stream>>>(a);
-      break;
+    case kF32: return launch<kF32, false>(a, stream);
+    case kF16: return q8 ? launch<kF16, true>(a, stream) : launch<kF16, false>(a, stream);
+    case kBF16: return q8 ? launch<kBF16, true>(a, stream) : launch<kBF16, false>(a, stream);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 }  // namespace nve_amd
