@@ -305,6 +305,8 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+constexpr int64_t kEnough = 2048;  // workgroups
+
 bool wide(const KvAppend& a) {
   const int e = value_elem_bytes(a.dtype);
   auto at16 = [&](const void* p, int64_t token, int64_t head) {
@@ -325,8 +327,9 @@ hipError_t launch(const KvAppend& a, hipStream_t stream) {
     const int need = (a.pages.dim + 15) / 16;
     while ((1 << p.lane_bits) < need) ++p.lane_bits;
     p.lanes = 1 << p.lane_bits;
-    // whole tokens that fill a workgroup once
-    p.tokens = std::max(1, kThreads / (rows * p.lanes));
+    // whole tokens: enough to fill the workgroup's threads, and more once there are workgroups for every CU
+    const int64_t fill = std::max(1, kThreads / (rows * p.lanes));
+    p.tokens = (int)std::max(fill, std::min<int64_t>(8 * fill, a.tokens / kEnough));
     if (a.rot > 0) p.tokens = std::min(p.tokens, kMaxTable / a.rot);
     const int64_t n = (a.tokens + p.tokens - 1) / p.tokens;
     kv_append_kernel<DT, E4M3><<<(unsigned)n, kThreads, 0, stream>>>(a, p);

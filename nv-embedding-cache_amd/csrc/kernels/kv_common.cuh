@@ -44,15 +44,17 @@ __device__ __forceinline__ int64_t kv_length(const int32_t* lengths, int64_t s, 
   return n < 0 ? 0 : n < max_length ? n : max_length;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-  return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+// x of the lanes up to and including this one, added; every lane of the wave is on.
+// Row shifts by 1, 2, 4 and 8, then each row's last lane to the rows behind it.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  asm volatile("" : "+v"(x));  // not moved under a condition, where some lanes are off
+  return x;
 }
 
 }  // namespace nve_amd
