@@ -216,8 +216,12 @@ __device__ __forceinline__ float high_of(uint32_t w) {
 // Two e4m3 codes (the low or high half of w) widened exactly.
 template <int QT>
 __device__ __forceinline__ uint32_t widen2(uint32_t w, bool high) {
-  const auto x = high ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-  return pack2<QT>(x[0], x[1]);
+  if constexpr (QT == kF16)
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  else
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
 }
 
 // 4 to 16 bytes of a row (any 4-byte alignment).
@@ -244,12 +248,17 @@ __device__ __forceinline__ void add_weights(const KvAttend& a, const Plan& p, co
     if (page < 0) continue;
     float* to = a.pages.weights + kv_row(a.pages, page, u.head, t);
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int q = 0; q < rows; ++q) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(scores + q * p.padded + t);
-      const float y = all[q] == -INFINITY ? INFINITY : all[q];  // an empty softmax has no weights
+    for (int q0 = 0; q0 < rows; q0 += 4) {  // four rows' loads together
+      f32x4 x[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += exp2_of(x[i] - y);
+      for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const f32x4*>(scores + min(q0 + j, rows - 1) * p.padded + t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // an empty softmax has no weights, nor has a row past the last
+        const float y = q0 + j >= rows || all[q0 + j] == -INFINITY ? INFINITY : all[q0 + j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += exp2_of(x[j][i] - y);
+      }
     }
     if (t + 4 <= t1) {
       *reinterpret_cast<f4*>(to) += sum;
@@ -478,7 +487,10 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
     load_ids(0);
     load_k(0);
     load_v(0);
-    for (int step = 0; step < steps; ++step) {
+    // A step; with `more` the next one's rows are requested on the way.  The last step is apart,
+    // because a wait after a branch around loads has to suit the path without them: it would wait
+    // for the next step's rows as well.
+    auto advance = [&](int step, auto more) {
       const int64_t t0 = t_base + (int64_t)step * (kWaves * kStep);
       f32x4 s[W::kTiles];
 #pragma unroll
@@ -513,9 +525,10 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
                 f32x4{y[n * 4], y[n * 4 + 1], y[n * 4 + 2], y[n * 4 + 3]};
         }
       }
-      const bool more = step + 1 < steps;
-      if (more && ((step + 1) & 15) == 0) load_ids(step + 1);
-      if (more) load_k(step + 1);
+      if constexpr (more) {
+        if (((step + 1) & 15) == 0) load_ids(step + 1);
+        load_k(step + 1);
+      }
 
       float top = y[0];
 #pragma unroll
@@ -537,8 +550,10 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
         if constexpr (CT == kE4M3) w[i] *= x.v_scale[i / 4][i % 4];
       }
       x.add_values(w);
-      if (more) load_v(step + 1);
-    }
+      if constexpr (more) load_v(step + 1);
+    };
+    for (int step = 0; step + 1 < steps; ++step) advance(step, std::true_type());
+    advance(steps - 1, std::false_type());
 
     // the workgroup's waves: rows relative to the largest m
     const float l = query_sum(x.l);
@@ -608,16 +623,16 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
   };
 
   if constexpr (GRID) {
-    const int unit = blockIdx.y;
+    const int unit = blockIdx.x;  // units first: their pieces, of which there may be fewer, spread over the XCDs
     Piece u;
     u.seq = unit / pages.heads;
     u.head = unit - u.seq * pages.heads;
     u.len = kv_length(a.lengths, u.seq, a.max_length);
     u.tiles = tiles_of(p, u.len);
-    u.first = blockIdx.x * p.chunk;
+    u.first = blockIdx.y * p.chunk;
     u.last = min(u.first + p.chunk, u.tiles);
     if (u.first >= u.tiles) return;
-    for (int qt = 0; qt < p.query_tiles; ++qt) process(u, qt, unit * p.pieces + blockIdx.x);
+    for (int qt = 0; qt < p.query_tiles; ++qt) process(u, qt, unit * p.pieces + blockIdx.y);
   } else {
     const Start start = find_start(a, p);
     const Shares shares(start.total, p.workgroups);
@@ -707,14 +722,15 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend a, const Pl
   const int tid = threadIdx.x, dim = a.pages.dim;
   Piece u;
   Pieces w;
-  int me;  // which of the unit's pieces this is
+  int me, joiners;  // which of the unit's workgroups this is, how many may join
   if constexpr (GRID) {
-    const int unit = blockIdx.y;
+    joiners = gridDim.y;
+    const int unit = blockIdx.x;
     u.seq = unit / a.pages.heads;
     u.head = unit - u.seq * a.pages.heads;
     u.len = kv_length(a.lengths, u.seq, a.max_length);
     u.tiles = tiles_of(p, u.len);
-    me = blockIdx.x;
+    me = blockIdx.y;
     u.first = me * p.chunk;
     u.last = min(u.first + p.chunk, u.tiles);
     w.count = (u.tiles + p.chunk - 1) / p.chunk;
@@ -733,11 +749,12 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend a, const Pl
     w.head = 2 * first + (shares.begin(first) == s.unit_tile ? 0 : 1);
     w.next = 2 * (first + 1);
     w.step = 2;
+    joiners = w.count;
   }
   for (int qt = 0; qt < p.query_tiles; ++qt) {
     // a run of the output values
     const int rows_here = min(16, p.group - qt * 16), values = rows_here * dim;
-    const int n = min(w.count, (values + kJoinValues - 1) / kJoinValues);
+    const int n = min(min(w.count, joiners), (values + kJoinValues - 1) / kJoinValues);
     if (!ACC && me >= n) continue;
     total_of(p, w, qt, tops, all);
     const int e0 = me < n ? me * values / n : 0, e1 = me < n ? (me + 1) * values / n : 0;
@@ -747,10 +764,17 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend a, const Pl
       const int way = tid / width, mine = e + tid - way * width, q = mine / dim, d = mine - q * dim;
       float o = 0.0f;
       if (way < ways) {
-#pragma unroll 8
-        for (int i = way; i < w.count; i += ways) {
-          const int64_t at = (int64_t)w.slot(i) * p.query_tiles + qt;
-          o += p.slot_rows[(at * 16 + q) * DP + d] * rescale(p.slot_ml[at * 32 + q], tops[q]);
+        for (int i0 = way; i0 < w.count; i0 += 4 * ways) {  // four pieces' loads together
+          float x[4], m[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * ways;
+            const int64_t at = (int64_t)w.slot(min(i, w.count - 1)) * p.query_tiles + qt;
+            x[j] = p.slot_rows[(at * 16 + q) * DP + d];
+            m[j] = i < w.count ? p.slot_ml[at * 32 + q] : -INFINITY;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o += m[j] == -INFINITY ? 0.0f : x[j] * exp2_of(m[j] - tops[q]);
         }
       }
       __syncthreads();
@@ -791,8 +815,27 @@ struct Layout {
   size_t bytes;
 };
 
-constexpr int64_t kGridWorkgroups = 2048;
-constexpr int64_t kGridChunk = 4;
+// Tiles of a grid workgroup, 0: stream mode.  The lengths are not known here, only the tables'
+// extent; all figures are for 128 values of 16 bits, 4 queries a key head and 128-slot tiles.
+//   Whole units, one launch, up to 4 tiles (one piece 12.2 us, 32 pieces and a join 10.3 us for one
+//   sequence of 4,096 slots, but 34.9 against 43.4 us for 256 of 32 to 512), and up to 16 where
+//   there are units for all CUs (64 sequences of 125 to 2,000 slots: whole 33.9, pieces of 8 42.3).
+//   One sequence is as long as its table: 256 pieces, one a CU, are enough (200,001 slots: 144 us,
+//   stream 155, pieces of 16 tiles 165; 16,384: 17.7, stream 23.6, 1 tile 22.0).
+//   Several may be much shorter than the longest: smaller pieces (7 of 33 to 30,011 slots, 2 key
+//   heads: pieces of 4 tiles 22 us, 8 29, stream 35; 64 of 512 to 8,192: 8 tiles 180, 16 188, stream 186).
+//   In f32 (64-slot tiles) 8 is the most: 48 sequences of up to 2,000 slots 30.5 us, 12 32.2.
+//   An empty workgroup costs 1.2 ns, so tables far longer than the sequences go to stream mode
+//   (64 sequences of up to 2,000 slots in tables of 131,072: stream 41 us, pieces of 12 tiles 91;
+//   in tables of 32,768: 42 and 44).
+int64_t grid_chunk(int64_t seqs, int64_t units, int64_t tiles, int tile) {
+  const int64_t all = units * tiles, most = tile < 128 ? 8 : 12;
+  int64_t chunk = std::min(most, (all + 1023) / 1024);
+  if (tiles <= 4 || (tiles <= 16 && units >= 256)) chunk = tiles;
+  else if (seqs == 1) chunk = (all + 255) / 256;
+  const int64_t pieces = (tiles + chunk - 1) / chunk;
+  return pieces == 1 || units * pieces <= 8192 ? chunk : 0;
+}
 
 Layout layout_of(const KvAttend& a, void* workspace) {
   Layout r{};
@@ -805,10 +848,10 @@ Layout layout_of(const KvAttend& a, void* workspace) {
   r.units = (unsigned)units;
   p.padded = tiles * p.tile;
   const int dp = padded_dim(a.pages.dim);
-  const int64_t chunk = tiles <= kGridChunk ? tiles : (units * tiles + kGridWorkgroups - 1) / kGridWorkgroups;
-  r.grid = chunk <= kGridChunk && units <= 65535;
+  const int64_t chunk = grid_chunk(a.seqs, units, tiles, p.tile);
+  r.grid = chunk > 0;
   p.chunk = (int)chunk;
-  p.pieces = (int)((tiles + chunk - 1) / chunk);
+  p.pieces = r.grid ? (int)((tiles + chunk - 1) / chunk) : 0;
   // what the 256 CUs hold at once
   p.workgroups = (int)std::min<int64_t>(256 * waves_per_simd(dp), units * tiles);
   uint8_t* at = static_cast<uint8_t*>(workspace);
@@ -828,9 +871,11 @@ Layout layout_of(const KvAttend& a, void* workspace) {
 template <int QT, int CT, int DP, bool EXACT, bool ACC>
 hipError_t launch_kernels(const KvAttend& a, const Layout& l, hipStream_t stream) {
   if (l.grid) {
-    const dim3 grid((unsigned)l.plan.pieces, l.units);
+    const dim3 grid(l.units, (unsigned)l.plan.pieces);
     kv_attend_kernel<QT, CT, DP, EXACT, ACC, true><<<grid, 256, 0, stream>>>(a, l.plan);
-    if (l.plan.pieces > 1) kv_join_kernel<QT, DP, ACC, true><<<grid, 256, 0, stream>>>(a, l.plan);
+    // weights are added piece by piece; to join alone, some workgroups a unit are enough
+    const unsigned join = ACC ? grid.y : std::min(grid.y, std::max(1u, 1024 / l.units));
+    if (l.plan.pieces > 1) kv_join_kernel<QT, DP, ACC, true><<<dim3(l.units, join), 256, 0, stream>>>(a, l.plan);
   } else {
     const unsigned n = (unsigned)l.plan.workgroups;
     kv_attend_kernel<QT, CT, DP, EXACT, ACC, false><<<n, 256, 0, stream>>>(a, l.plan);

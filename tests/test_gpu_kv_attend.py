@@ -129,6 +129,33 @@ def test_many_sequences(dtype, cache):
     check(s, 0.125, call(s, 0.125))
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256, 80])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_tables_far_longer_than_the_sequences(dtype, cache, accumulate, dim):
+    """Tables of 131,072 slots over short sequences: the workgroups share the slots there are."""
+    rng = np.random.default_rng(21)
+    lengths = [int(n) for n in rng.integers(0, 40, size=95)] + [2500, 0, 777, 1, 1300]
+    s = setup(dtype, cache, lengths, 6, 3, dim, 16, seed=22)
+    wide = np.full((len(lengths), 8192), -1, np.int32)
+    wide[:, :s["table"].shape[1]] = s["table"]
+    s["table"] = wide
+    poison_unused(s)
+    check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
+
+
+@pytest.mark.parametrize("dtype,cache", [("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("q_heads", [34, 40])
+def test_wide_groups_in_long_tables(dtype, cache, q_heads):
+    """More than 16 query heads a key head, sequences in several pieces, both ways of sharing the work."""
+    s = setup(dtype, cache, [2100, 3, 1500, 0] + [5] * 96, q_heads, 1, 64, 16, seed=23)
+    check(s, 0.125, call(s, 0.125))
+    wide = np.full((100, 8192), -1, np.int32)
+    wide[:, :s["table"].shape[1]] = s["table"]
+    s["table"] = wide
+    check(s, 0.125, call(s, 0.125))
+
+
 @pytest.mark.parametrize("dtype,cache", TYPES)
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_one_slot_is_copied(dtype, cache, accumulate):
