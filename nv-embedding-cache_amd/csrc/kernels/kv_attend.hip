@@ -5,10 +5,9 @@
 // maximum m and sum l of the softmax; what was summed before is scaled by
 // 2^(m_old - m) when the maximum grows (x in units of log2).
 //
-// Bound: every k and v row is read once for 4 flops per query head and byte
-// pair, so the pages' bytes bound it; the matrix instructions keep the work per
-// byte far below that, whatever the group of query heads (up to 16) that
-// shares a key head.
+// Bound: every k and v row is read once, so the pages' bytes bound it; the matrix
+// instructions keep the work per byte far below that for any group of up to 16 query
+// heads that share a key head (larger groups read the rows once per 16).
 //
 // Layout of a wave's step (kStep slots, 16 query columns).  Scores are computed
 // transposed: S^T = K Q^T, the k rows as the A operand (a lane reads 16 bytes of
@@ -20,6 +19,7 @@
 // the same piece of its 8 slots' rows and transposes 16-bit pairs in registers.
 // A value tile's row r is the value r * dim / 16 + tile, which makes those
 // pieces contiguous.  No shared memory until the waves of a workgroup join.
+// f32 has the same layout with 16 slots a step and products of one value a lane.
 //
 // Weights enter the second product as the sum of two values of the product's
 // type (at least 16 bits of the f32 weight): one alone would lose as much as the
@@ -28,13 +28,28 @@
 // maximum still counts).  e4m3 rows are widened exactly to the query's type
 // (scores) and to bf16 (values); their scales go into scores and weights.
 //
-// Split: workgroups of 4 waves are the machine's resident ones, and each takes
-// an equal run of the tiles (4 kStep slots) of all (sequence, key head, 16
-// queries) units laid end to end, whatever the lengths.  A unit inside one
-// workgroup is finished there; pieces of a unit go to the workspace as f32 rows
-// with their m and l, and the second kernel, mapped the same way, joins them.
-// It also adds the attention weights where they are asked for, from the scores
-// that the first kernel left in the workspace.
+// Split.  A workgroup of 4 waves takes a run of tiles (4 kStep slots) of one unit, a
+// (sequence, key head); its waves join through shared memory.  A unit that is one
+// workgroup's is finished there; others leave f32 rows with their m and l in the
+// workspace, and the second kernel joins them.  Weights are added by whoever knows
+// a unit's sum: the first kernel for whole units, the second, piece by piece, for
+// the others, from the scores that the first one left in the workspace.
+//   Grid mode: a workgroup per piece of grid_chunk() tiles, as the tables' extent
+//   asks for.  The unit is the fast index: consecutive workgroups go round the 8
+//   XCDs, and later pieces exist for the long sequences only; with the piece as the
+//   fast index (4 a unit) the first pieces met on two XCDs (64 sequences of 512 to
+//   8,192 slots: 273 us, units first 183).
+//   Stream mode, for tables far longer than their sequences: the machine's resident
+//   workgroups share all tiles there are, units laid end to end, in equal runs.
+// Two waves a SIMD at 128 values (one at 256, three at 64): k and v rows of the next
+// step are in flight meanwhile, 32 KiB a workgroup.  Three were slower (one sequence
+// of 200,001 slots: 170 us, two 146).
+//
+// Measured (bf16 / f16, 128 values, pages of 16): one sequence of 200,001 slots, 8 key
+// heads: 144 us, 5.7 TB/s of the pages' bytes (a large copy moves 4.7 TB/s, read and
+// written); 64 sequences of 512 to 8,192 slots with weights: 184 us (165 and 15 in the
+// two kernels), 4.1 TB/s; 256 of 200 to 4,096 in e4m3, 8 queries a key head: 158 us, 4.5 TB/s.
+// One of 777 slots: 9.8 us, two launches of three dependent reads each.
 #include <math.h>
 
 #include <algorithm>

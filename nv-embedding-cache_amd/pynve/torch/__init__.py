@@ -17,6 +17,9 @@ library's registry (nve_registry.cu:25-50), which pynve.nve.register_for_torch
 fills.  Shape inference (the fake kernels) uses only the baked
 `embedding_size` and `dtype` arguments, as the reference's
 pynve/torch/__init__.py does.
+
+The library also holds the operators of the paged key-value cache (nve_kv),
+nve_ops::kv_append, kv_attend, kv_attend_lse and kv_evict, for HIP tensors.
 """
 import ctypes
 import os
