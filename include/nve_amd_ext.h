@@ -269,7 +269,7 @@ NVE_C_API nve_status_t nve_amd_kv_append(const nve_amd_kv_pages_t* pages,
  * p_t, summed over the query heads of a key head, is added to pages->weights;
  * no page may then belong to two sequences of the call.  max_length: the
  * longest length that occurs, if the caller knows it (0: the table's extent);
- * it only sizes the launch.  workspace: device memory of
+ * it sizes the launch and the workspace.  workspace: device memory of
  * nve_amd_kv_attend_workspace_size bytes, 16-byte aligned. */
 typedef struct {
   int64_t num_seqs;

@@ -11,8 +11,8 @@
 // first rows' loads are under way.
 // Several tokens a workgroup once there are 2,048 workgroups: 9,000 tokens into e4m3
 // 51 -> 42 us.  Measured: 16,001 f16 tokens of 32 query and 8 key heads of 128 values
-// 83 to 92 us (4.4 to 4.8 TB/s, a large copy's rate); 9,000 bf16 tokens of 96 values
-// into e4m3 43 us (3.7 TB/s: a division a value, and 6 of 8 lanes a row); a step of 64
+// 83 to 92 us (4.4 to 4.8 TB/s; a large copy 4.7); 9,000 bf16 tokens of 96 values
+// into e4m3 42 to 44 us (3.6 TB/s; 6 of 8 lanes a row work); a step of 64
 // tokens 4.8 us, the chain position, cosine, shared memory, store.
 // kv_append_any_kernel, for rows that start off 16 bytes and for rotated widths
 // that are no multiple of 16: one value of a row per lane and step (409 us for the

@@ -47,8 +47,8 @@
 //
 // Measured (bf16 / f16, 128 values, pages of 16): one sequence of 200,001 slots, 8 key
 // heads: 144 us, 5.7 TB/s of the pages' bytes (a large copy moves 4.7 TB/s, read and
-// written); 64 sequences of 512 to 8,192 slots with weights: 184 us (165 and 15 in the
-// two kernels), 4.1 TB/s; 256 of 200 to 4,096 in e4m3, 8 queries a key head: 158 us, 4.5 TB/s.
+// written); 64 sequences of 512 to 8,192 slots with weights: 181 us (165 and 15 in the
+// two kernels), 4.1 TB/s; 256 of 200 to 4,096 in e4m3, 8 queries a key head: 157 us, 4.5 TB/s.
 // One of 777 slots: 9.8 us, two launches of three dependent reads each.
 #include <math.h>
 

@@ -22,9 +22,10 @@
 // through shared memory in two bits, so that a thread has slots in a row.  11 bits
 // a digit, because weights that fall off over some binades share their first 8
 // bits: their additions to one bin would queue.
-// Measured: 64 sequences of 2,064 slots and 8 key heads to 2,048: 13 us (launch 2,
-// loads 4, digits 5, pairs and moves 3); 8 prompts of 32,768 slots to 4,096: 39 us to
-// choose (64 workgroups on 256 CUs), 28 to 48 to move 3,584 rows a head where all move.
+// Measured: 64 sequences of 2,064 slots and 8 key heads to 2,048: 15 us
+// repeated on one cache, 17 to 19 on a fresh one; 8 prompts of 32,768 slots to 4,096: 41
+// to 45 us to choose (64 workgroups on 256 CUs) and 59 to 73 to move the rows of a fresh
+// cache, 35 and 9 once repeated, as fewer rows then move.
 #include <algorithm>
 #include <type_traits>
 

@@ -66,7 +66,8 @@ def kv_attend(q, k_pages, v_pages, block_tables, lengths, *, scale=None, k_scale
     [S, Hq].  A sequence without slots gives zeros (and -inf).  With `weights` the
     softmax of every slot, summed over the query heads of its key head, is added
     there; no page may then belong to two of the sequences.  `max_length` is a
-    bound on the lengths if the caller knows one below the tables' extent."""
+    bound on the lengths if the caller knows one below the tables' extent; it
+    sizes the launch and the workspace."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     f = _attend_lse if return_lse else _attend
