@@ -46,8 +46,13 @@ constexpr int64_t kFewPairs = 64;  // of a unit: copied by the selecting workgro
 // last, the two zeros equal.  No weight has one of the keys below.
 constexpr uint32_t kGoes = 0u;           // dropped in any case
 constexpr uint32_t kAbsent = 1u;         // of an absent page: before every weight
-constexpr uint32_t kNaN = 0xfffffffeu;
+constexpr uint32_t kNaN = 0xffc00000u;   // past +infinity's 0xff800000
 constexpr uint32_t kStays = 0xffffffffu; // kept in any case, or no slot
+// The select may end after the first 11 bits, and neither slots that stay nor slots that go are
+// counted in it: no key that is counted beside them may share those bits.  Beside slots that go
+// these are protected slots' only, whose pages are there (from -infinity's 0x007fffff on).
+constexpr int kFirstShift = 21;
+static_assert(kNaN >> kFirstShift != kStays >> kFirstShift && 0x007fffffu >> kFirstShift != kGoes >> kFirstShift);
 __device__ __forceinline__ uint32_t order_key(float w) {
   const uint32_t b = __float_as_uint(w + 0.0f);
   return w != w ? kNaN : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
@@ -299,10 +304,10 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvict a, int
 
   // The digits found so far and their bits: keys below `prefix` in those bits go, and the first
   // `rest` of those equal to it (all of them once as many are left as go).  Slots that go or stay
-  // in any case are not counted; the keys beside them have other first digits.
+  // in any case are not counted; no key that is counted has their first digit.
   int rest = among_held ? drop - opened : drop;
   uint32_t prefix = 0, found = 0;
-  for (int shift = 21, bits = 11;;) {
+  for (int shift = kFirstShift, bits = 11;;) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) hist[tid + i * THREADS] = 0;
     __syncthreads();
@@ -343,7 +348,7 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvict a, int
     found |= digit << shift;
     rest = chosen[1];
     if (shift == 0 || chosen[2] == rest) break;
-    bits = shift == 21 ? 11 : 10;
+    bits = shift == kFirstShift ? 11 : 10;
     shift -= bits;
   }
 

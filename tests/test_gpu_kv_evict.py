@@ -104,6 +104,30 @@ def test_nan_and_infinite_weights():
         run([300, 299, 61], budget, seed=6, weights=w, recent=10)
 
 
+@pytest.mark.parametrize("length", [20, 300, 1024, 1500, 6000, 20000, 40000])
+@pytest.mark.parametrize("nans", ["one a page", "some", "all"])
+@pytest.mark.parametrize("shuffled", [False, True])
+def test_a_budget_of_the_protected_slots_drops_every_other_one(length, nans, shuffled):
+    """As many unprotected slots as have to go, NaN weights among them: no protected slot goes with them
+    (every kernel variant: 1,024, 4,096, 16,384, 32,768 slots and more)."""
+    budget = 5 if length == 20 else 40
+    sinks = 2 if length == 20 else 8
+
+    def w(rng, s):
+        x = rng.normal(1, 1, size=s).astype(np.float32)
+        if nans == "one a page":
+            x[:, :, s[2] - 6] = np.nan
+        elif nans == "some":
+            x[rng.random(s) < 0.1] = np.nan
+        else:
+            x[:] = np.nan
+        return x
+
+    index = None if shuffled else lambda rng, n: np.arange(n)
+    run([length, length - 1, budget + 1, budget], budget, heads=1, dim=8, page=16, sinks=sinks, recent=budget - sinks,
+        seed=20 + length, weights=w, index=index, extra=0)
+
+
 def test_negative_tiny_and_close_weights():
     run([900], 300, seed=7, weights=lambda rng, s: (rng.integers(-3, 4, size=s) * np.float32(1e-45)).astype(np.float32))
     run([900], 300, seed=8, weights=lambda rng, s: np.nextafter(np.float32(1), np.float32(2)) *
