@@ -302,9 +302,10 @@ NVE_C_API nve_status_t nve_amd_kv_attend(const nve_amd_kv_pages_t* pages,
  * up to the head's newest index, a NaN weight is the greatest and slots of
  * absent pages come first.  The j-th dropped slot below `budget` then takes the
  * row (k, v, scales, weight, index) of the j-th kept slot at or past it;
- * nothing else is written.  new_lengths[s] = min(lengths[s], budget).  No page
- * may belong to two sequences of the call.  workspace: device memory of
- * nve_amd_kv_evict_workspace_size bytes, 16-byte aligned. */
+ * nothing else is written.  new_lengths[s] = min(lengths[s], budget); the two
+ * may not overlap.  No page may belong to two sequences of the call.
+ * workspace: device memory of nve_amd_kv_evict_workspace_size bytes, 16-byte
+ * aligned. */
 typedef struct {
   int64_t num_seqs;
   const int32_t* block_tables;

@@ -215,6 +215,9 @@ void kv_evict_run(const nve_amd_kv_pages_t* pages, const nve_amd_kv_evict_t* cal
                   hipStream_t s) {
   const KvEvict a = evict_of(pages, call);
   check_workspace(ws, ws_bytes, kv_evict_workspace(a));
+  // every head of a sequence reads its length, the first one writes the new one
+  NVE_CHECK_ARG(a.new_lengths + a.seqs <= a.lengths || a.lengths + a.seqs <= a.new_lengths,
+                "new_lengths must not overlap lengths");
   NVE_HIP(launch_kv_evict(a, ws, s));
 }
 

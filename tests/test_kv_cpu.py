@@ -124,6 +124,14 @@ def test_evict_needs_weights_index_and_a_workspace():
     assert "orkspace" in _lib.last_error()
 
 
+@pytest.mark.parametrize("offset", [0, 4, 8, -4, -8])
+def test_evict_in_place_lengths_are_refused(offset):
+    """A sequence's heads read its length while the first of them writes the new one."""
+    refs = [ctypes.byref(pages()), ctypes.byref(evict(new_lengths=FAKE + offset))]
+    assert L.nve_amd_kv_evict(*refs, FAKE, 1 << 20, None) == _lib.INVALID_ARGUMENT
+    assert "overlap" in _lib.last_error()
+
+
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
 @pytest.mark.parametrize("name,view", [("nve_amd_kv_pages_t", _lib.KvPages), ("nve_amd_kv_append_t", _lib.KvAppend),
                                        ("nve_amd_kv_attend_t", _lib.KvAttend), ("nve_amd_kv_evict_t", _lib.KvEvict)])
