@@ -5,7 +5,8 @@
 //
 // Shapes, types and devices are checked here, the rest by the C ABI; work runs
 // on the current stream, workspaces come from torch's allocator.  The operators
-// serve: none has a gradient, and inputs that ask for one are refused.
+// serve: none has a gradient, and inputs that ask for one are refused, the cache
+// and the rotary table among them.
 #include <ATen/DeviceGuard.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
@@ -60,6 +61,11 @@ void check_dense(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_contiguous(), "nve_ops: ", name, " must be contiguous");
 }
 
+void check_grad(const Tensor& t, const char* name) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), "nve_ops: ", name,
+              " asks for a gradient, and the key-value cache's operators have none (use torch.no_grad())");
+}
+
 // [rows, heads, dim] with a contiguous last dimension, any strides of the others.
 void check_rows(const Tensor& t, const Tensor& pages, const char* name) {
   check_device(t, pages, name);
@@ -67,8 +73,7 @@ void check_rows(const Tensor& t, const Tensor& pages, const char* name) {
                     pages.size(3), "], got ", t.sizes());
   TORCH_CHECK_VALUE(t.stride(2) == 1 || t.numel() == 0, "nve_ops: the last dimension of ", name,
                     " must be contiguous");
-  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), "nve_ops: ", name,
-              " asks for a gradient, and the key-value cache's operators have none (use torch.no_grad())");
+  check_grad(t, name);
 }
 
 const void* optional_row(const OptTensor& t, const Tensor& pages, at::ScalarType type, int64_t n, const char* name) {
@@ -87,6 +92,7 @@ T* slot_values(const OptTensor& t, const Tensor& pages, at::ScalarType type, con
   check_device(*t, pages, name);
   check_type(*t, type, name);
   check_dense(*t, name);
+  check_grad(*t, name);
   TORCH_CHECK_VALUE(t->sizes() == pages.sizes().slice(0, 3), "nve_ops: ", name, " must be ",
                     pages.sizes().slice(0, 3), ", got ", t->sizes());
   return static_cast<T*>(t->data_ptr());
@@ -103,6 +109,8 @@ nve_amd_kv_pages_t pages_of(const Tensor& k, const Tensor& v, const OptTensor& k
   check_device(v, k, "v_pages");
   check_dense(k, "k_pages");
   check_dense(v, "v_pages");
+  check_grad(k, "k_pages");
+  check_grad(v, "v_pages");
   nve_amd_kv_pages_t p{};
   p.k = k.data_ptr();
   p.v = v.data_ptr();
@@ -183,6 +191,7 @@ Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const 
       check_device(t, k_pages, "cos_sin");
       check_type(t, at::kFloat, "cos_sin");
       check_dense(t, "cos_sin");
+      check_grad(t, "cos_sin");
       TORCH_CHECK_VALUE(t.dim() == 2 && t.size(1) <= k_pages.size(3), "nve_ops: cos_sin must be [positions, rot_dim <= ",
                         k_pages.size(3), "], got ", t.sizes());
       c.cos_sin = static_cast<const float*>(t.data_ptr());
