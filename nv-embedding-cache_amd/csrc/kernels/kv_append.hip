@@ -312,6 +312,22 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const
 // host
 // ---------------------------------------------------------------------------
 constexpr int64_t kEnough = 2048;  // workgroups
+constexpr int64_t kMostGroups = 0xffffffffu / kThreads;  // a launch has fewer than 2^32 threads
+static_assert(kThreads == 64 * kRowsPerBlock);
+
+// The n tokens from t0 on.
+KvAppend part(const KvAppend& a, int64_t t0, int64_t n) {
+  const int e = value_elem_bytes(a.dtype);
+  KvAppend r = a;
+  r.tokens = n;
+  r.slots += t0;
+  for (KvRows* rows : {&r.k, &r.v, &r.q})
+    if (rows->p) rows->p += t0 * rows->token_stride * e;
+  if (r.q_out) r.q_out += t0 * r.q_out_token_stride * e;
+  if (r.index) r.index += t0;
+  if (r.positions) r.positions += t0;
+  return r;
+}
 
 bool wide(const KvAppend& a) {
   const int e = value_elem_bytes(a.dtype);
@@ -328,8 +344,10 @@ bool wide(const KvAppend& a) {
 template <int DT, bool E4M3>
 hipError_t launch(const KvAppend& a, hipStream_t stream) {
   const int rows = a.q_heads + 2 * a.pages.heads;
-  if (wide(a)) {
-    AppendPlan p{};
+  AppendPlan p{};
+  int64_t most;  // tokens of a launch
+  const bool in_words = wide(a);
+  if (in_words) {
     const int need = (a.pages.dim + 15) / 16;
     while ((1 << p.lane_bits) < need) ++p.lane_bits;
     p.lanes = 1 << p.lane_bits;
@@ -337,13 +355,20 @@ hipError_t launch(const KvAppend& a, hipStream_t stream) {
     const int64_t fill = std::max(1, kThreads / (rows * p.lanes));
     p.tokens = (int)std::max(fill, std::min<int64_t>(8 * fill, a.tokens / kEnough));
     if (a.rot > 0) p.tokens = std::min(p.tokens, kMaxTable / a.rot);
-    const int64_t n = (a.tokens + p.tokens - 1) / p.tokens;
-    kv_append_kernel<DT, E4M3><<<(unsigned)n, kThreads, 0, stream>>>(a, p);
+    most = kMostGroups * p.tokens;
   } else {
-    const int64_t n = (a.tokens * rows + kRowsPerBlock - 1) / kRowsPerBlock;
-    kv_append_any_kernel<DT, E4M3><<<(unsigned)n, 64 * kRowsPerBlock, 0, stream>>>(a);
+    most = kMostGroups * kRowsPerBlock / rows;
   }
-  return hipGetLastError();
+  for (int64_t t0 = 0; t0 < a.tokens; t0 += most) {
+    const KvAppend b = part(a, t0, std::min(most, a.tokens - t0));
+    if (in_words)
+      kv_append_kernel<DT, E4M3><<<(unsigned)((b.tokens + p.tokens - 1) / p.tokens), kThreads, 0, stream>>>(b, p);
+    else
+      kv_append_any_kernel<DT, E4M3>
+          <<<(unsigned)((b.tokens * rows + kRowsPerBlock - 1) / kRowsPerBlock), kThreads, 0, stream>>>(b);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
