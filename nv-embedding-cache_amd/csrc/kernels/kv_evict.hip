@@ -430,11 +430,14 @@ constexpr int kMoveAhead = 4;
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvict a, const int32_t* to, const int32_t* from,
                                                                const int32_t* counts, int64_t max_pairs) {
   __shared__ int64_t rows[kPairs][2];
-  const int64_t unit = blockIdx.x, s = unit / a.pages.heads, n = counts[unit];
-  // runs of kPairs pairs, one workgroup each in turn
-  for (int64_t p = (int64_t)blockIdx.y * kPairs; p < n; p += (int64_t)gridDim.y * kPairs)
-    move_rows<kMoveThreads, kMoveAhead>(a.pages, a.tables + s * a.table_stride, (int)(unit - s * a.pages.heads),
-                                        to + unit * max_pairs, from + unit * max_pairs, p, min(p + kPairs, n), rows);
+  const int64_t units = a.seqs * a.pages.heads;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int64_t s = unit / a.pages.heads, n = counts[unit];
+    // runs of kPairs pairs, one workgroup each in turn
+    for (int64_t p = (int64_t)blockIdx.y * kPairs; p < n; p += (int64_t)gridDim.y * kPairs)
+      move_rows<kMoveThreads, kMoveAhead>(a.pages, a.tables + s * a.table_stride, (int)(unit - s * a.pages.heads),
+                                          to + unit * max_pairs, from + unit * max_pairs, p, min(p + kPairs, n), rows);
+  }
 }
 
 // A unit's pairs: no more than slots are kept, or are dropped.
@@ -473,8 +476,8 @@ hipError_t launch_kv_evict(const KvEvict& a, void* workspace, hipStream_t stream
   // a workgroup per run of pairs, up to some rounds of the whole machine's
   const int64_t most = std::max<int64_t>(1, 16384 / units);
   const int64_t y = std::min(most, (pairs + kPairs - 1) / kPairs);
-  kv_move_kernel<<<dim3((unsigned)units, (unsigned)y), kMoveThreads, 0, stream>>>(a, to, from,
-                                                                                                     counts, pairs);
+  const int64_t x = std::min<int64_t>(units, 0xffffffffu / kMoveThreads);  // fewer than 2^32 threads
+  kv_move_kernel<<<dim3((unsigned)x, (unsigned)y), kMoveThreads, 0, stream>>>(a, to, from, counts, pairs);
   return hipGetLastError();
 }
 

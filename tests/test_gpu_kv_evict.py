@@ -190,6 +190,32 @@ def test_the_evicted_sequence_attends_to_what_is_kept():
             assert (got[2 * h + g].double() - want).abs().max() < 1e-5
 
 
+def test_more_heads_than_a_launch_has_workgroups():
+    """65,535 sequences of 257 heads, more than 2^32 threads of the kernel that moves rows; only the
+    first and the last are over the budget, and come out as they do by themselves."""
+    from pynve.torch import nve_kv
+
+    seqs, heads, page, dim, per = 65535, 257, 8, 8, 17
+    g = torch.Generator(device="cuda")
+    g.manual_seed(17)
+    shape = (2 * per, heads, page)
+    first = [torch.randn((*shape, dim), device="cuda", generator=g).half() for _ in range(2)]
+    first += [torch.rand(shape, device="cuda", generator=g)]
+    first += [torch.arange(per * page, device="cuda", dtype=torch.int32).view(per, 1, page).repeat(2, heads, 1)]
+    small = torch.arange(2 * per, device="cuda", dtype=torch.int32).view(2, per)
+    table = torch.full((seqs, per), -1, device="cuda", dtype=torch.int32)
+    lengths = torch.zeros(seqs, device="cuda", dtype=torch.int32)
+    table[0], table[-1] = small[0], small[1]
+    lengths[0] = lengths[-1] = per * page
+    got, want = [t.clone() for t in first], [t.clone() for t in first]
+    new = nve_kv.kv_evict(*got, table, lengths, 65, recent=5)
+    nve_kv.kv_evict(*want, small, torch.full((2,), per * page, device="cuda", dtype=torch.int32), 65, recent=5)
+    torch.cuda.synchronize()
+    assert new[0] == new[-1] == 65 and new.sum() == 130
+    assert not torch.equal(want[0], first[0])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_graph_replays():
     from pynve.torch import nve_kv
 
