@@ -80,7 +80,8 @@ KvAppend append_of(const nve_amd_kv_pages_t* pages, const nve_amd_kv_append_t* p
   check_dtype(a.pages, p->dtype);
   NVE_CHECK_ARG(p->num_tokens >= 0, "Invalid num_tokens ", p->num_tokens);
   a.q_heads = p->q ? p->num_q_heads : 0;
-  NVE_CHECK_ARG(a.q_heads >= 0, "Invalid num_q_heads ", p->num_q_heads);
+  // the launches go by whole tokens, of fewer than 2^26 rows
+  NVE_CHECK_ARG(a.q_heads >= 0 && a.q_heads < (1 << 25), "Invalid num_q_heads ", p->num_q_heads);
   NVE_CHECK_ARG(p->num_tokens <= kMaxGrid / (a.q_heads + 2 * (int64_t)a.pages.heads), "Too many tokens");
   if (p->num_tokens > 0) {
     NVE_CHECK_ARG(p->slots && p->k && p->v, "slots, k and v must not be NULL");
@@ -131,6 +132,9 @@ KvAttend attend_of(const nve_amd_kv_pages_t* pages, const nve_amd_kv_attend_t* p
   NVE_CHECK_ARG(p->num_seqs >= 0 && p->num_seqs <= 65535, "num_seqs must be in [0, 65535] (got ", p->num_seqs, ")");
   NVE_CHECK_ARG(p->num_q_heads >= 1 && p->num_q_heads <= 65535 && p->num_q_heads % a.pages.heads == 0,
                 "num_q_heads (", p->num_q_heads, ") must be a multiple of the pages' num_heads (", a.pages.heads, ")");
+  // a workgroup of 256 threads for each, and a launch has fewer than 2^32 threads
+  NVE_CHECK_ARG(p->num_seqs * a.pages.heads < (1 << 24), "Too many heads: ", p->num_seqs, " sequences of ",
+                a.pages.heads);
   NVE_CHECK_ARG(!std::isnan(p->scale), "scale must not be NaN");
   a.max_length = extent(a.pages, p->max_pages, p->max_length);
   // the kernels count tiles of at least 64 slots in 32 bits

@@ -124,6 +124,18 @@ def test_evict_needs_weights_index_and_a_workspace():
     assert "orkspace" in _lib.last_error()
 
 
+def test_more_heads_than_a_launch_has_workgroups():
+    """A launch has fewer than 2^32 threads: 2^24 heads of sequences are refused, one less is not."""
+    n = ctypes.c_uint64()
+    p, c = pages(num_heads=1 << 9), attend(num_seqs=1 << 15, num_q_heads=1 << 9, max_pages=1)
+    assert call("nve_amd_kv_attend", p, c) == _lib.INVALID_ARGUMENT
+    assert "Too many heads" in _lib.last_error()
+    c.num_seqs -= 1
+    _lib.call("nve_amd_kv_attend_workspace_size", ctypes.byref(p), ctypes.byref(c), ctypes.byref(n))
+    assert call("nve_amd_kv_append", pages(), append(num_tokens=1, num_q_heads=1 << 25)) == _lib.INVALID_ARGUMENT
+    assert "num_q_heads" in _lib.last_error()
+
+
 @pytest.mark.parametrize("offset", [0, 4, 8, -4, -8])
 def test_evict_in_place_lengths_are_refused(offset):
     """A sequence's heads read its length while the first of them writes the new one."""
