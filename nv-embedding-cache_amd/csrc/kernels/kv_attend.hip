@@ -81,8 +81,12 @@ struct Plan {
   int32_t query_tiles, group, tile;
   int32_t chunk, pieces;  // grid mode: tiles of a piece, pieces of a unit at most
   int32_t workgroups;     // stream mode
-  int64_t padded;         // slots of a row of scores
-  float* scores;          // [seqs * q_heads, padded], log2 units (accumulate)
+  // Scores in log2 units (accumulate): rows of score_row floats, one per query head of the call
+  // with its sequence's slots in order, or (by_slot) one per query of a group with the cache's
+  // slots as the weights have them.
+  int32_t by_slot;
+  int64_t score_row;
+  float* scores;
   float* slot_ml;         // [slots, query_tiles, 2, 16]
   float* slot_rows;       // [slots, query_tiles, 16, dim padded]
   struct Slot* slots;     // [2 * workgroups] (stream mode)
@@ -249,6 +253,11 @@ __device__ __forceinline__ words<N> load_words(const uint8_t* src) {
   return *(const __attribute__((address_space(1))) any*)(uintptr_t)src;
 }
 
+// The first row of scores of a unit's query tile.
+__device__ __forceinline__ int64_t score_row_of(const KvAttend& a, const Plan& p, const Piece& u, int query_tile) {
+  return (p.by_slot ? 0 : u.seq * (int64_t)a.q_heads + (int64_t)u.head * p.group) + query_tile * 16;
+}
+
 // The weights of a piece's slots under `rows` softmaxes whose sums are all[]; four slots a
 // thread, which lie in one page.
 __device__ __forceinline__ void add_weights(const KvAttend& a, const Plan& p, const Piece& u, int query_tile,
@@ -256,17 +265,17 @@ __device__ __forceinline__ void add_weights(const KvAttend& a, const Plan& p, co
   typedef f32x4 __attribute__((aligned(4))) f4;
   const int64_t t1 = min((int64_t)u.last * p.tile, u.len);
   const int rows = min(16, p.group - query_tile * 16);
-  const float* scores =
-      p.scores + (u.seq * (int64_t)a.q_heads + (int64_t)u.head * p.group + query_tile * 16) * p.padded;
+  const float* scores = p.scores + score_row_of(a, p, u, query_tile) * p.score_row;
   for (int64_t t = (int64_t)u.first * p.tile + 4 * threadIdx.x; t < t1; t += 4 * 256) {
     const int64_t page = kv_page(a.pages, a.tables + u.seq * a.table_stride, t);
     if (page < 0) continue;
-    float* to = a.pages.weights + kv_row(a.pages, page, u.head, t);
+    const int64_t row = kv_row(a.pages, page, u.head, t), at = p.by_slot ? row : t;
+    float* to = a.pages.weights + row;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int q0 = 0; q0 < rows; q0 += 4) {  // four rows' loads together
       f32x4 x[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const f32x4*>(scores + min(q0 + j, rows - 1) * p.padded + t);
+      for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const f32x4*>(scores + min(q0 + j, rows - 1) * p.score_row + at);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // an empty softmax has no weights, nor has a row past the last
@@ -452,6 +461,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
     x.m = -INFINITY;
     x.l = 0.0f;
 
+    float* score_row = nullptr;  // of this lane's query
+    if constexpr (ACC) score_row = p.scores + (score_row_of(a, p, u, query_tile) + c) * p.score_row;
     const int32_t* table = a.tables + u.seq * a.table_stride;
     const int steps = u.last - u.first;
     const int64_t t_base = (int64_t)u.first * (kWaves * kStep) + wave * kStep;  // this wave's first slot
@@ -535,9 +546,10 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
           }
         }
         if constexpr (ACC) {
-          if (there && t < u.len)  // rows of scores are padded to whole tiles
-            *reinterpret_cast<f32x4*>(p.scores + (u.seq * a.q_heads + q_head) * p.padded + t) =
-                f32x4{y[n * 4], y[n * 4 + 1], y[n * 4 + 2], y[n * 4 + 3]};
+          if (there && id >= 0 && t < u.len) {  // rows of scores are padded to whole tiles or pages
+            const int64_t at = p.by_slot ? kv_row(pages, id, u.head, t) : t;
+            *reinterpret_cast<f32x4*>(score_row + at) = f32x4{y[n * 4], y[n * 4 + 1], y[n * 4 + 2], y[n * 4 + 3]};
+          }
         }
       }
       if constexpr (more) {
@@ -852,6 +864,8 @@ int64_t grid_chunk(int64_t seqs, int64_t units, int64_t tiles, int tile) {
   return pieces == 1 || units * pieces <= 8192 ? chunk : 0;
 }
 
+constexpr int64_t kFewScores = 32 << 20;  // 128 MiB
+
 Layout layout_of(const KvAttend& a, void* workspace) {
   Layout r{};
   Plan& p = r.plan;
@@ -861,7 +875,6 @@ Layout layout_of(const KvAttend& a, void* workspace) {
   const int64_t tiles = std::max<int64_t>(1, (a.max_length + p.tile - 1) / p.tile);
   const int64_t units = a.seqs * a.pages.heads;
   r.units = (unsigned)units;
-  p.padded = tiles * p.tile;
   const int dp = padded_dim(a.pages.dim);
   const int64_t chunk = grid_chunk(a.seqs, units, tiles, p.tile);
   r.grid = chunk > 0;
@@ -879,7 +892,15 @@ Layout layout_of(const KvAttend& a, void* workspace) {
   p.slot_rows = static_cast<float*>(take(slots * p.query_tiles * 16 * dp * 4));
   p.slot_ml = static_cast<float*>(take(slots * p.query_tiles * 32 * 4));
   if (!r.grid) p.slots = static_cast<Slot*>(take(slots * sizeof(Slot)));
-  if (a.accumulate) p.scores = static_cast<float*>(take((size_t)a.seqs * a.q_heads * p.padded * 4));
+  if (a.accumulate) {
+    // Sequences may be far shorter than their tables: no page belongs to two of them, so scores by
+    // slot hold no more than the cache.  In order they are read in longer runs (64 sequences of 512 to
+    // 8,192 slots, 32 query heads: 180 us, by slot 187), so that is left where it saves little.
+    const int64_t in_order = a.seqs * a.q_heads * tiles * p.tile, of_cache = a.pages.num_pages * a.pages.page * a.q_heads;
+    p.by_slot = in_order > kFewScores && in_order > 4 * of_cache;
+    p.score_row = p.by_slot ? of_cache / p.group : tiles * p.tile;
+    p.scores = static_cast<float*>(take((size_t)(p.by_slot ? of_cache : in_order) * 4));
+  }
   return r;
 }
 

@@ -144,6 +144,44 @@ def test_tables_far_longer_than_the_sequences(dtype, cache, accumulate, dim):
     check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
 
 
+@pytest.mark.parametrize("page", [8, 32])
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_weights_in_tables_wider_than_the_cache(dtype, cache, page):
+    """Tables of 32,768 slots, 60 sequences of 40 query heads in pieces: the weights' scores lie by the cache's slots."""
+    rng = np.random.default_rng(24)
+    s = setup(dtype, cache, [2100, 3, 1500, 0, 1, 700] + [int(n) for n in rng.integers(0, 40, size=54)], 40, 2, 64, page,
+              seed=25)
+    wide = np.full((60, 32768 // page), -1, np.int32)
+    wide[:, :s["table"].shape[1]] = s["table"]
+    s["table"] = wide
+    s["table"][0, 7], s["table"][2, 1] = -1, s["k"].shape[0]
+    poison_unused(s)
+    check(s, 0.125, call(s, 0.125))
+
+
+@pytest.mark.parametrize("dtype,cache", [("f16", "f16"), ("f32", "f32")])
+def test_weights_of_many_short_sequences_in_wide_tables(dtype, cache):
+    """A workgroup a unit, scores by slot (2,100 sequences) and in order (half of them): the same bits."""
+    rng = np.random.default_rng(26)
+    s = setup(dtype, cache, [int(n) for n in rng.integers(0, 60, size=2100)], 32, 2, 64, 16, seed=27)
+    wide = np.full((2100, 16 if dtype == "f32" else 32), -1, np.int32)
+    wide[:, :s["table"].shape[1]] = s["table"]
+    s["table"] = wide
+    if dtype == "f32":  # a workgroup a unit up to 256 slots
+        for n in ("q", "table", "lengths"):
+            s[n] = np.concatenate([s[n]] * 2) if n != "q" else torch.cat([s[n]] * 2)
+        s["lengths"][2100:] = 0
+    out, lse, w = call(s, 0.125)
+    n = len(s["lengths"]) // 2
+    w2 = s["weights"]
+    for part in (slice(0, n), slice(n, 2 * n)):
+        h = {**s, "q": s["q"][part], "table": np.ascontiguousarray(s["table"][part]), "lengths": s["lengths"][part],
+             "weights": w2}
+        o2, l2, w2 = call(h, 0.125)
+        assert torch.equal(out[part], o2) and torch.equal(lse[part], l2)
+    assert torch.equal(w, w2) and not torch.equal(w, s["weights"])
+
+
 @pytest.mark.parametrize("dtype,cache", [("f16", "f16"), ("f32", "f32")])
 @pytest.mark.parametrize("q_heads", [34, 40])
 def test_wide_groups_in_long_tables(dtype, cache, q_heads):

@@ -124,6 +124,26 @@ def test_evict_needs_weights_index_and_a_workspace():
     assert "orkspace" in _lib.last_error()
 
 
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_attend_workspace_is_bounded_by_the_cache_and_by_the_tables(accumulate):
+    """128 MiB of scores, or 4 for every slot there is, not one for every entry that the tables have room
+    for; and none for the pages of a large cache that the tables cannot name."""
+    def need(num_pages, seqs, max_pages):
+        n = ctypes.c_uint64()
+        p = pages(num_pages=num_pages, page_size=16, num_heads=8, head_dim=128)
+        c = attend(num_seqs=seqs, num_q_heads=64, max_pages=max_pages, table_stride=max_pages, accumulate=accumulate)
+        _lib.call("nve_amd_kv_attend_workspace_size", ctypes.byref(p), ctypes.byref(c), ctypes.byref(n))
+        return n.value
+
+    # rows, maxima and sums of the pieces: no more than of 8,192 pieces of 16 queries
+    pieces = 8192 * 16 * (128 + 2) * 4 + (1 << 20)
+    for max_pages in (16, 1024, 8192, 1 << 17):
+        for num_pages in (2000, 50000):
+            assert need(num_pages, 256, max_pages) <= pieces + accumulate * max(1 << 27, 4 * 64 * num_pages * 16 * 4)
+    for num_pages in (100, 10000, 1 << 24):
+        assert need(num_pages, 2, 50) <= pieces + accumulate * 2 * 64 * 1024 * 4
+
+
 def test_more_heads_than_a_launch_has_workgroups():
     """A launch has fewer than 2^32 threads: 2^24 heads of sequences are refused, one less is not."""
     n = ctypes.c_uint64()
