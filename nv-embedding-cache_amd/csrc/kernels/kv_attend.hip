@@ -79,7 +79,7 @@ constexpr int step_slots(int qt) { return qt == kF32 ? 16 : 32; }
 // A unit is a (sequence, key head); a piece a run of its tiles in one workgroup.
 struct Plan {
   int32_t query_tiles, group, tile;
-  int32_t chunk, pieces;  // grid mode: tiles of a piece, pieces of a unit at most
+  int32_t chunk, pieces;  // grid mode: tiles of a piece (0: by the length), pieces of a unit at most
   int32_t workgroups;     // stream mode
   // Scores in log2 units (accumulate): rows of score_row floats, one per query head of the call
   // with its sequence's slots in order, or (by_slot) one per query of a group with the cache's
@@ -111,6 +111,11 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // Tiles of a sequence; one at least, so that an empty one is visited.
 __device__ __forceinline__ int tiles_of(const Plan& p, int64_t len) {
   return len <= p.tile ? 1 : (int)((len + p.tile - 1) / p.tile);
+}
+
+// Grid mode: tiles of a unit's pieces.
+__device__ __forceinline__ int chunk_of(const Plan& p, int tiles) {
+  return p.chunk > 0 ? p.chunk : (tiles + p.pieces - 1) / p.pieces;
 }
 
 // Stream mode: all tiles of the call, end to end, in shares that differ by one tile at most.
@@ -656,8 +661,9 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
     u.head = unit - u.seq * pages.heads;
     u.len = kv_length(a.lengths, u.seq, a.max_length);
     u.tiles = tiles_of(p, u.len);
-    u.first = blockIdx.y * p.chunk;
-    u.last = min(u.first + p.chunk, u.tiles);
+    const int chunk = chunk_of(p, u.tiles);
+    u.first = blockIdx.y * chunk;
+    u.last = min(u.first + chunk, u.tiles);
     if (u.first >= u.tiles) return;
     for (int qt = 0; qt < p.query_tiles; ++qt) process(u, qt, unit * p.pieces + blockIdx.y);
   } else {
@@ -758,9 +764,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend a, const Pl
     u.len = kv_length(a.lengths, u.seq, a.max_length);
     u.tiles = tiles_of(p, u.len);
     me = blockIdx.y;
-    u.first = me * p.chunk;
-    u.last = min(u.first + p.chunk, u.tiles);
-    w.count = (u.tiles + p.chunk - 1) / p.chunk;
+    const int chunk = chunk_of(p, u.tiles);
+    u.first = me * chunk;
+    u.last = min(u.first + chunk, u.tiles);
+    w.count = (u.tiles + chunk - 1) / chunk;
     w.head = unit * p.pieces;
     w.next = w.head + 1;
     w.step = 1;
@@ -847,8 +854,9 @@ struct Layout {
 //   Whole units, one launch, up to 4 tiles (one piece 12.2 us, 32 pieces and a join 10.3 us for one
 //   sequence of 4,096 slots, but 34.9 against 43.4 us for 256 of 32 to 512), and up to 16 where
 //   there are units for all CUs (64 sequences of 125 to 2,000 slots: whole 33.9, pieces of 8 42.3).
-//   One sequence is as long as its table: 256 pieces, one a CU, are enough (200,001 slots: 144 us,
-//   stream 155, pieces of 16 tiles 165; 16,384: 17.7, stream 23.6, 1 tile 22.0).
+//   One sequence: 256 pieces, one a CU, are enough (200,001 slots: 144 us, stream 155, pieces of 16
+//   tiles 165; 16,384: 17.7, stream 23.6, 1 tile 22.0). Its tiles are shared by these pieces as its
+//   length asks for, which only the kernels know: its table may be far longer.
 //   Several may be much shorter than the longest: smaller pieces (7 of 33 to 30,011 slots, 2 key
 //   heads: pieces of 4 tiles 22 us, 8 29, stream 35; 64 of 512 to 8,192: 8 tiles 180, 16 188, stream 186).
 //   In f32 (64-slot tiles) 8 is the most: 48 sequences of up to 2,000 slots 30.5 us, 12 32.2.
@@ -878,7 +886,7 @@ Layout layout_of(const KvAttend& a, void* workspace) {
   const int dp = padded_dim(a.pages.dim);
   const int64_t chunk = grid_chunk(a.seqs, units, tiles, p.tile);
   r.grid = chunk > 0;
-  p.chunk = (int)chunk;
+  p.chunk = a.seqs == 1 ? 0 : (int)chunk;
   p.pieces = r.grid ? (int)((tiles + chunk - 1) / chunk) : 0;
   // what the 256 CUs hold at once
   p.workgroups = (int)std::min<int64_t>(256 * waves_per_simd(dp), units * tiles);

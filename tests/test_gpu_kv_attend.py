@@ -144,6 +144,52 @@ def test_tables_far_longer_than_the_sequences(dtype, cache, accumulate, dim):
     check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("length,width", [(0, 1 << 20), (1, 131072), (100, 131072), (777, 1 << 20), (4000, 131072),
+                                          (20011, 1 << 20)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_one_sequence_in_a_wide_table(dtype, cache, length, width, accumulate):
+    """Pieces by the sequence's length: the result of a table that fits, bit for bit."""
+    s = setup(dtype, cache, [length], 6, 2, 64, 16, seed=28, extra=1)
+    poison_unused(s)
+    wide = {**s, "table": np.full((1, width // 16), -1, np.int32)}
+    wide["table"][:, :s["table"].shape[1]] = s["table"]
+    got = call(wide, 0.125, accumulate)
+    check(s, 0.125, got)
+    if length > 512:
+        for a, b in zip(got, call(s, 0.125, accumulate)):
+            assert a is b is None or torch.equal(a, b)
+
+
+def test_one_sequence_takes_no_longer_in_a_wide_table():
+    """32,000 slots in a table of 2^20, on as many workgroups as in a table that fits (it took 10 times as long on
+    the few pieces that the table's width gave them)."""
+    from pynve.torch import nve_kv
+
+    pages = 2000
+    k = torch.randn((pages, 8, 16, 128), device="cuda").half()
+    v, q = torch.randn_like(k), torch.randn((1, 32, 128), device="cuda").half()
+    length = torch.tensor([pages * 16], dtype=torch.int32, device="cuda")
+    tight = torch.randperm(pages, device="cuda").int().view(1, -1)
+    wide = torch.full((1, 1 << 16), -1, dtype=torch.int32, device="cuda")
+    wide[:, :pages] = tight
+
+    def time(table):
+        best = math.inf
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            nve_kv.kv_attend(q, k, v, table, length)
+            start.record()
+            for _ in range(20):
+                nve_kv.kv_attend(q, k, v, table, length)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best
+
+    assert time(wide) < 4 * time(tight)
+
+
 @pytest.mark.parametrize("page", [8, 32])
 @pytest.mark.parametrize("dtype,cache", TYPES)
 def test_weights_in_tables_wider_than_the_cache(dtype, cache, page):
