@@ -144,6 +144,21 @@ def test_tables_far_longer_than_the_sequences(dtype, cache, accumulate, dim):
     check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
 
 
+@pytest.mark.parametrize("dim", [8, 56, 192, 248])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_partly_filled_widths_in_tables_far_longer(dtype, cache, accumulate, dim):
+    """The kernels for up to 64 and up to 256 values with narrower rows, their workgroups sharing the slots there are."""
+    rng = np.random.default_rng(29)
+    lengths = [int(n) for n in rng.integers(0, 40, size=95)] + [2500, 0, 777, 1, 1300]
+    s = setup(dtype, cache, lengths, 6, 3, dim, 16, seed=30)
+    wide = np.full((len(lengths), 8192), -1, np.int32)
+    wide[:, :s["table"].shape[1]] = s["table"]
+    s["table"] = wide
+    poison_unused(s)
+    check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
+
+
 @pytest.mark.parametrize("dtype,cache", TYPES)
 @pytest.mark.parametrize("length,width", [(0, 1 << 20), (1, 131072), (100, 131072), (777, 1 << 20), (4000, 131072),
                                           (20011, 1 << 20)])
