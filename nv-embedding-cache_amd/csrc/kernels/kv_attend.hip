@@ -23,7 +23,9 @@
 //
 // Weights enter the second product as the sum of two values of the product's
 // type (at least 16 bits of the f32 weight): one alone would lose as much as the
-// output's own rounding, and the matrix units are idle anyway.  f16 weights are
+// output's own rounding, and the matrix units are idle anyway.  The first is rounded
+// towards zero and the second is not zero beside it, so that both have the weight's
+// sign and an infinite value gives an infinity, not a NaN.  f16 weights are
 // held times 2^14, so that a long flat tail does not underflow (2^-38 of the
 // maximum still counts).  e4m3 rows are widened exactly to the query's type
 // (scores) and to bf16 (values); their scales go into scores and weights.
@@ -226,6 +228,23 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, bhalf2{(__bf16)a, (__bf16)b});
   }
 }
+// Rounded towards zero.
+template <int QT>
+__device__ __forceinline__ uint32_t pack2_down(float a, float b) {
+  if constexpr (QT == kF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  else
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+// The type's least positive value in place of a zero beside a high half that is none.
+template <int QT>
+__device__ __forceinline__ uint32_t at_least_one(uint32_t low, uint32_t high) {
+  using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
+  const u16x2 one = {1, 1};
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_elementwise_max(__builtin_bit_cast(u16x2, low),
+                                                      __builtin_elementwise_min(__builtin_bit_cast(u16x2, high), one)));
+}
 template <int QT>
 __device__ __forceinline__ float low_of(uint32_t w) {
   if constexpr (QT == kF16) return (float)__builtin_bit_cast(_Float16, (uint16_t)w);
@@ -408,8 +427,9 @@ struct Wave {
       u32x4 high, low;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        high[i] = pack2<VT>(p[2 * i], p[2 * i + 1]);
-        low[i] = pack2<VT>(p[2 * i] - low_of<VT>(high[i]), p[2 * i + 1] - high_of<VT>(high[i]));
+        high[i] = pack2_down<VT>(p[2 * i], p[2 * i + 1]);
+        const uint32_t rest = pack2<VT>(p[2 * i] - low_of<VT>(high[i]), p[2 * i + 1] - high_of<VT>(high[i]));
+        low[i] = at_least_one<VT>(rest, high[i]);
       }
       uint32_t w[8][kValues / 2];
 #pragma unroll

@@ -144,6 +144,35 @@ def test_tables_far_longer_than_the_sequences(dtype, cache, accumulate, dim):
     check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES[:3])
+@pytest.mark.parametrize("length", [1, 30, 700, 5000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinite_values(dtype, cache, length, sign):
+    """An infinity among the values is the output in its column, as in the formula; both signs give NaN there."""
+    s = setup(dtype, cache, [length, length], 4, 2, 64, 16, seed=31)
+    s["q"] *= 0.25  # no weight below 2^-38 of the largest
+    at = np.random.default_rng(32).integers(0, length, size=3)
+    for i, (where, d) in enumerate(zip(at, (3, 40, 63))):
+        s["v"][int(s["table"][0, where // 16]), :, int(where) % 16, d] = sign * math.inf * (-1) ** i
+    both = length > 1
+    if both:
+        a, b = 0, length - 1
+        s["v"][int(s["table"][0, a // 16]), :, a % 16, 20] = math.inf
+        s["v"][int(s["table"][0, b // 16]), :, b % 16, 20] = -math.inf
+    out, lse, w = call(s, 0.125)
+    assert torch.isfinite(lse).all() and torch.isfinite(w).all()
+    for i, d in enumerate((3, 40, 63)):
+        assert (out[0, :, d] == sign * math.inf * (-1) ** i).all(), d
+    if both:
+        assert torch.isnan(out[0, :, 20]).all()
+    other = torch.ones(64, dtype=torch.bool)
+    other[[3, 40, 63] + [20] * both] = False
+    finite = {**s, "v": torch.nan_to_num(s["v"], posinf=0.0, neginf=0.0)}
+    clean = call(finite, 0.125)
+    assert torch.equal(out[0][:, other], clean[0][0][:, other]) and torch.equal(out[1], clean[0][1])
+    check(finite, 0.125, clean)
+
+
 @pytest.mark.parametrize("dim", [8, 56, 192, 248])
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("dtype,cache", TYPES)
