@@ -266,8 +266,8 @@ NVE_C_API nve_status_t nve_amd_kv_append(const nve_amd_kv_pages_t* pages,
  * log sum_t exp(x_t).  Where no slot has a score above -infinity (a length of
  * zero, say) out is 0 and lse -infinity.  What lies in a page's rows at or past
  * the length is not used, whatever it is.  Scores, lse, sums and the weights that
- * are added are f32; the p_t that meet 16- and 8-bit values keep 16 bits at least,
- * and for FLOAT16 pages those below 2^-38 of the largest count as 0.  accumulate:
+ * are added are f32; the p_t that meet FLOAT16 values keep 22 bits and those below
+ * 2^-38 of the largest count as 0, the p_t that meet E4M3 values keep 17.  accumulate:
  * p_t, summed over the query heads of a key head, is added to pages->weights;
  * no page may then belong to two sequences of the call.  max_length: the
  * longest length that occurs, if the caller knows it (0: the table's extent);

@@ -21,11 +21,13 @@
 // pieces contiguous.  No shared memory until the waves of a workgroup join.
 // f32 has the same layout with 16 slots a step and products of one value a lane.
 //
-// Weights enter the second product as the sum of two values of the product's
-// type (at least 16 bits of the f32 weight): one alone would lose as much as the
-// output's own rounding, and the matrix units are idle anyway.  The first is rounded
-// towards zero and the second is not zero beside it, so that both have the weight's
-// sign and an infinite value gives an infinity, not a NaN.  f16 weights are
+// Weights enter the second product as a sum of values of the product's type; one alone
+// would lose as much as the output's own rounding, and the matrix units are idle
+// anyway.  Three of bf16 hold all of an f32 weight, two of f16 22 bits of it.  All but
+// the last are rounded towards zero and none is zero beside the first, so that all have
+// the weight's sign and an infinite value gives an infinity, not a NaN.  e4m3 values,
+// of 4 bits and never infinite, get two of bf16, each rounded to nearest: 17 bits
+// (64 sequences of 2,000 slots of 64 values: 23.7 us, three 25.1).  f16 weights are
 // held times 2^14, so that a long flat tail does not underflow (2^-38 of the
 // maximum still counts).  e4m3 rows are widened exactly to the query's type
 // (scores) and to bf16 (values); their scales go into scores and weights.
@@ -237,7 +239,6 @@ __device__ __forceinline__ uint32_t pack2_down(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 // The type's least positive value in place of a zero beside a high half that is none.
-template <int QT>
 __device__ __forceinline__ uint32_t at_least_one(uint32_t low, uint32_t high) {
   using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
   const u16x2 one = {1, 1};
@@ -331,6 +332,7 @@ struct Wave {
   static constexpr int kValues = DP / 16;          // values of a v row in a lane, and output tiles
   static constexpr int kVWords = kValues * kBytes / 4;
   static constexpr int VT = CT == kE4M3 ? kBF16 : QT;  // the type of the second product
+  static constexpr int kParts = CT == kBF16 ? 3 : 2;    // of a weight
   static constexpr int kQWords = QT == kF32 ? DP / 4 : kSteps * 4;
 
   static constexpr int kVLoad = !EXACT && CT == kE4M3 ? (kVWords < 2 ? 1 : 2) : kVWords < 4 ? kVWords : 4;
@@ -424,12 +426,18 @@ struct Wave {
         for (int r = 0; r < 4; ++r)
           acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j / kVLoad][j % kVLoad]), p[r], acc[j], 0, 0, 0);
     } else {
-      u32x4 high, low;
+      u32x4 part[kParts];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        high[i] = pack2_down<VT>(p[2 * i], p[2 * i + 1]);
-        const uint32_t rest = pack2<VT>(p[2 * i] - low_of<VT>(high[i]), p[2 * i + 1] - high_of<VT>(high[i]));
-        low[i] = at_least_one<VT>(rest, high[i]);
+        float a = p[2 * i], b = p[2 * i + 1];
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) {
+          const bool last = n == kParts - 1;
+          const uint32_t w = CT == kE4M3 || (last && VT == kF16) ? pack2<VT>(a, b) : pack2_down<VT>(a, b);
+          a -= low_of<VT>(w);
+          b -= high_of<VT>(w);
+          part[n][i] = CT == kE4M3 || n == 0 ? w : at_least_one(w, part[0][i]);
+        }
       }
       uint32_t w[8][kValues / 2];
 #pragma unroll
@@ -447,8 +455,8 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           x[i] = __builtin_amdgcn_perm(w[2 * i + 1][j / 2], w[2 * i][j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
-        acc[j] = mma<VT>(x, high, acc[j]);
-        acc[j] = mma<VT>(x, low, acc[j]);
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) acc[j] = mma<VT>(x, part[n], acc[j]);
       }
     }
   }

@@ -144,6 +144,41 @@ def test_tables_far_longer_than_the_sequences(dtype, cache, accumulate, dim):
     check(s, dim**-0.5, call(s, dim**-0.5, accumulate))
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_weights_keep_their_bits(dtype, cache):
+    """Values that cancel under the exact weights leave what the weights lost: all but 2^-22 of them is kept, 2^-17
+    beside e4m3 values (of f32 statistics, D products added in f32, an exp2 and a sum)."""
+    n, dim, scale = 200, 8, 0.35
+    s = setup(dtype, cache, [4] * n, 2, 2, dim, 16, seed=33, q_spread=2.0**-6)
+    q = s["q"].double().numpy()
+    k = R.values64(s["k"], s["ks"])
+    want, mass, size = np.zeros((n, 2, 1)), np.zeros((n, 2, 1)), np.zeros((n, 2, 1))
+    for i in range(n):
+        page = int(s["table"][i, 0])
+        for h in range(2):
+            x = scale * k[page, h, :4] @ q[i, h]
+            w = np.exp(x - x.max())
+            w /= w.sum()
+            left = 0.0
+            for t in range(4):  # the first value is 1, the others take back what the sum is so far
+                v = 1.0 if t == 0 else -left / w[t]
+                if cache == "e4m3":
+                    s["v"][page, h, t] = math.copysign(1.0, v)
+                    s["vs"][page, h, t] = abs(v)
+                    v = math.copysign(float(s["vs"][page, h, t]), v)
+                else:
+                    s["v"][page, h, t] = v
+                    v = float(s["v"][page, h, t, 0])
+                left += w[t] * v
+                mass[i, h] += w[t] * abs(v)
+            want[i, h], size[i, h] = left, scale * (np.abs(k[page, h, :4]) @ np.abs(q[i, h])).max()
+    out = call(s, scale)[0].double().numpy()
+    rel = 2 * (dim + 8) * 2.0**-24 * size + 2.0**-20 + 2.0**-23 * math.log2(5) + (2.0**-17 if cache == "e4m3" else 2.0**-22)
+    bound = rel * mass * 1.01 + R.HALF_ULP[dtype] * np.maximum(np.abs(want) + rel * mass, R.SMALL[dtype])
+    err = np.abs(out - want)
+    assert (err <= bound).all(), f"{(err / bound).max()} times the bound"
+
+
 @pytest.mark.parametrize("dtype,cache", TYPES[:3])
 @pytest.mark.parametrize("length", [1, 30, 700, 5000])
 @pytest.mark.parametrize("sign", [1, -1])
