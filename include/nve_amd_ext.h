@@ -304,7 +304,8 @@ NVE_C_API nve_status_t nve_amd_kv_attend(const nve_amd_kv_pages_t* pages,
  * up to the head's newest index, a NaN weight is the greatest and slots of
  * absent pages come first.  The j-th dropped slot below `budget` then takes the
  * row (k, v, scales, weight, index) of the j-th kept slot at or past it;
- * nothing else is written.  new_lengths[s] = min(lengths[s], budget); the two
+ * nothing else is written, so a row whose gap lies in an absent page is lost
+ * (absent pages belong behind a table's others).  new_lengths[s] = min(lengths[s], budget); the two
  * may not overlap.  No page may belong to two sequences of the call.
  * workspace: device memory of nve_amd_kv_evict_workspace_size bytes, 16-byte
  * aligned. */

@@ -23,8 +23,8 @@
 // a digit, because weights that fall off over some binades share their first 8
 // bits: their additions to one bin would queue.
 // Measured: 64 sequences of 2,064 slots and 8 key heads to 2,048: 15 us
-// repeated on one cache, 17 to 19 on a fresh one; 8 prompts of 32,768 slots to 4,096: 41
-// to 45 us to choose (64 workgroups on 256 CUs) and 59 to 73 to move the rows of a fresh
+// repeated on one cache, 16 to 19 on a fresh one; 8 prompts of 32,768 slots to 4,096: 41
+// to 44 us to choose (64 workgroups on 256 CUs) and 58 to 74 to move the rows of a fresh
 // cache, 35 and 9 once repeated, as fewer rows then move.
 #include <algorithm>
 #include <type_traits>
@@ -40,7 +40,10 @@ using i32x4 = __attribute__((ext_vector_type(4))) int32_t;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 constexpr int kBins = 2048;
-constexpr int64_t kFewPairs = 64;  // of a unit: copied by the selecting workgroup
+// Pairs of a unit that the selecting workgroup copies itself.  One launch / two, us a call on fresh
+// caches, 8 key heads of 128 bf16 values: 64 sequences of 2,000 slots, 64 pairs 19.2 / 22.3, 256 pairs
+// 34.8 / 36.0, 512 59.2 / 56.0; 8 sequences 14.4 / 17.7, 128 pairs 17.6 / 18.5, 256 20.6 / 18.6.
+constexpr int64_t kFewPairs = 64;
 
 // Ascending order of the keys is that of the weights: -infinity first, NaN
 // last, the two zeros equal.  No weight has one of the keys below.
@@ -461,6 +464,12 @@ hipError_t launch_kv_evict(const KvEvict& a, void* workspace, hipStream_t stream
   int32_t* counts = from + units * pairs;
   const int few = pairs <= kFewPairs;
   const dim3 grid((unsigned)a.seqs, (unsigned)a.pages.heads);
+  // The fewest slots a thread that hold what the tables can name: a variant goes through all of its
+  // slots whatever the lengths are (64 sequences of 2,064 slots, 16 pairs, us a call: 16 slots a thread
+  // 15.8, 32 26.2, 64 58.8; of 1,024: 4 slots 11.0, 16 15.0).  Without registers places and weights
+  // are read again in every pass (9,000 slots: 32 a thread 28.8, none 48; 8 sequences of 16,384: 22.2 and
+  // 31.2; of 32,768: 64 a thread 37.2, none 49.4), which is slower at these limits, though not for
+  // sequences far shorter than their tables (2,064 slots: none 29.8).
   if (a.max_length <= 1024)
     kv_select_kernel<256, 4><<<grid, 256, 0, stream>>>(a, to, from, counts, pairs, few);
   else if (a.max_length <= 4096)

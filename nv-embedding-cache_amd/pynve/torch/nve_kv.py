@@ -12,7 +12,8 @@ operators work on the pages, each one a hand-written HIP kernel behind the C ABI
   kv_evict    drops the slots of the least accumulated weight from sequences that are over a budget
 
 `KVCache` holds the pages and calls the three.  Everything runs on the current
-stream of the pages' GPU, nothing waits for the GPU, and nothing has a gradient.
+stream of the pages' GPU, nothing waits for the GPU, and nothing has a gradient:
+inputs that ask for one are refused unless gradients are off.
 
 Shapes (P pages, H key heads, `page` slots a page, D values a head row, S sequences, T tokens):
 
@@ -65,9 +66,10 @@ def kv_attend(q, k_pages, v_pages, block_tables, lengths, *, scale=None, k_scale
     type, with `return_lse` also the logarithm of each softmax's sum, float32
     [S, Hq].  A sequence without slots gives zeros (and -inf).  With `weights` the
     softmax of every slot, summed over the query heads of its key head, is added
-    there; no page may then belong to two of the sequences.  `max_length` is a
-    bound on the lengths if the caller knows one below the tables' extent; it
-    sizes the launch and the workspace."""
+    there; no page may then belong to two of the sequences.  Sums are float32; the
+    softmax values that meet float16 values keep 22 bits, those that meet float8
+    values 17.  `max_length` is a bound on the lengths if the caller knows one below
+    the tables' extent; it sizes the launch and the workspace."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     f = _attend_lse if return_lse else _attend
@@ -82,7 +84,8 @@ def kv_evict(k_pages, v_pages, weights, index_pages, block_tables, lengths, budg
     those among the `recent` places up to its newest index.  Kept slots past the
     budget move into the gaps below it, so the order of the slots changes
     (attention does not depend on it; index_pages says which token a slot holds).
-    Pages past ceil(new length / page) are free for other sequences."""
+    Pages past ceil(new length / page) are free for other sequences.  A row whose
+    gap lies in an absent page is lost: absent pages belong behind a table's others."""
     return _evict(k_pages, v_pages, weights, index_pages, block_tables, lengths, budget, sinks, recent, k_scale,
                   v_scale)
 
