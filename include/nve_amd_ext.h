@@ -20,10 +20,17 @@ extern "C" {
  *   NVE_DTYPE_X_INT8_AFFINE_F32: int8 q[count], f32 scale, f32 offset;
  *                                value = fma(q, scale, offset)
  *   NVE_DTYPE_X_E4M3_ROWWISE_F32: OCP fp8 e4m3 q[count], f32 scale;
- *                                value = e4m3(q) * scale */
+ *                                value = e4m3(q) * scale
+ * and the 4-bit format of the key-value cache's pages, OCP MXFP4 (no table
+ * stores it, no lookup emits it):
+ *   NVE_DTYPE_X_MXFP4: e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), value
+ *                      2i in the low half of byte i, with an e8m0 scale (the
+ *                      exponent byte of a power of two, 255: NaN) for every 32;
+ *                      value = e2m1(code) * scale */
 enum {
   NVE_DTYPE_X_INT8_AFFINE_F32 = 32,
   NVE_DTYPE_X_E4M3_ROWWISE_F32 = 33,
+  NVE_DTYPE_X_MXFP4 = 34,
 };
 
 /* Fused find-and-pool over a linear table, keys and outputs in device memory.
@@ -188,13 +195,15 @@ NVE_C_API nve_status_t nve_amd_pooling_backprop(
 /* Paged key-value cache of an attention layer (serving; no counterpart in the
  * reference).  A page holds page_size slots of num_heads key / value heads:
  * k and v are [num_pages, num_heads, page_size, head_dim] of dtype (FLOAT32,
- * FLOAT16, BFLOAT16 or E4M3), 16-byte aligned.  E4M3 rows have one f32 scale
- * each (value = e4m3(code) * scale) in k_scale and v_scale [num_pages,
- * num_heads, page_size]; NULL for the other types.  weights (f32) and index
- * (int32) have the scales' shape: the attention weight a slot has received so
- * far, and its token's place in its sequence; either may be NULL where a call
- * does not need it.  page_size is a power of two from 8 to 1024, head_dim a
- * multiple of 8 from 8 to 256.
+ * FLOAT16, BFLOAT16, E4M3 or X_MXFP4), 16-byte aligned.  E4M3 rows have one f32
+ * scale each (value = e4m3(code) * scale) in k_scale and v_scale [num_pages,
+ * num_heads, page_size].  X_MXFP4 rows are head_dim / 2 bytes of codes, and
+ * k_scale and v_scale point to their head_dim / 32 e8m0 bytes each, [num_pages,
+ * num_heads, page_size, head_dim / 32].  NULL for the other types.  weights (f32)
+ * and index (int32) are [num_pages, num_heads, page_size]: the attention weight a
+ * slot has received so far, and its token's place in its sequence; either may be
+ * NULL where a call does not need it.  page_size is a power of two from 8 to
+ * 1024, head_dim a multiple of 8 (X_MXFP4: of 32) from 8 to 256.
  * A sequence is a row of block_tables: its slot t lies in page
  * block_tables[s * table_stride + t / page_size], row t % page_size.  Page ids
  * outside [0, num_pages) are neither read nor written: their slots count as
@@ -216,12 +225,15 @@ typedef struct {
 } nve_amd_kv_pages_t;
 
 /* New tokens enter the cache.  Token t's keys and values (num_heads heads of
- * `dtype`, the pages' type, or FLOAT16 / BFLOAT16 for E4M3 pages) are written to
+ * `dtype`, the pages' type, or FLOAT16 / BFLOAT16 for scaled pages) are written to
  * slot slots[t] = page * page_size + row (a slot outside the cache is skipped;
  * no slot may appear twice), index[t] to the slot's index (with pages->index;
  * index NULL: positions[0][t], or 0 without positions), 0 to its weight (with
  * pages->weights).  E4M3 rows: scale = max(largest magnitude, 1e-30) / 448,
- * code = value / scale rounded to nearest even.
+ * code = value / scale rounded to nearest even.  X_MXFP4 rows: the scale of 32
+ * values is the least power of two (2^-126 at least) of which no magnitude is
+ * over 7 times, code = value / scale rounded to nearest even (6 is the most); 32
+ * values with an infinity or a NaN among them have the scale NaN.
  * rot_dim > 0: the first rot_dim values of every key head, and of every head of
  * q, are rotated first.  Pair i (of rot_dim / 2) is values i and i +
  * rot_dim / 2, or 2i and 2i + 1 if interleaved; it belongs to one of num_axes
@@ -258,16 +270,30 @@ typedef struct {
 NVE_C_API nve_status_t nve_amd_kv_append(const nve_amd_kv_pages_t* pages,
                                          const nve_amd_kv_append_t* call, void* stream);
 
+/* The same with norms of the query and key heads, before the rotation: a head
+ * row x of head_dim values becomes (x[d] * r) * weight[d], both products f32,
+ * with r = 1 / sqrt(mean of x[d]^2 + eps), the mean and r in 64 bits and r then
+ * rounded to f32.  Weights: [head_dim] of the call's dtype; a NULL weight leaves
+ * those heads without a norm.  eps is finite and not negative. */
+typedef struct {
+  const void* q_weight;
+  const void* k_weight;
+  double eps;
+} nve_amd_kv_norm_t;
+NVE_C_API nve_status_t nve_amd_kv_append_norm(const nve_amd_kv_pages_t* pages,
+                                              const nve_amd_kv_append_t* call,
+                                              const nve_amd_kv_norm_t* norm, void* stream);
+
 /* Attention of one new token per sequence over its slots t < lengths[s]:
  *   x_t = scale * q . k_t,  p = softmax(x),  out = sum_t p_t v_t
  * q and out: [num_seqs, num_q_heads, head_dim] of `dtype` (the pages' type, or
- * FLOAT16 / BFLOAT16 for E4M3 pages); query head h reads key head
+ * FLOAT16 / BFLOAT16 for scaled pages); query head h reads key head
  * h / (num_q_heads / num_heads).  lse (may be NULL): [num_seqs, num_q_heads],
  * log sum_t exp(x_t).  Where no slot has a score above -infinity (a length of
  * zero, say) out is 0 and lse -infinity.  What lies in a page's rows at or past
  * the length is not used, whatever it is.  Scores, lse, sums and the weights that
  * are added are f32; the p_t that meet FLOAT16 values keep 22 bits and those below
- * 2^-38 of the largest count as 0, the p_t that meet E4M3 values keep 17.  accumulate:
+ * 2^-38 of the largest count as 0, the p_t that meet E4M3 and X_MXFP4 values keep 17.  accumulate:
  * p_t, summed over the query heads of a key head, is added to pages->weights;
  * no page may then belong to two sequences of the call.  max_length: the
  * longest length that occurs, if the caller knows it (0: the table's extent);

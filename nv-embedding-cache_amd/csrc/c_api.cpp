@@ -1014,6 +1014,15 @@ nve_status_t nve_amd_kv_append(const nve_amd_kv_pages_t* pages, const nve_amd_kv
   C_CATCH
 }
 
+nve_status_t nve_amd_kv_append_norm(const nve_amd_kv_pages_t* pages, const nve_amd_kv_append_t* call,
+                                    const nve_amd_kv_norm_t* norm, void* stream) {
+  C_TRY
+  NVE_TRACE("nve_amd_kv_append_norm");
+  kv_append_norm_run(pages, call, norm, (hipStream_t)stream);
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
 nve_status_t nve_amd_kv_attend_workspace_size(const nve_amd_kv_pages_t* pages,
                                               const nve_amd_kv_attend_t* call, uint64_t* bytes) {
   C_TRY

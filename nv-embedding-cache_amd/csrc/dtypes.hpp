@@ -22,7 +22,8 @@ enum : int {
   kQU8F32 = 9,    // uint8 values + f32 scale + f32 offset
   kQU8F16 = 10,   // uint8 values + f16 scale + f16 offset
   kXI8AF32 = 32,  // extension: int8 values + f32 scale + f32 offset
-  kXE4M3F32 = 33  // extension: OCP fp8 e4m3 values + f32 scale
+  kXE4M3F32 = 33,  // extension: OCP fp8 e4m3 values + f32 scale
+  kMXFP4 = 34      // extension, key-value pages: e2m1 values, an e8m0 scale for every 32
 };
 
 inline constexpr bool is_rowwise(int dt) {

@@ -97,16 +97,43 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float sc
   *reinterpret_cast<u32x2*>(p) = w;
 }
 
+// The exponent byte of the scale of 32 kMXFP4 values whose largest magnitude has the bits `top`:
+// the least power of two with top <= 7 times it, so that no value is further from a multiple than
+// half the widest step (4 to 6).  top is 1.75 * 4 times a power of two at most where its fraction is
+// 0x600000 at most, hence the carry.
+__device__ __forceinline__ uint32_t mxfp4_exponent(uint32_t top) {
+  return top >= 0x7f800000u ? 255u : max((top + 0x1fffffu) >> 23, 3u) - 2u;
+}
+__device__ __forceinline__ float mxfp4_scale(uint32_t exponent) { return __uint_as_float(exponent << 23); }
+
+// 8 values' codes, the first one's lowest.
+__device__ __forceinline__ uint32_t mxfp4_codes(const float* x, float scale) {
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
+  return w;
+}
+
+// 1 / sqrt(mean square + eps) of a row whose squares' sum is `sum`.  The sum is in 64 bits: what
+// follows is f32 steps that any order of it leaves alike, and 4- and 8-bit codes do not turn on it.
+__device__ __forceinline__ float inverse_rms(double sum, int dim, double eps) {
+  return (float)(1.0 / sqrt(sum / dim + eps));
+}
+
 struct AppendPlan {
   int32_t lanes, lane_bits;  // of a row
   int32_t tokens;            // of a workgroup
 };
 
-template <int DT, bool E4M3>
+// DT: the rows' type, CT: the pages'; NORM: queries or keys have a norm.
+template <int DT, int CT, bool NORM>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppend a, const AppendPlan p) {
   constexpr int kBytes = value_elem_bytes(DT);
   __shared__ alignas(16) float table[kMaxTable];
   __shared__ alignas(8) uint8_t turned[kMaxTable / 2];
+  __shared__ alignas(16) float norms[NORM ? 2 : 1][NORM ? 256 : 4];  // of queries and of keys
   const int tid = threadIdx.x, dim = a.pages.dim, heads = a.pages.heads, half = a.rot >> 1;
   const int rows = a.q_heads + 2 * heads;
   const int64_t t0 = (int64_t)blockIdx.x * p.tokens;
@@ -165,6 +192,11 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppend a, c
     table[e] = in ? a.cos_sin[pos * a.rot + i] : 0.0f;
     if (i < half) turned[token * half + i] = in;
   }
+  if constexpr (NORM) {
+    using T = kv_elem<DT>;
+    norms[0][tid] = a.q_norm && tid < dim ? (float)reinterpret_cast<const T*>(a.q_norm)[tid] : 0.0f;
+    norms[1][tid] = a.k_norm && tid < dim ? (float)reinterpret_cast<const T*>(a.k_norm)[tid] : 0.0f;
+  }
   __syncthreads();
 
   while (r < all) {
@@ -177,6 +209,22 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppend a, c
     if (at.have > 1) x1.get(x + 8);
     const int next = r + step;
     if (next < all) load(next);
+    if constexpr (NORM) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum = fma((double)x[i], (double)x[i], sum);
+      for (int m = p.lanes >> 1; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
+      if (u.kind == 0 ? a.q_norm != nullptr : u.kind == 1 && a.k_norm != nullptr) {
+        const float f = inverse_rms(sum, dim, a.eps);
+        const f32x4* w0 = reinterpret_cast<const f32x4*>(&norms[u.kind][at.first]);
+        const f32x4* w1 = reinterpret_cast<const f32x4*>(&norms[u.kind][at.second]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = x[i] * f * w0[i / 4][i % 4];
+          x[8 + i] = x[8 + i] * f * w1[i / 4][i % 4];
+        }
+      }
+    }
     if (at.turn) {
       // pair i of the lane: values i and i + 8, or 2 i and 2 i + 1
       const f32x4* cos = reinterpret_cast<const f32x4*>(table + (u.t - t0) * a.rot + 8 * lane);
@@ -205,7 +253,30 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppend a, c
     } else {
       const int64_t to = row_of(a, u.t, u.head);
       uint8_t* pages = u.kind == 2 ? a.pages.v : a.pages.k;
-      if constexpr (E4M3) {
+      if constexpr (CT == kMXFP4) {
+        // 32 values that share a scale: 4 lanes' 8 (two such runs), or 2 lanes' 16
+        uint32_t top[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top[i / 8] = max(top[i / 8], magnitude(x[i]));
+        const bool apart = at.turn && !a.interleaved;
+        if (!apart) top[0] = top[1] = max(top[0], top[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], 1));
+          if (apart) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], 2));
+        }
+        if (to >= 0 && at.have > 0) {  // dim is a multiple of 32: both halves are there
+          uint8_t* codes = pages + to * (dim / 2);
+          uint8_t* scales = static_cast<uint8_t*>(u.kind == 2 ? a.pages.v_scale : a.pages.k_scale) + to * (dim / 32);
+          const int first[2] = {at.first, at.second};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t e = mxfp4_exponent(top[i]);
+            *reinterpret_cast<uint32_t*>(codes + first[i] / 2) = mxfp4_codes(x + 8 * i, mxfp4_scale(e));
+            if (first[i] % 32 == 0) scales[first[i] / 32] = (uint8_t)e;
+          }
+        }
+      } else if constexpr (CT == kE4M3) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = max(top, magnitude(x[i]));
@@ -214,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppend a, c
         if (to >= 0) {
           if (at.have > 0) store_codes(pages + to * dim + at.first, x, scale);
           if (at.have > 1) store_codes(pages + to * dim + at.second, x + 8, scale);
-          if (lane == 0) (u.kind == 2 ? a.pages.v_scale : a.pages.k_scale)[to] = scale;
+          if (lane == 0) static_cast<float*>(u.kind == 2 ? a.pages.v_scale : a.pages.k_scale)[to] = scale;
         }
       } else if (to >= 0) {
         uint8_t* out = pages + to * dim * kBytes;
@@ -233,10 +304,39 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppend a, c
 constexpr int kRowsPerBlock = 4;  // waves
 constexpr int kMaxPer = 4;        // values per lane: head_dim <= 256
 
-// Value d of a head row of token t, rotated; f32 products and sum rounded one by one.
+// A row's norm: every value times f and its weight (null: no norm).
 template <typename T>
-__device__ __forceinline__ float rotated(const KvAppend& a, const T* row, int64_t t, int d) {
-  const float x = (float)row[d];
+struct Norm {
+  const T* weight;
+  float f;
+  __device__ __forceinline__ float of(const T* row, int d) const {
+    const float x = (float)row[d];
+    return weight ? x * f * (float)weight[d] : x;
+  }
+};
+
+// Of a whole wave's row.
+template <typename T>
+__device__ __forceinline__ Norm<T> norm_of(const KvAppend& a, const uint8_t* weight, const T* row, int lane) {
+  Norm<T> n{reinterpret_cast<const T*>(weight), 1.0f};
+  if (!weight) return n;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kMaxPer; ++i) {
+    const int d = lane + 64 * i;
+    const double x = d < a.pages.dim ? (double)(float)row[d] : 0.0;
+    sum = fma(x, x, sum);
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
+  n.f = inverse_rms(sum, a.pages.dim, a.eps);
+  return n;
+}
+
+// Value d of a head row of token t, normed and rotated; f32 products and sum rounded one by one.
+template <typename T>
+__device__ __forceinline__ float rotated(const KvAppend& a, const Norm<T>& norm, const T* row, int64_t t, int d) {
+  const float x = norm.of(row, d);
   if (d >= a.rot) return x;
   const int half = a.rot >> 1;
   const int pair = a.interleaved ? d >> 1 : (d < half ? d : d - half);
@@ -245,11 +345,11 @@ __device__ __forceinline__ float rotated(const KvAppend& a, const T* row, int64_
   const int64_t p = a.positions[axis_of(a, pair) * a.axis_stride + t];
   if (p < 0 || p >= a.max_position) return x;
   const float* cs = a.cos_sin + p * a.rot;
-  const float c = cs[pair], s = cs[pair + half], y = (float)row[other];
+  const float c = cs[pair], s = cs[pair + half], y = norm.of(row, other);
   return first ? x * c - y * s : x * c + y * s;
 }
 
-template <int DT, bool E4M3>
+template <int DT, int CT>
 __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const KvAppend a) {
   using T = kv_elem<DT>;
   const int lane = threadIdx.x & 63;
@@ -262,10 +362,11 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const
   if (head < a.q_heads) {
     const T* row = reinterpret_cast<const T*>(a.q.p) + t * a.q.token_stride + head * a.q.head_stride;
     T* out = reinterpret_cast<T*>(a.q_out) + t * a.q_out_token_stride + head * a.q_out_head_stride;
+    const Norm<T> norm = norm_of(a, a.q_norm, row, lane);
     float x[kMaxPer];
 #pragma unroll
     for (int i = 0; i < kMaxPer; ++i)
-      if (lane + 64 * i < dim) x[i] = rotated(a, row, t, lane + 64 * i);
+      if (lane + 64 * i < dim) x[i] = rotated(a, norm, row, t, lane + 64 * i);
     // q_out may be q: every lane's values are read before the first is written
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -281,13 +382,28 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const
   const KvRows& in = value ? a.v : a.k;
   const T* row = reinterpret_cast<const T*>(in.p) + t * in.token_stride + head * in.head_stride;
   uint8_t* pages = value ? a.pages.v : a.pages.k;
+  const Norm<T> norm = norm_of(a, value ? nullptr : a.k_norm, row, lane);
   float x[kMaxPer];
 #pragma unroll
   for (int i = 0; i < kMaxPer; ++i) {
     const int d = lane + 64 * i;
-    x[i] = d >= dim ? 0.0f : value ? (float)row[d] : rotated(a, row, t, d);
+    x[i] = d >= dim ? 0.0f : value ? (float)row[d] : rotated(a, norm, row, t, d);
   }
-  if constexpr (E4M3) {
+  if constexpr (CT == kMXFP4) {
+    uint8_t* scales = static_cast<uint8_t*>(value ? a.pages.v_scale : a.pages.k_scale) + at * (dim / 32);
+#pragma unroll
+    for (int i = 0; i < kMaxPer; ++i) {  // half a wave has 32 values of a scale, or none
+      const int d = lane + 64 * i;
+      uint32_t top = magnitude(x[i]);
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
+      const uint32_t e = mxfp4_exponent(top);
+      const float next = __shfl_xor(x[i], 1);
+      const uint32_t codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, x[i], next, mxfp4_scale(e), 0);
+      if (d < dim && lane % 2 == 0) pages[at * (dim / 2) + d / 2] = (uint8_t)codes;
+      if (d < dim && d % 32 == 0) scales[d / 32] = (uint8_t)e;
+    }
+  } else if constexpr (CT == kE4M3) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kMaxPer; ++i) top = max(top, magnitude(x[i]));
@@ -298,7 +414,7 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const
     for (int i = 0; i < kMaxPer; ++i)
       if (lane + 64 * i < dim)
         pages[at * dim + lane + 64 * i] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[i] / scale, 0.0f, 0, false);
-    if (lane == 0) (value ? a.pages.v_scale : a.pages.k_scale)[at] = scale;
+    if (lane == 0) static_cast<float*>(value ? a.pages.v_scale : a.pages.k_scale)[at] = scale;
   } else {
     T* out = reinterpret_cast<T*>(pages) + at * dim;
 #pragma unroll
@@ -334,19 +450,20 @@ bool wide(const KvAppend& a) {
   auto at16 = [&](const void* p, int64_t token, int64_t head) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && token * e % 16 == 0 && head * e % 16 == 0;
   };
-  // rows of an e4m3 cache are written 8 bytes at a time, the others' start at 16 bytes with head_dim
-  return a.rot % 16 == 0 && at16(a.k.p, a.k.token_stride, a.k.head_stride) &&
+  // rows of an e4m3 cache are written 8 bytes at a time, the others' start at 16 bytes with head_dim;
+  // 32 values with a scale of their own have to be in 4 lanes, or in 2 with 16 each
+  return a.rot % (a.pages.dtype == kMXFP4 && !a.interleaved ? 64 : 16) == 0 && at16(a.k.p, a.k.token_stride, a.k.head_stride) &&
          at16(a.v.p, a.v.token_stride, a.v.head_stride) &&
          (a.q_heads == 0 || (at16(a.q.p, a.q.token_stride, a.q.head_stride) &&
                              at16(a.q_out, a.q_out_token_stride, a.q_out_head_stride)));
 }
 
-template <int DT, bool E4M3>
+template <int DT, int CT>
 hipError_t launch(const KvAppend& a, hipStream_t stream) {
   const int rows = a.q_heads + 2 * a.pages.heads;
   AppendPlan p{};
   int64_t most;  // tokens of a launch
-  const bool in_words = wide(a);
+  const bool in_words = wide(a), norm = a.q_norm || a.k_norm;
   if (in_words) {
     const int need = (a.pages.dim + 15) / 16;
     while ((1 << p.lane_bits) < need) ++p.lane_bits;
@@ -361,25 +478,36 @@ hipError_t launch(const KvAppend& a, hipStream_t stream) {
   }
   for (int64_t t0 = 0; t0 < a.tokens; t0 += most) {
     const KvAppend b = part(a, t0, std::min(most, a.tokens - t0));
-    if (in_words)
-      kv_append_kernel<DT, E4M3><<<(unsigned)((b.tokens + p.tokens - 1) / p.tokens), kThreads, 0, stream>>>(b, p);
+    const unsigned groups = in_words ? (unsigned)((b.tokens + p.tokens - 1) / p.tokens) : 0;
+    if (in_words && norm)
+      kv_append_kernel<DT, CT, true><<<groups, kThreads, 0, stream>>>(b, p);
+    else if (in_words)
+      kv_append_kernel<DT, CT, false><<<groups, kThreads, 0, stream>>>(b, p);
     else
-      kv_append_any_kernel<DT, E4M3>
+      kv_append_any_kernel<DT, CT>
           <<<(unsigned)((b.tokens * rows + kRowsPerBlock - 1) / kRowsPerBlock), kThreads, 0, stream>>>(b);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
+template <int DT>
+hipError_t launch_pages(const KvAppend& a, hipStream_t stream) {
+  switch (a.pages.dtype) {
+    case kE4M3: return launch<DT, kE4M3>(a, stream);
+    case kMXFP4: return launch<DT, kMXFP4>(a, stream);
+    default: return launch<DT, DT>(a, stream);
+  }
+}
+
 }  // namespace
 
 hipError_t launch_kv_append(const KvAppend& a, hipStream_t stream) {
   if (a.tokens == 0) return hipSuccess;
-  const bool q8 = a.pages.dtype == kE4M3;
   switch (a.dtype) {
-    case kF32: return launch<kF32, false>(a, stream);
-    case kF16: return q8 ? launch<kF16, true>(a, stream) : launch<kF16, false>(a, stream);
-    case kBF16: return q8 ? launch<kBF16, true>(a, stream) : launch<kBF16, false>(a, stream);
+    case kF32: return launch<kF32, kF32>(a, stream);
+    case kF16: return launch_pages<kF16>(a, stream);
+    case kBF16: return launch_pages<kBF16>(a, stream);
     default: return hipErrorInvalidValue;
   }
 }

@@ -95,33 +95,43 @@ struct Scan {
   }
 };
 
-// A word of 16 or 8 bytes of a k row and of its v row; word 0 brings what goes with the row.
+// A word of 16 or 8 bytes of a k row and of its v row; word 0 brings what goes with the row.  A
+// kMXFP4 row has as many scales (bytes) as words of 16 bytes: each word brings one.
 template <typename WORD>
 struct Moved {
   WORD k, v;
-  float weight, k_scale, v_scale;
+  float weight;
+  uint32_t k_scale, v_scale;
   int32_t place;
   __device__ __forceinline__ void load(const KvPages& c, int64_t row, int words, int word) {
     k = reinterpret_cast<const WORD*>(c.k)[row * words + word];
     v = reinterpret_cast<const WORD*>(c.v)[row * words + word];
+    if (c.dtype == kMXFP4) {
+      k_scale = static_cast<const uint8_t*>(c.k_scale)[row * words + word];
+      v_scale = static_cast<const uint8_t*>(c.v_scale)[row * words + word];
+    }
     if (word == 0) {
       weight = c.weights[row];
       place = c.index[row];
-      if (c.k_scale) {
-        k_scale = c.k_scale[row];
-        v_scale = c.v_scale[row];
+      if (c.dtype == kE4M3) {
+        k_scale = static_cast<const uint32_t*>(c.k_scale)[row];
+        v_scale = static_cast<const uint32_t*>(c.v_scale)[row];
       }
     }
   }
   __device__ __forceinline__ void store(const KvPages& c, int64_t row, int words, int word) const {
     reinterpret_cast<WORD*>(c.k)[row * words + word] = k;
     reinterpret_cast<WORD*>(c.v)[row * words + word] = v;
+    if (c.dtype == kMXFP4) {
+      static_cast<uint8_t*>(c.k_scale)[row * words + word] = (uint8_t)k_scale;
+      static_cast<uint8_t*>(c.v_scale)[row * words + word] = (uint8_t)v_scale;
+    }
     if (word == 0) {
       c.weights[row] = weight;
       c.index[row] = place;
-      if (c.k_scale) {
-        c.k_scale[row] = k_scale;
-        c.v_scale[row] = v_scale;
+      if (c.dtype == kE4M3) {
+        static_cast<uint32_t*>(c.k_scale)[row] = k_scale;
+        static_cast<uint32_t*>(c.v_scale)[row] = v_scale;
       }
     }
   }
@@ -134,7 +144,7 @@ constexpr int kPairs = 64;  // resolved at a time
 template <typename WORD, int THREADS, int AHEAD>
 __device__ __forceinline__ void move_words(const KvPages& c, const int32_t* table, int head, const int32_t* to,
                                            const int32_t* from, int64_t first, int64_t last, int64_t (*rows)[2]) {
-  const int words = c.dim * value_elem_bytes(c.dtype) / (int)sizeof(WORD);
+  const int words = kv_row_bytes(c.dtype, c.dim) / (int)sizeof(WORD);
   for (int64_t p0 = first; p0 < last; p0 += kPairs) {
     const int n = (int)min((int64_t)kPairs, last - p0);
     __syncthreads();
@@ -168,7 +178,7 @@ __device__ __forceinline__ void move_words(const KvPages& c, const int32_t* tabl
 template <int THREADS, int AHEAD>
 __device__ __forceinline__ void move_rows(const KvPages& c, const int32_t* table, int head, const int32_t* to,
                                           const int32_t* from, int64_t first, int64_t last, int64_t (*rows)[2]) {
-  if (c.dim * value_elem_bytes(c.dtype) % 16 == 0)
+  if (kv_row_bytes(c.dtype, c.dim) % 16 == 0)
     move_words<u32x4, THREADS, AHEAD>(c, table, head, to, from, first, last, rows);
   else
     move_words<uint64_t, THREADS, AHEAD>(c, table, head, to, from, first, last, rows);

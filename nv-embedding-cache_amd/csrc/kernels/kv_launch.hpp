@@ -1,5 +1,5 @@
 // kv_launch.hpp -- host launchers of the paged key-value cache's kernels
-// (kv_append.hip, kv_attend.hip, kv_evict.hip).
+// (kv_append.hip, kv_attend.hip, kv_attend_mxfp4.hip, kv_evict.hip).
 //
 // Every pointer is device memory; shapes, types and strides are checked by the
 // caller (kv_cache.cpp).  Values read from device memory (slots, positions,
@@ -9,14 +9,21 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../dtypes.hpp"
+
 namespace nve_amd {
 
-// The pages: k and v [num_pages, heads, page, dim] of dtype, the rest [num_pages, heads, page].
+// Bytes of a head's row, and of its scales.
+inline constexpr int kv_row_bytes(int dtype, int dim) { return dtype == kMXFP4 ? dim / 2 : dim * value_elem_bytes(dtype); }
+inline constexpr int kv_scale_bytes(int dtype, int dim) { return dtype == kMXFP4 ? dim / 32 : dtype == kE4M3 ? 4 : 0; }
+
+// The pages: k and v [num_pages, heads, page, dim] of dtype, the rest [num_pages, heads, page]
+// (kMXFP4: the scales are [num_pages, heads, page, dim / 32] bytes).
 struct KvPages {
   uint8_t* k;
   uint8_t* v;
-  float* k_scale;
-  float* v_scale;
+  void* k_scale;
+  void* v_scale;
   float* weights;
   int32_t* index;
   int64_t num_pages;
@@ -45,6 +52,9 @@ struct KvAppend {
   int64_t max_position;
   int32_t rot, interleaved, axes;
   int32_t ends[4];  // the first pair past each axis
+  const uint8_t* q_norm;  // [dim] of dtype, or null: no norm
+  const uint8_t* k_norm;
+  double eps;
 };
 
 struct KvAttend {
@@ -77,6 +87,7 @@ struct KvEvict {
 hipError_t launch_kv_append(const KvAppend& a, hipStream_t stream);
 size_t kv_attend_workspace(const KvAttend& a);
 hipError_t launch_kv_attend(const KvAttend& a, void* workspace, hipStream_t stream);
+hipError_t launch_kv_attend_mxfp4(const KvAttend& a, void* workspace, hipStream_t stream);  // of launch_kv_attend
 size_t kv_evict_workspace(const KvEvict& a);
 hipError_t launch_kv_evict(const KvEvict& a, void* workspace, hipStream_t stream);
 

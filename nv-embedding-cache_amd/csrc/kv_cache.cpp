@@ -21,6 +21,8 @@ constexpr int64_t kMaxGrid = std::numeric_limits<int32_t>::max();
 
 bool aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+bool scaled(int dtype) { return dtype == kE4M3 || dtype == kMXFP4; }
+
 KvPages pages_of(const nve_amd_kv_pages_t* p) {
   NVE_CHECK_ARG(p != nullptr, "pages must not be NULL");
   NVE_CHECK_ARG(p->num_pages >= 0 && p->num_pages <= kMaxGrid, "Invalid num_pages ", p->num_pages);
@@ -30,16 +32,18 @@ KvPages pages_of(const nve_amd_kv_pages_t* p) {
   NVE_CHECK_ARG(p->head_dim >= 8 && p->head_dim <= 256 && p->head_dim % 8 == 0,
                 "head_dim must be a multiple of 8 from 8 to 256 (got ", p->head_dim, ")");
   const int dt = (int)p->dtype;
-  NVE_CHECK_ARG(dt == kF32 || dt == kF16 || dt == kBF16 || dt == kE4M3,
-                "pages must be float32, float16, bfloat16 or e4m3 (got type ", dt, ")");
+  NVE_CHECK_ARG(dt == kF32 || dt == kF16 || dt == kBF16 || dt == kE4M3 || dt == kMXFP4,
+                "pages must be float32, float16, bfloat16, e4m3 or mxfp4 (got type ", dt, ")");
+  NVE_CHECK_ARG(dt != kMXFP4 || p->head_dim % 32 == 0, "head_dim of mxfp4 pages must be a multiple of 32 (got ",
+                p->head_dim, ")");
   if (p->num_pages > 0) NVE_CHECK_ARG(p->k && p->v, "k and v pages must not be NULL");
   NVE_CHECK_ARG(aligned(p->k, 16) && aligned(p->v, 16), "k and v pages must be 16-byte aligned");
-  if (dt == kE4M3) {
-    if (p->num_pages > 0) NVE_CHECK_ARG(p->k_scale && p->v_scale, "e4m3 pages need k_scale and v_scale");
+  if (scaled(dt)) {
+    if (p->num_pages > 0) NVE_CHECK_ARG(p->k_scale && p->v_scale, "e4m3 and mxfp4 pages need k_scale and v_scale");
   } else {
-    NVE_CHECK_ARG(!p->k_scale && !p->v_scale, "only e4m3 pages have scales");
+    NVE_CHECK_ARG(!p->k_scale && !p->v_scale, "only e4m3 and mxfp4 pages have scales");
   }
-  NVE_CHECK_ARG((int64_t)p->num_heads * p->page_size * p->head_dim * value_elem_bytes(dt) <= kMaxGrid,
+  NVE_CHECK_ARG((int64_t)p->num_heads * p->page_size * kv_row_bytes(dt, p->head_dim) <= kMaxGrid,
                 "a page of all heads must be smaller than 2 GiB");
   KvPages c{};
   c.k = static_cast<uint8_t*>(p->k);
@@ -58,9 +62,9 @@ KvPages pages_of(const nve_amd_kv_pages_t* p) {
 }
 
 void check_dtype(const KvPages& c, nve_data_type_t dtype) {
-  if (c.dtype == kE4M3)
+  if (scaled(c.dtype))
     NVE_CHECK_ARG(dtype == NVE_DTYPE_FLOAT16 || dtype == NVE_DTYPE_BFLOAT16,
-                  "e4m3 pages take float16 or bfloat16 rows (got type ", (int)dtype, ")");
+                  "e4m3 and mxfp4 pages take float16 or bfloat16 rows (got type ", (int)dtype, ")");
   else
     NVE_CHECK_ARG((int)dtype == c.dtype, "the rows' type ", (int)dtype, " is not the pages' type ", c.dtype);
 }
@@ -198,6 +202,18 @@ void check_workspace(const void* ws, size_t have, size_t need) {
 
 void kv_append_run(const nve_amd_kv_pages_t* pages, const nve_amd_kv_append_t* call, hipStream_t s) {
   NVE_HIP(launch_kv_append(append_of(pages, call), s));
+}
+
+void kv_append_norm_run(const nve_amd_kv_pages_t* pages, const nve_amd_kv_append_t* call,
+                        const nve_amd_kv_norm_t* norm, hipStream_t s) {
+  KvAppend a = append_of(pages, call);
+  NVE_CHECK_ARG(norm != nullptr, "norm must not be NULL");
+  NVE_CHECK_ARG(norm->q_weight == nullptr || call->q != nullptr || a.tokens == 0, "q_weight needs q");
+  NVE_CHECK_ARG(std::isfinite(norm->eps) && norm->eps >= 0, "eps must be finite and not negative (got ", norm->eps, ")");
+  a.q_norm = static_cast<const uint8_t*>(norm->q_weight);
+  a.k_norm = static_cast<const uint8_t*>(norm->k_weight);
+  a.eps = norm->eps;
+  NVE_HIP(launch_kv_append(a, s));
 }
 
 size_t kv_attend_workspace_bytes(const nve_amd_kv_pages_t* pages, const nve_amd_kv_attend_t* call) {

@@ -1,7 +1,7 @@
 // nve_kv_ops.cpp -- the nve_ops torch library's operators of the paged key-value
 // cache (HIP tensors), calling libnve_amd.so's C ABI (nve_amd_kv_*) directly:
 //
-//   kv_append, kv_attend, kv_attend_lse, kv_evict   (schemas below)
+//   kv_append, kv_append_norm, kv_attend, kv_attend_lse, kv_evict   (schemas below)
 //
 // Shapes, types and devices are checked here, the rest by the C ABI; work runs
 // on the current stream, workspaces come from torch's allocator.  The operators
@@ -42,6 +42,7 @@ nve_data_type_t dtype_of(const Tensor& t, const char* name) {
     case at::kHalf: return NVE_DTYPE_FLOAT16;
     case at::kBFloat16: return NVE_DTYPE_BFLOAT16;
     case at::kFloat8_e4m3fn: return NVE_DTYPE_E4M3;
+    case at::kFloat4_e2m1fn_x2: return NVE_DTYPE_X_MXFP4;
     default: break;
   }
   TORCH_CHECK_TYPE(false, "nve_ops: ", name, " cannot be ", t.scalar_type());
@@ -66,11 +67,16 @@ void check_grad(const Tensor& t, const char* name) {
               " asks for a gradient, and the key-value cache's operators have none (use torch.no_grad())");
 }
 
+// Values of a head's row: 4-bit pages hold two in an element.
+int64_t dim_of(const Tensor& pages) {
+  return pages.size(3) * (pages.scalar_type() == at::kFloat4_e2m1fn_x2 ? 2 : 1);
+}
+
 // [rows, heads, dim] with a contiguous last dimension, any strides of the others.
 void check_rows(const Tensor& t, const Tensor& pages, const char* name) {
   check_device(t, pages, name);
-  TORCH_CHECK_VALUE(t.dim() == 3 && t.size(2) == pages.size(3), "nve_ops: ", name, " must be [rows, heads, ",
-                    pages.size(3), "], got ", t.sizes());
+  TORCH_CHECK_VALUE(t.dim() == 3 && t.size(2) == dim_of(pages), "nve_ops: ", name, " must be [rows, heads, ",
+                    dim_of(pages), "], got ", t.sizes());
   TORCH_CHECK_VALUE(t.stride(2) == 1 || t.numel() == 0, "nve_ops: the last dimension of ", name,
                     " must be contiguous");
   check_grad(t, name);
@@ -98,13 +104,28 @@ T* slot_values(const OptTensor& t, const Tensor& pages, at::ScalarType type, con
   return static_cast<T*>(t->data_ptr());
 }
 
+// The scales of e4m3 pages (one float32 a row) or of 4-bit pages (one e8m0 for every 32 values).
+float* scales_of(const OptTensor& t, const Tensor& pages, const char* name) {
+  if (pages.scalar_type() != at::kFloat4_e2m1fn_x2) return slot_values<float>(t, pages, at::kFloat, name);
+  if (!t.has_value() || !t->defined()) return nullptr;
+  check_device(*t, pages, name);
+  check_type(*t, at::kFloat8_e8m0fnu, name);
+  check_dense(*t, name);
+  check_grad(*t, name);
+  TORCH_CHECK_VALUE(t->dim() == 4 && t->sizes().slice(0, 3) == pages.sizes().slice(0, 3) &&
+                        t->size(3) * 32 == dim_of(pages),
+                    "nve_ops: ", name, " must be ", pages.sizes().slice(0, 3), " rows of ", dim_of(pages) / 32, ", got ",
+                    t->sizes());
+  return static_cast<float*>(t->data_ptr());
+}
+
 nve_amd_kv_pages_t pages_of(const Tensor& k, const Tensor& v, const OptTensor& k_scale, const OptTensor& v_scale,
                             const OptTensor& weights, const OptTensor& index) {
   TORCH_CHECK_VALUE(k.dim() == 4, "nve_ops: the pages must be [pages, heads, page, dim], got ", k.sizes());
   TORCH_CHECK_VALUE(v.sizes() == k.sizes(), "nve_ops: the k pages are ", k.sizes(), ", the v pages ", v.sizes());
   TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type(), "nve_ops: the k pages are ", k.scalar_type(),
                    ", the v pages ", v.scalar_type());
-  TORCH_CHECK_VALUE(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX && k.size(3) <= INT32_MAX,
+  TORCH_CHECK_VALUE(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX && dim_of(k) <= INT32_MAX,
                     "nve_ops: pages too large");
   check_device(v, k, "v_pages");
   check_dense(k, "k_pages");
@@ -114,14 +135,14 @@ nve_amd_kv_pages_t pages_of(const Tensor& k, const Tensor& v, const OptTensor& k
   nve_amd_kv_pages_t p{};
   p.k = k.data_ptr();
   p.v = v.data_ptr();
-  p.k_scale = slot_values<float>(k_scale, k, at::kFloat, "k_scale");
-  p.v_scale = slot_values<float>(v_scale, k, at::kFloat, "v_scale");
+  p.k_scale = scales_of(k_scale, k, "k_scale");
+  p.v_scale = scales_of(v_scale, k, "v_scale");
   p.weights = slot_values<float>(weights, k, at::kFloat, "weights");
   p.index = slot_values<int32_t>(index, k, at::kInt, "index_pages");
   p.num_pages = k.size(0);
   p.num_heads = (int32_t)k.size(1);
   p.page_size = (int32_t)k.size(2);
-  p.head_dim = (int32_t)k.size(3);
+  p.head_dim = (int32_t)dim_of(k);
   p.dtype = dtype_of(k, "k_pages");
   return p;
 }
@@ -132,17 +153,25 @@ Tensor bytes(uint64_t n, const Tensor& like) {
   return at::empty({(int64_t)n}, like.options().dtype(at::kByte));
 }
 
-Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& slots,
-                 const OptTensor& q, const OptTensor& positions, const OptTensor& cos_sin,
-                 const std::optional<std::vector<int64_t>>& sections, bool interleaved, const OptTensor& index,
-                 const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& weights,
-                 const OptTensor& index_pages) {
+// The weight of a norm: [dim] of the rows' type.
+const void* norm_weight(const OptTensor& t, const Tensor& k, const Tensor& pages, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  check_grad(*t, name);
+  return optional_row(t, pages, k.scalar_type(), dim_of(pages), name);
+}
+
+Tensor append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& slots,
+              const OptTensor& q, const OptTensor& positions, const OptTensor& cos_sin,
+              const std::optional<std::vector<int64_t>>& sections, bool interleaved, const OptTensor& index,
+              const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& weights,
+              const OptTensor& index_pages, const OptTensor& q_norm, const OptTensor& k_norm,
+              std::optional<double> eps) {
   const at::DeviceGuard guard(k_pages.device());
   const nve_amd_kv_pages_t pages = pages_of(k_pages, v_pages, k_scale, v_scale, weights, index_pages);
   check_rows(k, k_pages, "k");
   check_rows(v, k_pages, "v");
   TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(1) == k_pages.size(1), "nve_ops: k and v must be [tokens, ",
-                    k_pages.size(1), ", ", k_pages.size(3), "], got ", k.sizes(), " and ", v.sizes());
+                    k_pages.size(1), ", ", dim_of(k_pages), "], got ", k.sizes(), " and ", v.sizes());
   TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), "nve_ops: k is ", k.scalar_type(), ", v ", v.scalar_type());
   const int64_t n = k.size(0);
   nve_amd_kv_append_t c{};
@@ -192,8 +221,8 @@ Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const 
       check_type(t, at::kFloat, "cos_sin");
       check_dense(t, "cos_sin");
       check_grad(t, "cos_sin");
-      TORCH_CHECK_VALUE(t.dim() == 2 && t.size(1) <= k_pages.size(3), "nve_ops: cos_sin must be [positions, rot_dim <= ",
-                        k_pages.size(3), "], got ", t.sizes());
+      TORCH_CHECK_VALUE(t.dim() == 2 && t.size(1) <= dim_of(k_pages), "nve_ops: cos_sin must be [positions, rot_dim <= ",
+                        dim_of(k_pages), "], got ", t.sizes());
       c.cos_sin = static_cast<const float*>(t.data_ptr());
       c.max_position = t.size(0);
       c.rot_dim = (int32_t)t.size(1);
@@ -212,8 +241,35 @@ Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const 
     }
   }
   c.interleaved = interleaved;
-  check_status(nve_amd_kv_append(&pages, &c, stream_of(k_pages)));
+  if (eps.has_value()) {
+    nve_amd_kv_norm_t norm{};
+    norm.q_weight = norm_weight(q_norm, k, k_pages, "q_norm");
+    norm.k_weight = norm_weight(k_norm, k, k_pages, "k_norm");
+    TORCH_CHECK_VALUE(!norm.q_weight || (q.has_value() && q->defined()), "nve_ops: q_norm needs q");
+    norm.eps = *eps;
+    check_status(nve_amd_kv_append_norm(&pages, &c, &norm, stream_of(k_pages)));
+  } else {
+    check_status(nve_amd_kv_append(&pages, &c, stream_of(k_pages)));
+  }
   return q_out;
+}
+
+Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& slots,
+                 const OptTensor& q, const OptTensor& positions, const OptTensor& cos_sin,
+                 const std::optional<std::vector<int64_t>>& sections, bool interleaved, const OptTensor& index,
+                 const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& weights,
+                 const OptTensor& index_pages) {
+  return append(k, v, k_pages, v_pages, slots, q, positions, cos_sin, sections, interleaved, index, k_scale, v_scale,
+                weights, index_pages, std::nullopt, std::nullopt, std::nullopt);
+}
+
+Tensor kv_append_norm(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+                      const Tensor& slots, const OptTensor& q, const OptTensor& positions, const OptTensor& cos_sin,
+                      const std::optional<std::vector<int64_t>>& sections, bool interleaved, const OptTensor& index,
+                      const OptTensor& k_scale, const OptTensor& v_scale, const OptTensor& weights,
+                      const OptTensor& index_pages, const OptTensor& q_norm, const OptTensor& k_norm, double eps) {
+  return append(k, v, k_pages, v_pages, slots, q, positions, cos_sin, sections, interleaved, index, k_scale, v_scale,
+                weights, index_pages, q_norm, k_norm, eps);
 }
 
 std::tuple<Tensor, Tensor> attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
@@ -315,6 +371,11 @@ TORCH_LIBRARY_FRAGMENT(nve_ops, m) {
       "Tensor? positions, Tensor? cos_sin, int[]? sections, bool interleaved, Tensor? index, Tensor(c!)? k_scale, "
       "Tensor(d!)? v_scale, Tensor(e!)? weights, Tensor(f!)? index_pages) -> Tensor");
   m.def(
+      "kv_append_norm(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor slots, Tensor? q, "
+      "Tensor? positions, Tensor? cos_sin, int[]? sections, bool interleaved, Tensor? index, Tensor(c!)? k_scale, "
+      "Tensor(d!)? v_scale, Tensor(e!)? weights, Tensor(f!)? index_pages, Tensor? q_norm, Tensor? k_norm, "
+      "float eps) -> Tensor");
+  m.def(
       "kv_attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_tables, Tensor lengths, float scale, "
       "Tensor? k_scale, Tensor? v_scale, Tensor(a!)? weights, int max_length) -> Tensor");
   m.def(
@@ -328,6 +389,7 @@ TORCH_LIBRARY_FRAGMENT(nve_ops, m) {
 
 TORCH_LIBRARY_IMPL(nve_ops, CUDA, m) {
   m.impl("kv_append", &kv_append);
+  m.impl("kv_append_norm", &kv_append_norm);
   m.impl("kv_attend", &kv_attend);
   m.impl("kv_attend_lse", &kv_attend_lse);
   m.impl("kv_evict", &kv_evict);

@@ -11,7 +11,7 @@ SUCCESS, INVALID_ARGUMENT, HIP_ERROR, RUNTIME, NOT_IMPLEMENTED, OUT_OF_MEMORY = 
 # nve_data_type_t
 (DT_UNKNOWN, DT_F32, DT_BF16, DT_F16, DT_E4M3, DT_E5M2, DT_F64, DT_QI8_F32, DT_QI8_F16,
  DT_QU8_F32, DT_QU8_F16) = range(11)
-DT_XI8A_F32, DT_XE4M3_F32 = 32, 33
+DT_XI8A_F32, DT_XE4M3_F32, DT_XMXFP4 = 32, 33, 34
 # enums
 SPARSE_FIXED, SPARSE_CSR = 0, 1
 POOL_CONCAT, POOL_SUM, POOL_MEAN, POOL_WSUM, POOL_WMEAN = range(5)
@@ -99,6 +99,10 @@ class KvAppend(ctypes.Structure):
                 ("num_q_heads", I32), ("index", P), ("positions", P), ("axis_stride", I64),
                 ("cos_sin", P), ("max_position", I64), ("rot_dim", I32), ("interleaved", I32),
                 ("num_axes", I32), ("sections", I32 * 4)]
+
+
+class KvNorm(ctypes.Structure):
+    _fields_ = [("q_weight", P), ("k_weight", P), ("eps", ctypes.c_double)]
 
 
 class KvAttend(ctypes.Structure):
@@ -192,6 +196,7 @@ SIGNATURES = {
     "nve_amd_pooling_backprop": (I32, [ctypes.c_int, I64, P, ctypes.c_int, ctypes.c_int, P, I64, I64, P, I32,
                                        P, I32, I64, P, P, PI64, P, U64, P]),
     "nve_amd_kv_append": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvAppend), P]),
+    "nve_amd_kv_append_norm": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvAppend), ctypes.POINTER(KvNorm), P]),
     "nve_amd_kv_attend_workspace_size": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvAttend),
                                                ctypes.POINTER(U64)]),
     "nve_amd_kv_attend": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvAttend), P, U64, P]),

@@ -6,7 +6,7 @@ lie in pages of a few slots; a sequence is a row of page numbers.  Three
 operators work on the pages, each one a hand-written HIP kernel behind the C ABI
 (nve_amd_kv_*) and a torch op (torch.ops.nve_ops.kv_*):
 
-  kv_append   rotary positions on new queries and keys, keys and values into their slots
+  kv_append   norms of new queries' and keys' heads, rotary positions, keys and values into their slots
   kv_attend   attention of one new token per sequence over its pages; can add each slot's attention
               weight to the weight the cache holds for it
   kv_evict    drops the slots of the least accumulated weight from sequences that are over a budget
@@ -17,15 +17,17 @@ inputs that ask for one are refused unless gradients are off.
 
 Shapes (P pages, H key heads, `page` slots a page, D values a head row, S sequences, T tokens):
 
-  k_pages, v_pages   [P, H, page, D]  float32, float16, bfloat16 or float8_e4m3fn
+  k_pages, v_pages   [P, H, page, D]  float32, float16, bfloat16 or float8_e4m3fn, or
+                     [P, H, page, D / 2]   float4_e2m1fn_x2 (two values an element, the first one low)
   k_scale, v_scale   [P, H, page]     float32, float8 pages only: a row's value is code * scale
+                     [P, H, page, D / 32]  float8_e8m0fnu, 4-bit pages only: of 32 values each
   weights            [P, H, page]     float32, accumulated attention weight
   index_pages        [P, H, page]     int32, the token's place in its sequence
   block_tables       [S, pages]       int32; slot t of sequence s is row t % page of page
                                       block_tables[s, t // page]
   lengths            [S]              int32
 
-`page` is a power of two from 8 to 1024, D a multiple of 8 up to 256.  Page
+`page` is a power of two from 8 to 1024, D a multiple of 8 up to 256 (of 32 for 4-bit pages).  Page
 numbers outside [0, P) name no page: their slots are neither read nor written.
 """
 import torch
@@ -33,13 +35,15 @@ import torch
 from . import HAS_TORCH_OPS  # noqa: F401  (importing registers the ops)
 
 _append = torch.ops.nve_ops.kv_append.default
+_append_norm = torch.ops.nve_ops.kv_append_norm.default
 _attend = torch.ops.nve_ops.kv_attend.default
 _attend_lse = torch.ops.nve_ops.kv_attend_lse.default
 _evict = torch.ops.nve_ops.kv_evict.default
 
 
 def kv_append(k, v, k_pages, v_pages, slots, *, q=None, positions=None, cos_sin=None, sections=None,
-              interleaved=False, index=None, k_scale=None, v_scale=None, weights=None, index_pages=None):
+              interleaved=False, index=None, k_scale=None, v_scale=None, weights=None, index_pages=None, q_norm=None,
+              k_norm=None, eps=1e-6):
     """Writes the keys and values of T new tokens [T, H, D] to the slots `slots`
     (int64: page number * page + row; a slot outside the cache is skipped, none
     may appear twice) and returns the rotated queries, or None without `q`.
@@ -52,9 +56,21 @@ def kv_append(k, v, k_pages, v_pages, slots, *, q=None, positions=None, cos_sin=
     sections[1] by axis 1 and so on.  A position outside the table leaves its
     pairs as they are.  `index` (int32 [T], by default positions of axis 0, or 0)
     goes to index_pages, 0 to weights.  Strides are free but for the last
-    dimension."""
-    out = _append(k, v, k_pages, v_pages, slots, q, positions, cos_sin, sections, interleaved, index, k_scale,
-                  v_scale, weights, index_pages)
+    dimension.
+
+    With `q_norm` or `k_norm` ([D] of the rows' type) the query or key heads are
+    normalised first: x / sqrt(mean(x ** 2) + eps) * norm, head by head (the mean
+    in 64 bits, the products float32).
+
+    4-bit pages: 32 values share a scale, the least power of two of which no
+    magnitude is over 7 times; a value becomes the nearest of 0, .5, 1, 1.5, 2, 3, 4
+    and 6 times it, ties to the even code.  An infinity or a NaN makes the 32 NaN."""
+    rest = (k, v, k_pages, v_pages, slots, q, positions, cos_sin, sections, interleaved, index, k_scale, v_scale,
+            weights, index_pages)
+    if q_norm is None and k_norm is None:
+        out = _append(*rest)
+    else:
+        out = _append_norm(*rest, q_norm, k_norm, eps)
     return None if q is None else out
 
 
@@ -67,8 +83,8 @@ def kv_attend(q, k_pages, v_pages, block_tables, lengths, *, scale=None, k_scale
     [S, Hq].  A sequence without slots gives zeros (and -inf).  With `weights` the
     softmax of every slot, summed over the query heads of its key head, is added
     there; no page may then belong to two of the sequences.  Sums are float32; the
-    softmax values that meet float16 values keep 22 bits, those that meet float8
-    values 17.  `max_length` is a bound on the lengths if the caller knows one below
+    softmax values that meet float16 values keep 22 bits, those that meet float8 or
+    4-bit values 17.  `max_length` is a bound on the lengths if the caller knows one below
     the tables' extent; it sizes the launch and the workspace."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
@@ -93,19 +109,27 @@ def kv_evict(k_pages, v_pages, weights, index_pages, block_tables, lengths, budg
 class KVCache:
     """Pages of one attention layer and their companions.
 
-    `dtype` is that of the queries and keys, or torch.float8_e4m3fn (with
-    float16 or bfloat16 queries); `track_weights=False` leaves out what eviction
-    needs (weights and index)."""
+    `dtype` is that of the queries and keys, or torch.float8_e4m3fn or
+    torch.float4_e2m1fn_x2 (with float16 or bfloat16 queries);
+    `track_weights=False` leaves out what eviction needs (weights and index)."""
 
     def __init__(self, num_pages, num_kv_heads, head_dim, page=16, dtype=torch.float16, device="cuda",
                  track_weights=True):
         shape = (num_pages, num_kv_heads, page)
         self.page = page
-        self.k = torch.zeros((*shape, head_dim), dtype=dtype, device=device)
-        self.v = torch.zeros((*shape, head_dim), dtype=dtype, device=device)
-        scaled = dtype == torch.float8_e4m3fn
-        self.k_scale = torch.zeros(shape, dtype=torch.float32, device=device) if scaled else None
-        self.v_scale = torch.zeros(shape, dtype=torch.float32, device=device) if scaled else None
+        if dtype == torch.float4_e2m1fn_x2:
+            if head_dim % 32:
+                raise ValueError(f"head_dim of 4-bit pages must be a multiple of 32, got {head_dim}")
+            zeros = lambda n, t: torch.zeros((*shape, n), dtype=torch.uint8, device=device).view(t)  # noqa: E731
+            self.k, self.v = zeros(head_dim // 2, dtype), zeros(head_dim // 2, dtype)
+            self.k_scale = zeros(head_dim // 32, torch.float8_e8m0fnu)
+            self.v_scale = zeros(head_dim // 32, torch.float8_e8m0fnu)
+        else:
+            self.k = torch.zeros((*shape, head_dim), dtype=dtype, device=device)
+            self.v = torch.zeros((*shape, head_dim), dtype=dtype, device=device)
+            scaled = dtype == torch.float8_e4m3fn
+            self.k_scale = torch.zeros(shape, dtype=torch.float32, device=device) if scaled else None
+            self.v_scale = torch.zeros(shape, dtype=torch.float32, device=device) if scaled else None
         self.weights = torch.zeros(shape, dtype=torch.float32, device=device) if track_weights else None
         self.index = torch.zeros(shape, dtype=torch.int32, device=device) if track_weights else None
 
@@ -114,11 +138,11 @@ class KVCache:
         return block_tables[seq, place // self.page].long() * self.page + place % self.page
 
     def append(self, k, v, slots, *, q=None, positions=None, cos_sin=None, sections=None, interleaved=False,
-               index=None):
+               index=None, q_norm=None, k_norm=None, eps=1e-6):
         """kv_append on these pages."""
         return kv_append(k, v, self.k, self.v, slots, q=q, positions=positions, cos_sin=cos_sin, sections=sections,
                          interleaved=interleaved, index=index, k_scale=self.k_scale, v_scale=self.v_scale,
-                         weights=self.weights, index_pages=self.index)
+                         weights=self.weights, index_pages=self.index, q_norm=q_norm, k_norm=k_norm, eps=eps)
 
     def attend(self, q, block_tables, lengths, *, scale=None, accumulate=None, max_length=None, return_lse=False):
         """kv_attend on these pages; accumulates weights where the cache tracks them, unless told not to."""
@@ -140,6 +164,11 @@ class KVCache:
 
 @torch.library.register_fake("nve_ops::kv_append")
 def _kv_append_fake(k, v, k_pages, v_pages, slots, q, *rest):
+    return k.new_empty((0,) if q is None else q.shape)
+
+
+@torch.library.register_fake("nve_ops::kv_append_norm")
+def _kv_append_norm_fake(k, v, k_pages, v_pages, slots, q, *rest):
     return k.new_empty((0,) if q is None else q.shape)
 
 
