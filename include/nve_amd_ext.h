@@ -353,6 +353,44 @@ NVE_C_API nve_status_t nve_amd_kv_evict(const nve_amd_kv_pages_t* pages,
                                         const nve_amd_kv_evict_t* call, void* workspace,
                                         uint64_t workspace_bytes, void* stream);
 
+/* A token for every row of logits [num_rows, vocab_size] (FLOAT32, FLOAT16 or
+ * BFLOAT16, rows row_stride elements apart), drawn with u[row] in [0, 1):
+ *   w_i = exp((x_i - max x) / temperature)
+ * kept are, in the order (x descending, index ascending), the first top_k (0 or
+ * at least vocab_size: all), of these the ones whose preceding sum of w is below
+ * top_p times the sum over them (1 or more: all; the first one always), and of
+ * these the ones with w_i >= min_p.  The token is the first index i, in the
+ * vocabulary's order, at which the sum of the kept w_j, j <= i, exceeds u times
+ * their sum.  temperature 0: the first of the largest logits.  Exponentials and
+ * sums are 64-bit.  temperatures, top_ks, top_ps and min_ps (device, [num_rows])
+ * hold a limit for each row; NULL: the one value beside it counts for all.  In
+ * device memory a temperature that is not above 0 counts as 0, a top_k below 1
+ * as 0, a top_p or min_p that is no number as none, one outside [0, 1] as the
+ * nearer of 0 and 1.  Logits that are no number count as -infinity; a row of
+ * nothing else gives -1.  Where a logit is +infinity the others have no weight.
+ * workspace: device memory of nve_amd_sample_workspace_size bytes, 16-byte
+ * aligned. */
+typedef struct {
+  int64_t num_rows;
+  int64_t vocab_size;
+  nve_data_type_t dtype;
+  int32_t top_k;
+  const void* logits;
+  int64_t row_stride;
+  const float* u;
+  const float* temperatures;
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  float temperature;
+  float top_p;
+  float min_p;
+  int64_t* tokens;
+} nve_amd_sample_t;
+NVE_C_API nve_status_t nve_amd_sample_workspace_size(const nve_amd_sample_t* call, uint64_t* bytes);
+NVE_C_API nve_status_t nve_amd_sample(const nve_amd_sample_t* call, void* workspace,
+                                      uint64_t workspace_bytes, void* stream);
+
 /* Log level (include/logging.hpp:34-203): messages at or below the level are
  * written, errors to stderr and the rest to stdout.  Levels: 0 critical,
  * 10 error, 20 warning, 30 perf, 40 info, 100 verbose.  The initial level is

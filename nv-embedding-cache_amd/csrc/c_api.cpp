@@ -14,6 +14,7 @@
 #include "host_layer.hpp"
 #include "kernels/noalloc_launch.hpp"
 #include "kv_cache.hpp"
+#include "sample.hpp"
 #include "layers.hpp"
 #include "trace.hpp"
 
@@ -1055,6 +1056,22 @@ nve_status_t nve_amd_kv_evict(const nve_amd_kv_pages_t* pages, const nve_amd_kv_
   C_TRY
   NVE_TRACE("nve_amd_kv_evict");
   kv_evict_run(pages, call, workspace, workspace_bytes, (hipStream_t)stream);
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
+nve_status_t nve_amd_sample_workspace_size(const nve_amd_sample_t* call, uint64_t* bytes) {
+  C_TRY
+  NVE_CHECK_ARG(bytes != nullptr, "bytes must not be NULL");
+  *bytes = sample_workspace_bytes(call);
+  return NVE_SUCCESS;
+  C_CATCH
+}
+
+nve_status_t nve_amd_sample(const nve_amd_sample_t* call, void* workspace, uint64_t workspace_bytes, void* stream) {
+  C_TRY
+  NVE_TRACE("nve_amd_sample");
+  sample_run(call, workspace, workspace_bytes, (hipStream_t)stream);
   return NVE_SUCCESS;
   C_CATCH
 }

@@ -113,6 +113,12 @@ class KvAttend(ctypes.Structure):
                 ("max_length", I64), ("scale", ctypes.c_float), ("accumulate", I32)]
 
 
+class Sample(ctypes.Structure):
+    _fields_ = [("num_rows", I64), ("vocab_size", I64), ("dtype", I32), ("top_k", I32), ("logits", P), ("row_stride", I64),
+                ("u", P), ("temperatures", P), ("top_ks", P), ("top_ps", P), ("min_ps", P),
+                ("temperature", ctypes.c_float), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float), ("tokens", P)]
+
+
 class KvEvict(ctypes.Structure):
     _fields_ = [("num_seqs", I64), ("block_tables", P), ("table_stride", I64), ("max_pages", I64),
                 ("lengths", P), ("new_lengths", P), ("budget", I64), ("sinks", I64), ("recent", I64)]
@@ -203,6 +209,8 @@ SIGNATURES = {
     "nve_amd_kv_evict_workspace_size": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvEvict),
                                               ctypes.POINTER(U64)]),
     "nve_amd_kv_evict": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvEvict), P, U64, P]),
+    "nve_amd_sample_workspace_size": (I32, [ctypes.POINTER(Sample), ctypes.POINTER(U64)]),
+    "nve_amd_sample": (I32, [ctypes.POINTER(Sample), P, U64, P]),
 }
 
 _lib = None

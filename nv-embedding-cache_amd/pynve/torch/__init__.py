@@ -19,7 +19,8 @@ fills.  Shape inference (the fake kernels) uses only the baked
 pynve/torch/__init__.py does.
 
 The library also holds the operators of the paged key-value cache (nve_kv),
-nve_ops::kv_append, kv_attend, kv_attend_lse and kv_evict, for HIP tensors.
+nve_ops::kv_append, kv_append_norm, kv_attend, kv_attend_lse and kv_evict, and
+token sampling (nve_sample), nve_ops::sample_tokens, for HIP tensors.
 """
 import ctypes
 import os
