@@ -11,19 +11,24 @@
 // long here as one in 32.  Sums that pick a cut are integers (weights times 2^shift), so that the order
 // of the LDS additions changes nothing.
 //
-// Bound: the logits' bytes, read once.  scan_kernel reads them and leaves the maximum of every 64
-// neighbours (a group) and, for rows that need the whole distribution's mass, the mass of every wave's
-// unit.  pick_kernel, a workgroup a row, goes on with these:
-//   nothing is cut off     the unit that u times the mass falls into is read again
-//   few tokens are kept    k maxima above a value are k tokens above it, and weights of maxima that sum
-//                          to p of all are a nucleus: only groups whose maximum is above such a value
-//                          are read again, and their values above it sorted
-//   a wide nucleus         a histogram of the row's masses, then the masses of units above the cut's bin
-// select() serves what is left (a large top-k, infinities, many equals at a wide cut, vocabularies of
-// more than 2^19): it shrinks the range that the cut is in by histograms, from nothing but the row.
+// Bound: the logits' bytes, read once.
+//   scan_kernel    reads them and leaves the maximum of every 64 or 16 neighbours (a group) and, for
+//                  rows that need the whole distribution's mass, the mass of every wave's unit
+//   pick_kernel    a workgroup a row.  Nothing is cut off: the unit that u times the mass falls into is
+//                  read again.  Few tokens are kept: k maxima above a value are k tokens above it, and
+//                  maxima whose weights sum to p of all are a nucleus, so only groups with a maximum
+//                  above such a value are read again, and their values above it sorted
+//   slice_kernel   up to 8 workgroups for each row that pick_kernel found too wide (a flat nucleus, a low
+//                  min-p): histograms of mass.  Launched where the limits allow such rows
+//   rest_kernel    those rows: the cut's bin is gathered and sorted, the slice that u falls into read
+//                  again; and what is left (a top-k of over 2,048 or of more than there are groups,
+//                  infinities, many equals at a wide cut), with sample_row() (sample_select.cuh)
+// Vocabularies of more than 2^19 are sample_row()'s alone.  It is no function that pick_kernel calls: a
+// kernel with a stack took 20 us where one without took 6.
 #include <math.h>
 
 #include <algorithm>
+#include <array>
 
 #include "../dtypes.hpp"
 #include "kv_common.cuh"
@@ -36,19 +41,31 @@ namespace {
 
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
-constexpr int kCandidates = 2048;        // sorted at most
+constexpr int kCandidates = 2 * kThreads;  // sorted at most
+constexpr int kCounted = 256;              // placed by counting at most: 64 cost 0.5 us, sorting them 3.7
 constexpr int kMostGroups = 8192;
 constexpr int kMostUnits = 512;
 constexpr int kPieces = 4;               // 16-byte pieces of a lane in a unit
-constexpr int64_t kMostVocab = 1 << 19;  // of the two kernels: 8192 groups, 512 units
+constexpr int kMostSlices = 8;           // of a wide row
+constexpr int64_t kMostVocab = 1 << 19;  // of these kernels: 8192 groups, 512 units
 
-// What scan_kernel leaves of the rows of a launch.
+// A row that pick_kernel left.
+struct Wide {
+  int32_t kind;             // 0: none; 1: a nucleus; 2: every weight of min_p and more; 3: for sample_row()
+  float top, least;         // the greatest value; one below the cut
+  unsigned long long target;  // the nucleus' mass times 2^shift
+};
+
+// What the kernels leave for the ones behind them, of the rows of a launch.
 struct Left {
   int64_t groups, units;
   int32_t group;      // values
+  int32_t slices, slice_units;
   float* group_top;   // [rows, groups]
   float* unit_top;    // [rows, units]
   double* unit_mass;  // [rows, units], relative to the unit's maximum
+  Wide* wide;         // [rows]
+  unsigned long long* bins;  // [rows, slices, kBins]
 };
 
 // A row's limits.
@@ -72,30 +89,67 @@ struct Limits {
   __device__ __forceinline__ bool all_mass() const { return !greedy && !k_on && (p_on || !low_on); }
 };
 
-// 2^z for z <= 0, to some 2^-52: a table of 2^(j / 32) and the exponential's series up to the fifth power for
-// the rest, |r| <= 1/64, whose next term is (ln 2 / 64)^6 / 720 = 2.2e-15.  2^-1100 and less is 0, and so
-// is what is no number.
+// ---------------------------------------------------------------------------
+// 2^z in 64 bits
+// ---------------------------------------------------------------------------
+constexpr int kSteps = 256;  // of the table
+
+// 2^(j / kSteps) from the exponential's series, with j taken off the exponent's field again, so that
+// adding the whole exponent (in units of 1 / kSteps) to the high word gives the power.
+constexpr std::array<uint64_t, kSteps> make_powers() {
+  std::array<uint64_t, kSteps> t{};
+  for (int j = 0; j < kSteps; ++j) {
+    const long double x = 0.693147180559945309417232121458L * j / kSteps;
+    long double term = 1, sum = 1;
+    for (int n = 1; n < 30; ++n) {
+      term *= x / n;
+      sum += term;
+    }
+    // 1 <= sum < 2: its 52 bits behind the point
+    uint64_t bits = 0;
+    long double rest = sum - 1;
+    for (int b = 0; b < 52; ++b) {
+      rest *= 2;
+      bits <<= 1;
+      if (rest >= 1) {
+        bits |= 1;
+        rest -= 1;
+      }
+    }
+    if (rest >= 0.5L) ++bits;
+    t[j] = (bits | (uint64_t)1023 << 52) - ((uint64_t)j << (52 - 8));
+  }
+  return t;
+}
+__constant__ const std::array<uint64_t, kSteps> kPowers = make_powers();
+static_assert(kSteps == 1 << 8);
+
+// 2^z for z <= 0: the table and the series up to the third power for the rest, |r| <= 1/512, whose next
+// term is (ln 2 / 512)^4 / 24 = 1.4e-13.  Less than 2^-1000, and what is no number, is 0 (parts(): 2^-1000,
+// nothing beside a sum of 1 and more).
 struct Exp2 {
-  const double* table;
-  static __device__ __forceinline__ void fill(double* t) {
-    if (threadIdx.x < 32) t[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  const uint64_t* table;
+  static __device__ __forceinline__ void fill(uint64_t* t) {
+    if (threadIdx.x < kSteps) t[threadIdx.x] = kPowers[threadIdx.x];
+  }
+  // The power and the factor that completes it.
+  __device__ __forceinline__ void parts(double z, double& power, double& factor) const {
+    z = __builtin_fmax(z, -1000.0);
+    const double t = z + 0x1.8p44;  // a multiple of 1 / 256
+    const int n = (int)__double_as_longlong(t);
+    const double r = z - (t - 0x1.8p44);
+    factor = fma(r, fma(r, fma(r, 0.05550410866482158, 0.2402265069591007), 0.6931471805599453), 1.0);
+    const uint64_t p = table[n & (kSteps - 1)];
+    power = __hiloint2double((int)(p >> 32) + (n << 12), (int)p);
   }
   __device__ __forceinline__ double operator()(double z) const {
-    z = fmax(z, -1100.0);
-    const double t = z + 0x1.8p47;  // a multiple of 1/32
-    const int n = (int)__double_as_longlong(t);
-    const double r = z - (t - 0x1.8p47);
-    double y = fma(r, 0.0013333558146428443, 0.009618129107628477);
-    y = fma(r, y, 0.05550410866482158);
-    y = fma(r, y, 0.2402265069591007);
-    y = fma(r, y, 0.6931471805599453);
-    y = fma(r, y, 1.0);
-    return ldexp(table[n & 31] * y, n >> 5);
+    double power, factor;
+    parts(z, power, factor);
+    return z >= -1000.0 ? power * factor : 0.0;
   }
 };
 
-// A lane's 16 bytes of a row from `first` on; what is past the row's end, or no number, is minus infinity
-// (or stays a NaN, which every comparison leaves out).
+// A lane's 16 bytes of a row from `first` on; what is past the row's end is minus infinity.
 template <int DT>
 struct Piece {
   static constexpr int kValues = 16 / value_elem_bytes(DT);
@@ -118,6 +172,9 @@ constexpr int unit_values() {
   return kPieces * 64 * Piece<DT>::kValues;
 }
 
+// ---------------------------------------------------------------------------
+// lanes and workgroups
+// ---------------------------------------------------------------------------
 // Maxima over 2, 4, 8, 16 or 64 neighbouring lanes.
 template <int CTRL>
 __device__ __forceinline__ float max_with(float x) {
@@ -136,6 +193,120 @@ __device__ __forceinline__ float lanes_max(float x) {
   return x;
 }
 
+// x of the lane that CTRL names, 0 where it names none; every lane of the wave is on.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T moved(T x) {
+  uint32_t w[sizeof(T) / 4];
+  __builtin_memcpy(w, &x, sizeof(T));
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) {
+    w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[i], CTRL, ROWS, 0xf, false);
+    asm volatile("" : "+v"(w[i]));  // not moved under a condition, where some lanes are off
+  }
+  __builtin_memcpy(&x, w, sizeof(T));
+  return x;
+}
+// Running sums in each row of 16 lanes, and over the wave.
+template <typename T>
+__device__ __forceinline__ T row_scan(T x) {
+  x += moved<0x111, 0xf>(x);
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ T lanes_scan(T x) {
+  x = row_scan(x);
+  x += moved<0x142, 0xa>(x);
+  x += moved<0x143, 0xc>(x);
+  return x;
+}
+// x of one lane, the same for all.
+template <typename T>
+__device__ __forceinline__ T of_lane(T x, int lane) {
+  uint32_t w[sizeof(T) / 4];
+  __builtin_memcpy(w, &x, sizeof(T));
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) w[i] = (uint32_t)__builtin_amdgcn_readlane((int)w[i], lane);
+  __builtin_memcpy(&x, w, sizeof(T));
+  return x;
+}
+
+// The sum over 4, 8 or 16 neighbouring lanes.
+template <typename T>
+__device__ __forceinline__ T group_sum(T x, int bits) {
+  x += moved<0xb1, 0xf>(x);
+  x += moved<0x4e, 0xf>(x);
+  if (bits >= 3) x += moved<0x141, 0xf>(x);
+  if (bits >= 4) x += moved<0x140, 0xf>(x);
+  return x;
+}
+
+// x of the threads up to and including this one, added in one order; total: of all.
+template <typename T>
+__device__ __forceinline__ T block_scan(T x, T* red, T& total) {
+  static_assert(kWaves == 16);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  x = lanes_scan(x);
+  __syncthreads();
+  if (lane == 63) red[wave] = x;
+  __syncthreads();
+  const T r = row_scan(red[lane & 15]);
+  total = of_lane(r, 15);
+  if (wave > 0) x += of_lane(r, wave - 1);
+  return x;
+}
+
+// The order of tokens as one number: the value, then the lower index first.  Both zeros are one value.
+__device__ __forceinline__ uint64_t key_of(float x, int64_t index) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return (uint64_t)o << 32 | (uint32_t)~(uint32_t)index;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ int64_t index_of(uint64_t key) { return (uint32_t)~(uint32_t)key; }
+
+// Sorts n <= kCandidates keys, the greatest first; those behind them up to a power of two become 0.
+__device__ __forceinline__ void sort_keys(uint64_t* keys, int n) {
+  const int tid = threadIdx.x;
+  int size2 = 2;
+  while (size2 < n) size2 <<= 1;
+  for (int i = n + tid; i < size2; i += kThreads) keys[i] = 0;
+  __syncthreads();
+  const bool one_wave = size2 <= 128;
+  if (!one_wave || tid < 64) {
+    for (int size = 2; size <= size2; size <<= 1) {
+      for (int stride = size >> 1; stride > 0; stride >>= 1) {
+        if (tid < size2 / 2) {
+          const int low = 2 * tid - (tid & (stride - 1)), high = low + stride;
+          const uint64_t x = keys[low], y = keys[high];
+          if ((x < y) == ((low & size) == 0)) {
+            keys[low] = y;
+            keys[high] = x;
+          }
+        }
+        if (one_wave) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        else __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// kBins bins of one width from `high` down; the last one has all that is below, and what is no number.
+struct Steps {
+  float high, scale;
+  __device__ __forceinline__ Steps(float high, float low) : high(high) {
+    const float width = high - low;
+    scale = width > 0.0f ? fminf((kBins - 0.1f) / width, 3e38f) : 3e38f;
+  }
+  __device__ __forceinline__ int of(float x) const { return (int)fminf((high - x) * scale, kBins - 1.0f); }
+};
+
 // ---------------------------------------------------------------------------
 // the first kernel: a unit a wave
 // ---------------------------------------------------------------------------
@@ -144,19 +315,24 @@ constexpr int kScanThreads = 256;
 template <int DT, int GROUP>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Sample a, const Left l, const int blocks) {
   constexpr int kValues = Piece<DT>::kValues, kLanes = GROUP / kValues;
-  __shared__ double table[32];
+  __shared__ uint64_t table[kSteps];
   const int lane = threadIdx.x & 63;
   const int64_t row = blockIdx.x / blocks;
   const int64_t unit = (int64_t)(blockIdx.x - row * blocks) * (kScanThreads / 64) + (threadIdx.x >> 6);
+  const kv_elem<DT>* p = reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride;
+  const int64_t base = unit * unit_values<DT>() + lane * kValues;
+  Piece<DT> x[kPieces];
+  if ((unit + 1) * unit_values<DT>() <= a.vocab) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, INT64_MAX);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
+  }
   const Limits limits(a, row);
   if (limits.all_mass()) Exp2::fill(table);
   __syncthreads();
   if (unit >= l.units) return;
-  const kv_elem<DT>* p = reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride;
-  const int64_t base = unit * unit_values<DT>() + lane * kValues;
-  Piece<DT> x[kPieces];
-#pragma unroll
-  for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
@@ -177,8 +353,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Sample a, cons
 #pragma unroll
     for (int j = 0; j < kPieces; ++j)
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) sum += exp2_of(((double)x[j][i] - high) * limits.scale);
-    sum = wave_sum(sum);
+      for (int i = 0; i < kValues; ++i) {
+        double power, factor;
+        exp2_of.parts(((double)x[j][i] - high) * limits.scale, power, factor);
+        sum = fma(power, factor, sum);
+      }
+    sum = of_lane(lanes_scan(sum), 63);
   }
   if (lane == 0) {
     l.unit_top[row * l.units + unit] = top;
@@ -187,124 +367,42 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Sample a, cons
 }
 
 // ---------------------------------------------------------------------------
-// the second kernel: a row a workgroup
+// a row in one workgroup
 // ---------------------------------------------------------------------------
-struct PickShared {
-  uint64_t keys[kCandidates];    // in the vocabulary's order
-  uint64_t sorted[kCandidates];  // the greatest first
+struct RowShared {
   union {
-    uint16_t groups[kMostGroups];
+    float tops[kMostGroups];
+    struct {
+      uint64_t keys[kCandidates];  // in the vocabulary's order
+      union {
+        uint64_t sorted[kCandidates];  // the greatest first
+        double weights[kCandidates];   // in the vocabulary's order, 0 where one is not kept
+      };
+    };
+  };
+  union {
+    uint16_t groups[kCandidates];
     struct {
       uint32_t count[kBins];
       unsigned long long mass[kBins];
     };
   };
-  double unit[kMostUnits];
+  uint64_t table[kSteps];
+  double unit[kMostUnits / kMostSlices];
   double red_sum[kWaves];
   unsigned long long red_mass[kWaves];
   int red_count[kWaves];
   float red_low[kWaves], red_high[kWaves];
-  double table[32];
-  int found, last, bin, bin2;
-  int n;
-  double before;
+  unsigned long long slice[kMostSlices];
+  int first_item[kWaves], last_item[kWaves], bin, n;
+  double first_before[kWaves], last_before[kWaves];
   unsigned long long before_mass;
   uint64_t cut;
 };
 
 union AnyShared {
   SelectShared select;
-  PickShared pick;
-};
-
-// The order of tokens as one number: the value, then the lower index first.  Both zeros are one value.
-__device__ __forceinline__ uint64_t key_of(float x, int64_t index) {
-  const uint32_t b = __float_as_uint(x + 0.0f);
-  const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-  return (uint64_t)o << 32 | (uint32_t)~(uint32_t)index;
-}
-__device__ __forceinline__ float value_of(uint64_t key) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
-}
-__device__ __forceinline__ int64_t index_of(uint64_t key) { return (uint32_t)~(uint32_t)key; }
-
-// x of the threads up to and including this one, added in one order; total: of all.
-template <typename T>
-__device__ __forceinline__ T block_scan(T x, T* red, T& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T o = __shfl_up(x, d);
-    if (lane >= d) x += o;
-  }
-  __syncthreads();
-  if (lane == 63) red[wave] = x;
-  __syncthreads();
-  T before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const T r = red[w];
-    if (w < wave) before += r;
-    total += r;
-  }
-  return before + x;
-}
-
-// The first of n <= 2 kThreads items at which the running sum of their weights, from `base` on, exceeds the
-// target; the last one with a weight where none does.  share: the target is u times the sum.
-template <typename F>
-__device__ __forceinline__ int pick_item(PickShared& s, int n, double base, double target, bool share, F weight) {
-  const int i = 2 * threadIdx.x;
-  const double w0 = i < n ? weight(i) : 0.0, w1 = i + 1 < n ? weight(i + 1) : 0.0;
-  double total;
-  const double end = block_scan(w0 + w1, s.red_sum, total);
-  if (threadIdx.x == 0) {
-    s.found = 1 << 30;
-    s.last = 0;
-  }
-  __syncthreads();
-  if (share) target *= total;
-  if (w0 > 0.0 && base + (end - w1) > target) atomicMin(&s.found, i);
-  else if (w1 > 0.0 && base + end > target) atomicMin(&s.found, i + 1);
-  if (w1 > 0.0) atomicMax(&s.last, i + 1);
-  else if (w0 > 0.0) atomicMax(&s.last, i);
-  __syncthreads();
-  return s.found < (1 << 30) ? s.found : s.last;
-}
-
-// Sorts n <= kCandidates keys, the greatest first; those behind them up to a power of two become 0.
-__device__ __forceinline__ void sort_keys(uint64_t* keys, int n) {
-  const int tid = threadIdx.x;
-  int size2 = 2;
-  while (size2 < n) size2 <<= 1;
-  for (int i = n + tid; i < size2; i += kThreads) keys[i] = 0;
-  __syncthreads();
-  for (int size = 2; size <= size2; size <<= 1) {
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      if (tid < size2 / 2) {
-        const int low = 2 * tid - (tid & (stride - 1)), high = low + stride;
-        const uint64_t x = keys[low], y = keys[high];
-        if ((x < y) == ((low & size) == 0)) {
-          keys[low] = y;
-          keys[high] = x;
-        }
-      }
-      __syncthreads();
-    }
-  }
-}
-static_assert(kCandidates == 2 * kThreads);
-
-// kBins bins of one width from `high` down; the last one has all that is below, and what is no number.
-struct Steps {
-  float high, scale;
-  __device__ __forceinline__ Steps(float high, float low) : high(high) {
-    const float width = high - low;
-    scale = width > 0.0f ? fminf((kBins - 0.1f) / width, 3e38f) : 3e38f;
-  }
-  __device__ __forceinline__ int of(float x) const { return (int)fminf((high - x) * scale, kBins - 1.0f); }
+  RowShared row;
 };
 
 template <int DT, int GROUP>
@@ -313,16 +411,17 @@ struct Pick {
   const Sample& a;
   const Left& l;
   const Limits& limits;
-  PickShared& s;
+  RowShared& s;
   const int64_t row;
   const kv_elem<DT>* p;
+  double mass_scale;
   float top;
-  double high, mass_scale;
-  double u;
+  double high, u;
 
   __device__ __forceinline__ double weight(float x) const {
     return Exp2{s.table}(((double)x - high) * limits.scale);
   }
+  // A weight times 2^shift, rounded; the sum is below 2^52.
   __device__ __forceinline__ unsigned long long mass_of(double w) const {
     return (unsigned long long)__double_as_longlong(w * mass_scale + 0x1p52) & ((1ull << 52) - 1);
   }
@@ -330,259 +429,208 @@ struct Pick {
     if (threadIdx.x == 0) a.tokens[row] = token;
   }
 
-  // The bin at which the running sum of the bins' numbers reaches the target, or -1; its predecessors' sum.
-  template <typename T>
-  __device__ __forceinline__ int bin_at(const T* bins, T target, T& before) const {
+  // The bin at which the running sum of two bins a thread reaches the target, or -1; s.before_mass: before it.
+  __device__ __forceinline__ int bin_at(unsigned long long x0, unsigned long long x1, unsigned long long target) const {
     const int tid = threadIdx.x;
-    const unsigned long long x0 = bins[2 * tid], x1 = bins[2 * tid + 1];
     unsigned long long total;
     const unsigned long long end = block_scan<unsigned long long>(x0 + x1, s.red_mass, total);
-    if (tid == 0) s.bin = -1;
-    __syncthreads();
-    const unsigned long long b1 = end - x1, b0 = b1 - x0, t = target;
-    if (b0 < t && b1 >= t) {
+    if (total < target) return -1;
+    const unsigned long long b1 = end - x1, b0 = b1 - x0;
+    if (b0 < target && b1 >= target) {
       s.bin = 2 * tid;
       s.before_mass = b0;
-    } else if (b1 < t && end >= t) {
+    } else if (b1 < target && end >= target) {
       s.bin = 2 * tid + 1;
       s.before_mass = b1;
     }
     __syncthreads();
-    before = (T)s.before_mass;
     return s.bin;
   }
 
-  // The token within a unit: values from `cut` on, the least weight `low`.
-  __device__ __forceinline__ int64_t pick_in_unit(int64_t unit, double base, double target, uint64_t cut, double low) const {
-    const int64_t first = unit * kUnit;
-    const int n = (int)min((int64_t)kUnit, a.vocab - first);
-    return first + pick_item(s, n, base, target, false, [&](int i) {
-      const float x = (float)p[first + i];
-      if (!(x > -INFINITY) || key_of(x, first + i) < cut) return 0.0;
-      const double w = weight(x);
-      return w >= low ? w : 0.0;
-    });
-  }
-
-  // The unit whose mass the share u falls into (s.unit has the units' masses), and the token in it.
-  __device__ __forceinline__ void pick_unit(uint64_t cut, double low) const {
-    const int tid = threadIdx.x, n = (int)l.units;
-    const int unit = pick_item(s, n, 0.0, u, true, [&](int i) { return s.unit[i]; });
-    // the sum before it, and the target, from the same numbers
+  // The first of the threads' two items each at which the running sum of their weights, from `base` on, exceeds
+  // the target; the last one with a weight where none does.  share: the target is that times the sum.
+  // before: the running sum before it.
+  __device__ __forceinline__ int pick_item(double w0, double w1, double base, double& target, bool share,
+                                           double& before) const {
+    const int i = 2 * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double total;
-    const double own = tid < n ? s.unit[tid] : 0.0;
-    const double end = block_scan(own, s.red_sum, total);
+    const double end = base + block_scan(w0 + w1, s.red_sum, total);
+    if (share) target *= total;
+    const bool f0 = w0 > 0.0 && end - w1 > target, f1 = w1 > 0.0 && end > target;
+    const uint64_t over = __ballot(f0 || f1), any = __ballot(w0 > 0.0 || w1 > 0.0);
+    if (over ? lane == __builtin_ctzll(over) : lane == 0) {
+      s.first_item[wave] = over ? (f0 ? i : i + 1) : -1;
+      s.first_before[wave] = f0 ? end - w1 - w0 : end - w1;
+    }
+    if (any ? lane == 63 - __builtin_clzll(any) : lane == 0) {
+      s.last_item[wave] = any ? (w1 > 0.0 ? i + 1 : i) : -1;
+      s.last_before[wave] = w1 > 0.0 ? end - w1 : end - w1 - w0;
+    }
     __syncthreads();
-    if (tid == unit) s.before = end - own;
+    const uint64_t first = __ballot(s.first_item[lane & 15] >= 0) & 0xffff;
+    const uint64_t last = __ballot(s.last_item[lane & 15] >= 0) & 0xffff;
+    const int w = first ? __builtin_ctzll(first) : last ? 63 - __builtin_clzll(last) : 0;
+    const int item = first ? s.first_item[w] : s.last_item[w];
+    before = first ? s.first_before[w] : s.last_before[w];
     __syncthreads();
-    answer(pick_in_unit(unit, s.before, u * total, cut, low));
+    return item;
   }
 
-  // A wide nucleus (target: the mass it needs, in units of 2^-shift), or the tokens of weight `low` and more
-  // (target 0).  all: the mass of all.  false: not decided here.
-  __device__ __forceinline__ bool wide(unsigned long long target, double all) const {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // a nucleus leaves out (1 - p) of the mass at most, so its least weight is at least that over the vocabulary
-    float least = -INFINITY;
-    if (target > 0) {
-      const double depth = log2((double)a.vocab / ((1.0 - limits.p) * all)) / limits.scale;
-      if (!(depth < 1e30)) return false;
-      least = (float)(high - fmax(depth, 0.0) * 1.0001 - 1e-6 * fabs(high));
-      if (!(least > -3e38f)) return false;
-    }
-    const Steps steps(top, target > 0 ? least : top);
-    int bin = kBins;  // what is before it is kept whole
-    unsigned long long above = 0;
-    if (target > 0) {
-      for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0;
-      __syncthreads();
-      for (int64_t unit = wave; unit < l.units; unit += kWaves) {
-        const int64_t base = unit * kUnit + lane * kValues;
-        Piece<DT> x[kPieces];
+  // The token within a unit: values from `cut` on, the least weight `low`.
+  __device__ __forceinline__ void pick_in_unit(int64_t unit, double base, double target, uint64_t cut, double low) const {
+    const int64_t first = unit * kUnit;
+    double w[2];
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
-#pragma unroll
-        for (int j = 0; j < kPieces; ++j)
-#pragma unroll
-          for (int i = 0; i < kValues; ++i)
-            if (x[j][i] >= least) atomicAdd(&s.mass[steps.of(x[j][i])], mass_of(weight(x[j][i])));
+    for (int i = 0; i < 2; ++i) {
+      const int64_t at = first + 2 * threadIdx.x + i;
+      w[i] = 0.0;
+      if (2 * threadIdx.x + i < kUnit && at < a.vocab) {
+        const float x = (float)p[at];
+        const double y = weight(x);
+        if (x > -INFINITY && key_of(x, at) >= cut && y >= low) w[i] = y;
       }
-      __syncthreads();
-      bin = bin_at<unsigned long long>(s.mass, target, above);
-      if (bin < 0) return false;
     }
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    for (int64_t unit = wave; unit < l.units; unit += kWaves) {
-      const int64_t base = unit * kUnit + lane * kValues;
-      Piece<DT> x[kPieces];
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
-      double sum = 0.0;
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j)
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) {
-          const float v = x[j][i];
-          const int b = target > 0 ? steps.of(v) : 0;
-          if (b == bin && v >= least) {
-            const int at = atomicAdd(&s.n, 1);
-            if (at < kCandidates) s.sorted[at] = key_of(v, base + j * 64 * kValues + i);
-          } else if (b < bin && v > -INFINITY) {
-            const double w = weight(v);
-            sum += w >= limits.low ? w : 0.0;
-          }
-        }
-      sum = wave_sum(sum);
-      if (lane == 0) s.unit[unit] = sum;
-    }
-    __syncthreads();
-    uint64_t cut = 0;
-    const int n = s.n;
-    if (n > kCandidates) return false;
-    if (n > 0) {
-      sort_keys(s.sorted, n);
-      const int i = 2 * tid;
-      const double w0 = i < n ? weight(value_of(s.sorted[i])) : 0.0, w1 = i + 1 < n ? weight(value_of(s.sorted[i + 1])) : 0.0;
-      const unsigned long long m0 = mass_of(w0), m1 = i + 1 < n ? mass_of(w1) : 0;
-      unsigned long long total;
-      const unsigned long long end = above + block_scan<unsigned long long>((i < n ? m0 : 0) + m1, s.red_mass, total);
-      if (tid == 0) s.cut = s.sorted[n - 1];
-      __syncthreads();
-      const unsigned long long b1 = end - m1, b0 = b1 - m0;
-      if (i < n && b0 < target && b1 >= target) s.cut = s.sorted[i];
-      else if (i + 1 < n && b1 < target && end >= target) s.cut = s.sorted[i + 1];
-      __syncthreads();
-      cut = s.cut;
-      // the bin's kept values join their units, in the order of the sorting
-      for (int unit = tid; unit < l.units; unit += kThreads) {
-        double sum = s.unit[unit];
-        for (int j = 0; j < n && s.sorted[j] >= cut; ++j) {
-          if (index_of(s.sorted[j]) / kUnit != unit) continue;
-          const double w = weight(value_of(s.sorted[j]));
-          sum += w >= limits.low ? w : 0.0;
-        }
-        s.unit[unit] = sum;
-      }
-    } else if (target > 0) {
-      return false;
-    }
-    __syncthreads();
-    pick_unit(cut, limits.low);
-    return true;
+    double before;
+    answer(first + pick_item(w[0], w[1], base, target, false, before));
   }
 
-  // false: not decided here.
-  __device__ __forceinline__ bool run() {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (int)((l.groups + kThreads - 1) / kThreads), g0 = tid * per;
-    constexpr int kMostPer = kMostGroups / kThreads;
-    float tops[kMostPer];
-#pragma unroll
-    for (int i = 0; i < kMostPer; ++i)
-      tops[i] = i < per && g0 + i < l.groups ? l.group_top[row * l.groups + g0 + i] : -INFINITY;
-    float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kMostPer; ++i) {
-      hi = fmaxf(hi, tops[i]);
-      if (tops[i] > -INFINITY) lo = fminf(lo, tops[i]);
-    }
+  // Greatest and least of the finite ones of lo and hi over the workgroup.
+  __device__ __forceinline__ void reduce_range(float& lo, float& hi) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     hi = lanes_max<64>(hi);
     lo = -lanes_max<64>(-lo);
     if (lane == 0) {
       s.red_high[wave] = hi;
       s.red_low[wave] = lo;
     }
-    Exp2::fill(s.table);
     __syncthreads();
+    hi = lanes_max<16>(s.red_high[lane & 15]);
+    lo = -lanes_max<16>(-s.red_low[lane & 15]);
+  }
+
+  enum Found { kDone, kWide, kElse };
+
+  __device__ __forceinline__ Found run(Wide& left) {
+    const int tid = threadIdx.x;
+    Exp2::fill(s.table);
+    u = a.u[row] > 0.0f ? (double)a.u[row] : 0.0;
+    float lo = INFINITY, hi = -INFINITY;
+
+    double all = 0.0;  // the mass of all, where it counts
+    if (limits.all_mass()) {
+      const int i = 2 * tid;
+      float t[2] = {-INFINITY, -INFINITY};
+      double m[2] = {0.0, 0.0};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      hi = fmaxf(hi, s.red_high[w]);
-      lo = fminf(lo, s.red_low[w]);
+      for (int j = 0; j < 2; ++j) {
+        if (i + j < l.units) {
+          t[j] = l.unit_top[row * l.units + i + j];
+          m[j] = l.unit_mass[row * l.units + i + j];
+        }
+      }
+      hi = fmaxf(t[0], t[1]);
+      reduce_range(lo, hi);
+      top = hi;
+      high = hi;
+      if (top == -INFINITY) {
+        answer(-1);
+        return kDone;
+      }
+      if (top == INFINITY) return kElse;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 2; ++j) m[j] = t[j] > -INFINITY ? m[j] * weight(t[j]) : 0.0;
+      if (!limits.p_on) {
+        double target = u, before;
+        const int unit = pick_item(m[0], m[1], 0.0, target, true, before);
+        pick_in_unit(unit, before, target, 0, 0.0);
+        return kDone;
+      }
+      block_scan(m[0] + m[1], s.red_sum, all);
+      __syncthreads();
+      lo = INFINITY;
+      hi = -INFINITY;
     }
+
+    for (int64_t g = tid; g < l.groups; g += kThreads) {
+      const float t = l.group_top[row * l.groups + g];
+      s.tops[g] = t;
+      hi = fmaxf(hi, t);
+      if (t > -INFINITY) lo = fminf(lo, t);
+    }
+    reduce_range(lo, hi);
     top = hi;
     high = hi;
     if (top == -INFINITY) {
       answer(-1);
-      return true;
+      return kDone;
     }
-    if (top == INFINITY) return false;
-    u = a.u[row] > 0.0f ? (double)a.u[row] : 0.0;
-
-    double all = 0.0;  // the mass of all, where it counts
-    if (limits.all_mass()) {
-      double m = 0.0;
-      if (tid < l.units) {
-        const float t = l.unit_top[row * l.units + tid];
-        m = t > -INFINITY ? l.unit_mass[row * l.units + tid] * weight(t) : 0.0;
-        s.unit[tid] = m;
-      }
-      block_scan(m, s.red_sum, all);
-      if (!limits.p_on) {
-        __syncthreads();
-        pick_unit(0, 0.0);
-        return true;
-      }
-    }
+    if (top == INFINITY) return kElse;
 
     // candidates: values in the first `limit` + 1 steps and not below `least`
-    Steps steps(top, lo);
+    const Steps steps(top, lo);
     int limit = kBins;
     float least = -INFINITY;
     unsigned long long target = 0;
     if (limits.greedy) {
       least = top;
     } else {
-      if (limits.low_on && !limits.p_on && limits.scale > 0.0) {  // top-p's sums are of all of top-k's
+      // min-p's tokens are a part of a nucleus or hold all of it, but top-p's sum after top-k is of all of top-k's
+      if (limits.low_on && !(limits.k_on && limits.p_on) && limits.scale > 0.0) {
         // a little below the least weight's value: what is between is left out by its weight
         const double low = high + log2(limits.low) / limits.scale;
         least = (float)(low - 1e-6 * fabs(low) - 1e-6 * fabs(high));
       }
-      if (limits.k_on || limits.p_on) {
+      target = (unsigned long long)fmax(ceil(limits.p * all * mass_scale), 1.0);
+      if ((limits.k_on || limits.p_on) && a.vocab > kCandidates) {
+        if (limits.k_on && limits.k > kCandidates) return kElse;
         for (int i = tid; i < kBins; i += kThreads) {
           s.count[i] = 0;
           s.mass[i] = 0;
         }
         __syncthreads();
-        const bool by_mass = !limits.k_on;
-#pragma unroll
-        for (int i = 0; i < kMostPer; ++i) {
-          if (tops[i] > -INFINITY) {
-            const int b = steps.of(tops[i]);
+        for (int64_t g = tid; g < l.groups; g += kThreads) {
+          const float t = s.tops[g];
+          if (t > -INFINITY) {
+            const int b = steps.of(t);
             atomicAdd(&s.count[b], 1u);
-            if (by_mass) atomicAdd(&s.mass[b], mass_of(weight(tops[i])));
+            if (!limits.k_on) atomicAdd(&s.mass[b], mass_of(weight(t)));
           }
         }
         __syncthreads();
-        uint32_t before;
         if (limits.k_on) {
-          if (limits.k > kCandidates) return false;
-          limit = bin_at<uint32_t>(s.count, (uint32_t)limits.k, before);
-          if (limit < 0) return false;
+          limit = bin_at(s.count[2 * tid], s.count[2 * tid + 1], limits.k);
+          if (limit < 0) return kElse;
         } else {
-          target = (unsigned long long)fmax(ceil(limits.p * all * mass_scale), 1.0);
-          unsigned long long mass_before;
-          const int sure = bin_at<unsigned long long>(s.mass, target, mass_before);
-          const int many = bin_at<uint32_t>(s.count, (uint32_t)min((int64_t)768, (l.groups + 1) / 2), before);
-          limit = sure >= 0 && (many < 0 || sure < many) ? sure : many;
-          if (limit < 0) return wide(target, all);
+          const int sure = bin_at(s.mass[2 * tid], s.mass[2 * tid + 1], target);
+          if (sure >= 0 || !limits.low_on) {
+            // else the maxima that sum to most of it, if they are few: likely with all of it around them
+            limit = sure >= 0 ? sure : bin_at(s.mass[2 * tid], s.mass[2 * tid + 1], target - target / 4);
+            if (limit < 0) limit = kBins;
+          }
         }
       }
+      // A nucleus leaves out (1 - p) of the mass at most, so its least weight is at least that over the vocabulary.
+      float bound = least;
+      if (limits.p_on) {
+        const double depth = log2((double)a.vocab / ((1.0 - limits.p) * all)) / limits.scale;
+        bound = (float)(high - fmax(depth, 0.0) * 1.0001 - 1e-6 * fabs(high));
+      }
+      left = Wide{limits.p_on ? 1 : 2, top, bound, target};
     }
+    const Found rest = !limits.k_on && left.least > -3e38f ? kWide : kElse;
     auto wanted = [&](float x) { return x >= least && x > -INFINITY && (limit >= kBins || steps.of(x) <= limit); };
 
     // the groups with candidates, in order
-    int mine = 0;
-#pragma unroll
-    for (int i = 0; i < kMostPer; ++i) mine += wanted(tops[i]);
+    const int per = (int)((l.groups + kThreads - 1) / kThreads), g0 = tid * per;
+    uint32_t mine = 0;
+    for (int i = 0; i < per; ++i) mine |= (uint32_t)(g0 + i < l.groups && wanted(s.tops[g0 + i])) << i;
     int groups;
-    int at = block_scan(mine, s.red_count, groups) - mine;
+    int at = block_scan((int)__popc(mine), s.red_count, groups) - __popc(mine);
     bool few = groups <= kCandidates;
     int n = 0;
     if (few) {
-#pragma unroll
-      for (int i = 0; i < kMostPer; ++i)
-        if (wanted(tops[i])) s.groups[at++] = (uint16_t)(g0 + i);
+      for (; mine; mine &= mine - 1) s.groups[at++] = (uint16_t)(g0 + __builtin_ctz(mine));
       __syncthreads();
       // their candidates, in order
       for (int b0 = 0; b0 < groups; b0 += kThreads / kLanes) {
@@ -609,57 +657,274 @@ struct Pick {
       }
     }
     __syncthreads();
-    if (limits.greedy) {  // the first group with the maximum has the first of them
+    if (limits.greedy) {  // the first of them
       if (few) answer(index_of(s.keys[0]));
-      return few;
+      return few ? kDone : kElse;
     }
-    if (!few) {
-      if (limits.k_on) return false;
-      return wide(target, all);
-    }
+    if (!few) return rest;
 
-    uint64_t cut = 0;
-    if (limits.k_on || limits.p_on) {
-      for (int i = tid; i < n; i += kThreads) s.sorted[i] = s.keys[i];
-      sort_keys(s.sorted, n);
-      const int kept = limits.k_on ? (int)min((int64_t)n, limits.k) : n;
-      cut = s.sorted[kept - 1];
-      if (limits.p_on) {
-        const int i = 2 * tid;
-        const unsigned long long m0 = i < kept ? mass_of(weight(value_of(s.sorted[i]))) : 0;
-        const unsigned long long m1 = i + 1 < kept ? mass_of(weight(value_of(s.sorted[i + 1]))) : 0;
-        unsigned long long total;
-        const unsigned long long end = block_scan<unsigned long long>(m0 + m1, s.red_mass, total);
-        if (limits.k_on) target = (unsigned long long)fmax(ceil(limits.p * (double)total), 1.0);
-        else if (total < target) return wide(target, all);  // the candidates are not all of the nucleus
-        if (tid == 0) s.cut = cut;
+    const int i = 2 * tid;
+    double w[2] = {0.0, 0.0};
+    double share = u, before;
+    if (n <= kCounted) {
+      // every token's place in the order, and the mass before it, by comparing it with all: 4 to 16 threads each
+      if (tid < n) {
+        const double y = weight(value_of(s.keys[tid]));
+        s.weights[tid] = y >= limits.low ? y : 0.0;
+        s.mass[tid] = mass_of(y);
+      }
+      __syncthreads();
+      if (limits.k_on || limits.p_on) {
+        const int bits = n <= 64 ? 4 : n <= 128 ? 3 : 2, mine_at = tid >> bits;
+        uint32_t rank = 0;
+        unsigned long long ahead = 0, own = 0;
+        if (mine_at < n) {
+          const uint64_t key = s.keys[mine_at];
+          own = s.mass[mine_at];
+          for (int j = tid & ((1 << bits) - 1); j < n; j += 1 << bits) {
+            const bool first = s.keys[j] > key;
+            rank += first;
+            ahead += first ? s.mass[j] : 0;
+          }
+        }
+        rank = group_sum(rank, bits);
+        ahead = group_sum(ahead, bits);
+        bool kept = mine_at < n && (!limits.k_on || rank < limits.k);
+        if (limits.p_on) {
+          unsigned long long total;
+          block_scan<unsigned long long>(kept && (tid & ((1 << bits) - 1)) == 0 ? own : 0, s.red_mass, total);
+          if (limits.k_on) target = (unsigned long long)fmax(ceil(limits.p * (double)total), 1.0);
+          else if (total < target && !limits.low_on && a.vocab > kCandidates) return rest;  // not all of the nucleus
+          kept = kept && (ahead < target || rank == 0);
+        }
+        if (mine_at < n && !kept && (tid & ((1 << bits) - 1)) == 0) s.weights[mine_at] = 0.0;
         __syncthreads();
-        const unsigned long long b1 = end - m1, b0 = b1 - m0;
-        if (i < kept && b0 < target && b1 >= target) s.cut = s.sorted[i];
-        else if (i + 1 < kept && b1 < target && end >= target) s.cut = s.sorted[i + 1];
-        __syncthreads();
-        cut = s.cut;
+      }
+      if (i < n) w[0] = s.weights[i];
+      if (i + 1 < n) w[1] = s.weights[i + 1];
+    } else {
+      uint64_t cut = 0;
+      if (limits.k_on || limits.p_on) {
+        for (int j = tid; j < n; j += kThreads) s.sorted[j] = s.keys[j];
+        sort_keys(s.sorted, n);
+        const int kept = limits.k_on ? (int)min((int64_t)n, limits.k) : n;
+        cut = s.sorted[kept - 1];
+        if (limits.p_on) {
+          const unsigned long long m0 = i < kept ? mass_of(weight(value_of(s.sorted[i]))) : 0;
+          const unsigned long long m1 = i + 1 < kept ? mass_of(weight(value_of(s.sorted[i + 1]))) : 0;
+          if (limits.k_on) {
+            unsigned long long total;
+            block_scan<unsigned long long>(m0 + m1, s.red_mass, total);
+            target = (unsigned long long)fmax(ceil(limits.p * (double)total), 1.0);
+          }
+          const int j = bin_at(m0, m1, target);
+          if (j >= 0) cut = s.sorted[j];
+          else if (!limits.k_on && !limits.low_on && a.vocab > kCandidates) return rest;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (i + j < n && s.keys[i + j] >= cut) {
+          const double y = weight(value_of(s.keys[i + j]));
+          if (y >= limits.low) w[j] = y;
+        }
       }
     }
-    const int item = pick_item(s, n, 0.0, u, true, [&](int i) {
-      if (s.keys[i] < cut) return 0.0;
-      const double w = weight(value_of(s.keys[i]));
-      return w >= limits.low ? w : 0.0;
-    });
-    answer(index_of(s.keys[item]));
+    answer(index_of(s.keys[pick_item(w[0], w[1], 0.0, share, true, before)]));
+    return kDone;
+  }
+
+  // A wide row from its slices' histograms; false: not decided here.
+  __device__ __forceinline__ bool finish(const Wide& of) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Exp2::fill(s.table);
+    u = a.u[row] > 0.0f ? (double)a.u[row] : 0.0;
+    top = of.top;
+    high = of.top;
+    const Steps steps(top, of.least);
+    const unsigned long long* bins = l.bins + row * l.slices * kBins;
+    int whole = kBins;  // bins before it are kept whole
+    uint64_t cut = 0;
+    int n = 0;
+    if (of.kind == 1) {
+      unsigned long long x0 = 0, x1 = 0;
+      for (int j = 0; j < l.slices; ++j) {
+        x0 += bins[j * kBins + 2 * tid];
+        x1 += bins[j * kBins + 2 * tid + 1];
+      }
+      const int bin = bin_at(x0, x1, of.target);
+      if (bin < 0) return false;
+      // the bins that need a look at their values: the nucleus' last one, or those around min-p's value where
+      // that comes first
+      int last = bin;
+      whole = bin;
+      if (limits.low_on) {
+        const int low = steps.of((float)(high + log2(limits.low) / limits.scale));
+        whole = min(bin, max(low - 1, 0));
+        last = min(bin, low + 1);
+      }
+      unsigned long long above;
+      block_scan((2 * tid < whole ? x0 : 0) + (2 * tid + 1 < whole ? x1 : 0), s.red_mass, above);
+      if (tid == 0) s.n = 0;
+      __syncthreads();
+      for (int64_t unit = wave; unit < l.units; unit += kWaves) {
+        const int64_t base = unit * kUnit + lane * kValues;
+        Piece<DT> x[kPieces];
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+          for (int i = 0; i < kValues; ++i) {
+            const int b = steps.of(x[j][i]);
+            if (b >= whole && b <= last && x[j][i] >= of.least) {
+              const int at = atomicAdd(&s.n, 1);
+              if (at < kCandidates) s.sorted[at] = key_of(x[j][i], base + j * 64 * kValues + i);
+            }
+          }
+      }
+      __syncthreads();
+      n = s.n;
+      if (n > kCandidates) return false;
+      sort_keys(s.sorted, n);
+      const int i = 2 * tid;
+      const int j = bin_at(i < n ? mass_of(weight(value_of(s.sorted[i]))) : 0,
+                           i + 1 < n ? mass_of(weight(value_of(s.sorted[i + 1]))) : 0,
+                           of.target > above ? of.target - above : 1);
+      if (j >= 0) cut = s.sorted[j];
+      else if (last == bin) return false;
+    }
+    // the slices' kept masses, a wave each
+    if (wave < l.slices) {
+      unsigned long long sum = 0;
+      for (int b = lane; b < whole; b += 64) sum += bins[wave * kBins + b];
+      for (int j = lane; j < n; j += 64) {
+        const uint64_t key = s.sorted[j];
+        const double w = weight(value_of(key));
+        if (key >= cut && w >= limits.low && index_of(key) / (kUnit * l.slice_units) == wave) sum += mass_of(w);
+      }
+      sum = of_lane(lanes_scan(sum), 63);
+      if (lane == 0) s.slice[wave] = sum;
+    }
+    __syncthreads();
+    unsigned long long total = 0;
+    for (int j = 0; j < l.slices; ++j) total += s.slice[j];
+    const double target = u * ((double)total / mass_scale);
+    int slice = -1;
+    double base = 0.0;
+    unsigned long long sum = 0;
+    for (int j = 0; j < l.slices; ++j) {
+      if (s.slice[j] == 0) continue;
+      slice = j;
+      base = (double)sum / mass_scale;
+      sum += s.slice[j];
+      if ((double)sum / mass_scale > target) break;
+    }
+    if (slice < 0) return false;
+    // the units' in that slice
+    const int64_t first = (int64_t)slice * l.slice_units, last = min(first + l.slice_units, l.units);
+    for (int64_t unit = first + wave; unit < last; unit += kWaves) {
+      const int64_t at = unit * kUnit + lane * kValues;
+      Piece<DT> x[kPieces];
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) x[j].load(p, at + j * 64 * kValues, a.vocab);
+      double mass = 0.0;
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+          const double w = weight(x[j][i]);
+          const bool kept = x[j][i] > -INFINITY && key_of(x[j][i], at + j * 64 * kValues + i) >= cut && w >= limits.low;
+          mass += kept ? w : 0.0;
+        }
+      mass = of_lane(lanes_scan(mass), 63);
+      if (lane == 0) s.unit[unit - first] = mass;
+    }
+    __syncthreads();
+    const int i = 2 * tid, count = (int)(last - first);
+    double to = target;
+    double before;
+    const int unit = pick_item(i < count ? s.unit[i] : 0.0, i + 1 < count ? s.unit[i + 1] : 0.0, base, to, false, before);
+    pick_in_unit(first + unit, before, to, cut, limits.low);
     return true;
   }
 };
 
 template <int DT, int GROUP>
 __global__ __launch_bounds__(kThreads) void pick_kernel(const Sample a, const Left l, const int shift) {
-  __shared__ AnyShared s;
+  __shared__ RowShared s;
   const int64_t row = blockIdx.x;
   const Limits limits(a, row);
-  Pick<DT, GROUP> pick{a, l, limits, s.pick, row, reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride};
-  pick.mass_scale = ldexp(1.0, shift);
-  if (pick.run()) return;
+  using P = Pick<DT, GROUP>;
+  P pick{a, l, limits, s, row, reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride,
+         __hiloint2double((1023 + shift) << 20, 0)};
+  Wide left{};
+  const typename P::Found found = pick.run(left);
+  if (threadIdx.x == 0) {
+    if (found == P::kDone) left.kind = 0;
+    else if (found == P::kElse || l.slices == 0) left.kind = 3;
+    l.wide[row] = left;
+  }
+}
+
+// Masses of a slice's values in bins.
+constexpr int kSliceThreads = 512;
+
+template <int DT>
+__global__ __launch_bounds__(kSliceThreads) void slice_kernel(const Sample a, const Left l, const int shift) {
+  constexpr int kValues = Piece<DT>::kValues, kUnit = unit_values<DT>();
+  __shared__ unsigned long long mass[kBins];
+  __shared__ uint64_t table[kSteps];
+  const int64_t row = blockIdx.x / l.slices;
+  const int slice = blockIdx.x - row * l.slices;
+  const Wide of = l.wide[row];
+  if (of.kind != 1 && of.kind != 2) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < kBins; i += kSliceThreads) mass[i] = 0;
+  Exp2::fill(table);
   __syncthreads();
+  const Limits limits(a, row);
+  const Exp2 exp2_of{table};
+  const Steps steps(of.top, of.least);
+  const double high = of.top, mass_scale = __hiloint2double((1023 + shift) << 20, 0);
+  const double low = of.kind == 2 ? limits.low : 0.0;
+  const kv_elem<DT>* p = reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride;
+  const int64_t last = min((int64_t)(slice + 1) * l.slice_units, l.units);
+  for (int64_t unit = (int64_t)slice * l.slice_units + wave; unit < last; unit += kSliceThreads / 64) {
+    const int64_t base = unit * kUnit + lane * kValues;
+    Piece<DT> x[kPieces];
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+      for (int i = 0; i < kValues; ++i) {
+        if (x[j][i] >= of.least) {
+          const double w = exp2_of(((double)x[j][i] - high) * limits.scale);
+          if (w >= low)
+            atomicAdd(&mass[steps.of(x[j][i])],
+                      (unsigned long long)__double_as_longlong(w * mass_scale + 0x1p52) & ((1ull << 52) - 1));
+        }
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kSliceThreads) l.bins[(row * l.slices + slice) * kBins + i] = mass[i];
+}
+
+// What pick_kernel left.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void rest_kernel(const Sample a, const Left l, const int shift) {
+  __shared__ AnyShared s;
+  const int64_t row = blockIdx.x;
+  const Wide of = l.wide[row];
+  if (of.kind == 0) return;
+  if (of.kind < 3) {
+    const Limits limits(a, row);
+    Pick<DT, 64> pick{a, l, limits, s.row, row, reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride,
+                      __hiloint2double((1023 + shift) << 20, 0)};
+    if (pick.finish(of)) return;
+    __syncthreads();
+  }
   sample_row<DT>(a, shift, row, s.select);
 }
 
@@ -686,13 +951,20 @@ Sample part(const Sample& a, int64_t r0, int64_t n) {
   return r;
 }
 
-// Rows of a launch: 2^27 values, but a few hundred rows at least, whose workspace (an eighth of the values
-// at most) the next launch takes over.
+// Rows of a launch: 2^25 values, but some hundred rows at least, whose workspace the next launch takes over.
 int64_t most_rows(const Sample& a) {
-  return std::min(a.rows, std::max<int64_t>(256, ((int64_t)1 << 27) / std::max<int64_t>(a.vocab, 1024)));
+  return std::min(a.rows, std::max<int64_t>(256, ((int64_t)1 << 25) / std::max<int64_t>(a.vocab, 1 << 14)));
 }
 
 int unit_of(int dtype) { return dtype == kF32 ? unit_values<kF32>() : unit_values<kF16>(); }
+
+// Whether a row may keep more tokens than pick_kernel sorts, as far as the host can see.
+bool may_be_wide(const Sample& a) {
+  if (a.vocab <= kCandidates) return false;
+  if (!a.temperature && a.temperature_all == 0.0f) return false;
+  if (!a.top_k && a.top_k_all > 0 && a.top_k_all < a.vocab) return false;
+  return a.top_p || a.top_p_all < 1.0f || a.min_p || a.min_p_all > 0.0f;
+}
 
 Left layout_of(const Sample& a, void* workspace, size_t* bytes) {
   Left l{};
@@ -711,25 +983,31 @@ Left layout_of(const Sample& a, void* workspace, size_t* bytes) {
   l.unit_mass = static_cast<double*>(take(rows * l.units * 8));
   l.unit_top = static_cast<float*>(take(rows * l.units * 4));
   l.group_top = static_cast<float*>(take(rows * l.groups * 4));
+  if (may_be_wide(a)) {
+    l.slice_units = (int)((l.units + kMostSlices - 1) / kMostSlices);
+    l.slices = (int)((l.units + l.slice_units - 1) / l.slice_units);
+    l.bins = static_cast<unsigned long long*>(take(rows * l.slices * kBins * 8));
+  }
+  l.wide = static_cast<Wide*>(take(rows * sizeof(Wide)));
   *bytes = used;
   return l;
 }
 
+template <int DT, int GROUP>
+void launch_groups(const Sample& a, const Left& l, int shift, hipStream_t stream) {
+  const unsigned n = (unsigned)a.rows;
+  const int blocks = (int)((l.units + kScanThreads / 64 - 1) / (kScanThreads / 64));
+  scan_kernel<DT, GROUP><<<n * blocks, kScanThreads, 0, stream>>>(a, l, blocks);
+  pick_kernel<DT, GROUP><<<n, kThreads, 0, stream>>>(a, l, shift);
+  if (l.slices > 0) slice_kernel<DT><<<n * l.slices, kSliceThreads, 0, stream>>>(a, l, shift);
+  rest_kernel<DT><<<n, kThreads, 0, stream>>>(a, l, shift);
+}
+
 template <int DT>
 hipError_t launch_rows(const Sample& a, const Left& l, int shift, hipStream_t stream) {
-  const unsigned n = (unsigned)a.rows;
-  if (a.vocab > kMostVocab) {
-    select_kernel<DT><<<n, kThreads, 0, stream>>>(a, shift);
-    return hipGetLastError();
-  }
-  const int blocks = (int)((l.units + 3) / 4);
-  if (l.group == 16) {
-    scan_kernel<DT, 16><<<n * blocks, kScanThreads, 0, stream>>>(a, l, blocks);
-    pick_kernel<DT, 16><<<n, kThreads, 0, stream>>>(a, l, shift);
-  } else {
-    scan_kernel<DT, 64><<<n * blocks, kScanThreads, 0, stream>>>(a, l, blocks);
-    pick_kernel<DT, 64><<<n, kThreads, 0, stream>>>(a, l, shift);
-  }
+  if (a.vocab > kMostVocab) select_kernel<DT><<<(unsigned)a.rows, kThreads, 0, stream>>>(a, shift);
+  else if (l.group == 16) launch_groups<DT, 16>(a, l, shift, stream);
+  else launch_groups<DT, 64>(a, l, shift, stream);
   return hipGetLastError();
 }
 

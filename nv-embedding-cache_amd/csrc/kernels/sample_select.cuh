@@ -178,7 +178,7 @@ __device__ __forceinline__ bool select(const Row<DT>& r, SelectShared& s, float 
 
 // A row from nothing but its logits.
 template <int DT>
-__device__ void sample_row(const Sample& a, const int shift, const int64_t row, SelectShared& s) {
+__device__ __forceinline__ void sample_row(const Sample& a, const int shift, const int64_t row, SelectShared& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float t = a.temperature ? a.temperature[row] : a.temperature_all;
   const int64_t k = a.top_k ? a.top_k[row] : a.top_k_all;
