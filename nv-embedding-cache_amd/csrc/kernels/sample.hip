@@ -23,7 +23,7 @@
 //   rest_kernel    those rows: the cut's bin is gathered and sorted, the slice that u falls into read
 //                  again; and what is left (a top-k of over 2,048 or of more than there are groups,
 //                  infinities, many equals at a wide cut), with sample_row() (sample_select.cuh)
-// Vocabularies of more than 2^19 are sample_row()'s alone.  It is no function that pick_kernel calls: a
+// Vocabularies of more than 2^19 and of less than 16 are sample_row()'s alone.  It is no function that pick_kernel calls: a
 // kernel with a stack took 20 us where one without took 6.
 #include <math.h>
 
@@ -47,7 +47,7 @@ constexpr int kMostGroups = 8192;
 constexpr int kMostUnits = 512;
 constexpr int kPieces = 4;               // 16-byte pieces of a lane in a unit
 constexpr int kMostSlices = 8;           // of a wide row
-constexpr int64_t kMostVocab = 1 << 19;  // of these kernels: 8192 groups, 512 units
+constexpr int64_t kLeastVocab = 16, kMostVocab = 1 << 19;  // of these kernels: a piece; 8192 groups, 512 units
 
 // A row that pick_kernel left.
 struct Wide {
@@ -71,6 +71,7 @@ struct Left {
 // A row's limits.
 struct Limits {
   bool greedy, k_on, p_on, low_on;
+  bool plain;  // the temperature leaves everything in f32's range
   int64_t k;
   double p, low, scale;  // scale: log2(e) / T
   __device__ __forceinline__ Limits(const Sample& a, int64_t row) {
@@ -84,9 +85,10 @@ struct Limits {
     low_on = lf > 0.0f;
     p = pf;
     low = low_on ? fmin((double)lf, 1.0) : 0.0;
+    plain = t >= 1e-30f && t <= 1e30f;
     scale = greedy ? 0.0 : 1.4426950408889634 / (double)t;
   }
-  __device__ __forceinline__ bool all_mass() const { return !greedy && !k_on && (p_on || !low_on); }
+  __device__ __forceinline__ bool all_mass() const { return !greedy && plain && !k_on && (p_on || !low_on); }
 };
 
 // ---------------------------------------------------------------------------
@@ -124,52 +126,131 @@ constexpr std::array<uint64_t, kSteps> make_powers() {
 __constant__ const std::array<uint64_t, kSteps> kPowers = make_powers();
 static_assert(kSteps == 1 << 8);
 
-// 2^z for z <= 0: the table and the series up to the third power for the rest, |r| <= 1/512, whose next
-// term is (ln 2 / 512)^4 / 24 = 1.4e-13.  Less than 2^-1000, and what is no number, is 0 (parts(): 2^-1000,
-// nothing beside a sum of 1 and more).
-struct Exp2 {
+// Weights 2^((x - high) scale) for x <= high: n, the exponent in steps of 1 / 256, the table, and the series up
+// to the third power for the rest, |r| <= 1/2 of a step, whose next term is (ln 2 / 512)^4 / 24 = 1.4e-13.
+// Less than 2^-1000 is 0 (parts(): 2^-1000, nothing beside a sum of 1 and more).
+struct Weights {
   const uint64_t* table;
+  double high, scale;  // of a step
+  double least;        // x - high: what is below has no weight
+  __device__ __forceinline__ Weights(const uint64_t* table, const Limits& limits, float high)
+      : table(table), high(high), scale(limits.scale * kSteps), least(-1000.0 / limits.scale) {}
   static __device__ __forceinline__ void fill(uint64_t* t) {
     if (threadIdx.x < kSteps) t[threadIdx.x] = kPowers[threadIdx.x];
   }
-  // The power and the factor that completes it.
-  __device__ __forceinline__ void parts(double z, double& power, double& factor) const {
-    z = __builtin_fmax(z, -1000.0);
-    const double t = z + 0x1.8p44;  // a multiple of 1 / 256
+  // The power and the factor that completes it; a NaN counts as nothing.
+  __device__ __forceinline__ void parts(float x, double& power, double& factor) const {
+    constexpr double k1 = 0.6931471805599453 / kSteps, k2 = k1 * k1 / 2, k3 = k1 * k1 * k1 / 6;
+    const double d = __builtin_fmax((double)x - high, least);
+    const double t = fma(d, scale, 0x1.8p52);  // rounds to a whole number of steps
     const int n = (int)__double_as_longlong(t);
-    const double r = z - (t - 0x1.8p44);
-    factor = fma(r, fma(r, fma(r, 0.05550410866482158, 0.2402265069591007), 0.6931471805599453), 1.0);
+    const double r = fma(d, scale, 0x1.8p52 - t);
+    double y;  // the compiler would copy k2 for every use
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(r), "s"(k3), "v"(k2));
+    factor = fma(r, fma(r, y, k1), 1.0);
     const uint64_t p = table[n & (kSteps - 1)];
     power = __hiloint2double((int)(p >> 32) + (n << 12), (int)p);
   }
-  __device__ __forceinline__ double operator()(double z) const {
+  __device__ __forceinline__ double operator()(float x) const {
     double power, factor;
-    parts(z, power, factor);
-    return z >= -1000.0 ? power * factor : 0.0;
+    parts(x, power, factor);
+    return (double)x - high >= least ? power * factor : 0.0;
   }
 };
 
-// A lane's 16 bytes of a row from `first` on; what is past the row's end is minus infinity.
+// Adds weights of 16-bit logits to a sum, with what is small in 32 bits, as 64 take twice as long: the difference
+// to the maximum (exact where it is not 2^16 times x, 2^13 for f16, and its 2^-25 else), its product with the scale in
+// two parts, and the series without its 1, at most 2^-10 and 2^-24 of that off.  So a weight is 2^-34 off at most,
+// and a sum of thousands far less; the maximum's is exactly 1.
+struct Weights16 {
+  const uint64_t* table;
+  float high, scale, scale_rest, least;
+  __device__ __forceinline__ Weights16(const uint64_t* table, const Limits& limits, float high)
+      : table(table), high(high), scale((float)(limits.scale * kSteps)),
+        scale_rest((float)(limits.scale * kSteps - (double)scale)), least((float)(-1000.0 / limits.scale)) {}
+  __device__ __forceinline__ void add(float x, double& sum) const {
+    constexpr double k = 0.6931471805599453 / kSteps;
+    constexpr float k1 = (float)k, k2 = (float)(k * k / 2), k3 = (float)(k * k * k / 6);
+    const float d = __builtin_fmaxf(x - high, least);
+    const float t = fmaf(d, scale, 0x1.8p23f);  // rounds to a whole number of steps
+    const float m = t - 0x1.8p23f;
+    const int n = __float_as_int(t) - __float_as_int(0x1.8p23f);
+    const float r = fmaf(d, scale_rest, fmaf(d, scale, -m));
+    const float y = r * fmaf(r, fmaf(r, k3, k2), k1);
+    const uint64_t p = table[n & (kSteps - 1)];
+    const double power = __hiloint2double((int)(p >> 32) + (n << 12), (int)p);
+    sum = fma(power, (double)y, sum + power);
+  }
+};
+
+// A lane's 16 bytes of a row (of 16 bytes at least) from `first` on; what is past the row's end is minus infinity.
 template <int DT>
 struct Piece {
   static constexpr int kValues = 16 / value_elem_bytes(DT);
-  kv_elem<DT> v[kValues];
-  __device__ __forceinline__ void load(const kv_elem<DT>* row, int64_t first, int64_t n) {
+  u32x4 w;
+  // The row's last 16 bytes where those from `first` on would be past its end; settle() then moves them.
+  __device__ __forceinline__ void request(const kv_elem<DT>* row, int first, int n) {
     typedef u32x4 __attribute__((aligned(2))) any;  // a row may start at any element
-    if (first + kValues <= n) {
-      const u32x4 w = *reinterpret_cast<const any*>(row + first);
-      __builtin_memcpy(v, &w, 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kValues; ++i) v[i] = first + i < n ? row[first + i] : (kv_elem<DT>)-INFINITY;
-    }
+    const uint32_t offset = (uint32_t)min(first, n - kValues) * (uint32_t)sizeof(kv_elem<DT>);
+    w = *reinterpret_cast<const any*>(reinterpret_cast<const uint8_t*>(row) + offset);
   }
-  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+  __device__ __forceinline__ void settle(int first, int n) {
+    if (first + kValues <= n) return;
+    constexpr uint64_t kNone = DT == kF32 ? 0xff800000ff800000u : DT == kBF16 ? 0xff80ff80ff80ff80u : 0xfc00fc00fc00fc00u;
+    uint64_t x[2];
+    __builtin_memcpy(x, &w, 16);
+    const int bits = min(kValues, first + kValues - n) * (int)(8 * sizeof(kv_elem<DT>));
+    if (bits >= 64) {
+      x[0] = x[1];
+      x[1] = kNone;
+    }
+    if (bits == 128) x[0] = kNone;
+    if (const int b = bits & 63) {
+      x[0] = x[0] >> b | x[1] << (64 - b);
+      x[1] = x[1] >> b | kNone << (64 - b);
+    }
+    __builtin_memcpy(&w, x, 16);
+  }
+  __device__ __forceinline__ void load(const kv_elem<DT>* row, int first, int n) {
+    request(row, first, n);
+    settle(first, n);
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (DT == kF32) return __uint_as_float(w[i]);
+    if constexpr (DT == kBF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i / 2] >> (i & 1 ? 16 : 0)));
+  }
+  // The greatest value; a NaN where the instruction makes one of the NaNs among them.
+  __device__ __forceinline__ float top() const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kValues; i += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(m) : "v"((*this)[i]), "v"((*this)[i + 1]));
+    return m;
+  }
+  // The same of what is no NaN.
+  __device__ __forceinline__ float top_of_numbers() const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) m = (*this)[i] > m ? (*this)[i] : m;
+    return m;
+  }
 };
 
 template <int DT>
 constexpr int unit_values() {
   return kPieces * 64 * Piece<DT>::kValues;
+}
+
+// A wave's unit, this lane's pieces from `first` on.
+template <int DT>
+__device__ __forceinline__ void load_unit(Piece<DT> (&x)[kPieces], const kv_elem<DT>* row, int first, int n) {
+  constexpr int kStep = 64 * Piece<DT>::kValues;
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) x[j].request(row, first + j * kStep, n);
+  if (__any(first + (kPieces - 1) * kStep + Piece<DT>::kValues > n)) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) x[j].settle(first + j * kStep, n);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -312,52 +393,65 @@ struct Steps {
 // ---------------------------------------------------------------------------
 constexpr int kScanThreads = 256;
 
+// More units a wave, the next one's pieces requested as this one's are summed, took longer (256 rows of 131,072 bf16:
+// 1 unit 22.8 us, 2 23.6, 4 25.1; f32 32.6, 37.2, 36.9).
 template <int DT, int GROUP>
-__global__ __launch_bounds__(kScanThreads) void scan_kernel(const Sample a, const Left l, const int blocks) {
-  constexpr int kValues = Piece<DT>::kValues, kLanes = GROUP / kValues;
+__global__ __launch_bounds__(kScanThreads, 7) void scan_kernel(const Sample a, const Left l, const int blocks) {
+  constexpr int kValues = Piece<DT>::kValues, kLanes = GROUP / kValues, kUnit = unit_values<DT>();
   __shared__ uint64_t table[kSteps];
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, vocab = (int)a.vocab;
   const int64_t row = blockIdx.x / blocks;
-  const int64_t unit = (int64_t)(blockIdx.x - row * blocks) * (kScanThreads / 64) + (threadIdx.x >> 6);
-  const kv_elem<DT>* p = reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride;
-  const int64_t base = unit * unit_values<DT>() + lane * kValues;
+  const int unit = __builtin_amdgcn_readfirstlane((int)(blockIdx.x - row * blocks) * (kScanThreads / 64) +
+                                                  (int)(threadIdx.x >> 6));
+  const int base = unit * kUnit + lane * kValues;
   Piece<DT> x[kPieces];
-  if ((unit + 1) * unit_values<DT>() <= a.vocab) {
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, INT64_MAX);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
-  }
+  load_unit(x, reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride, base, vocab);
   const Limits limits(a, row);
-  if (limits.all_mass()) Exp2::fill(table);
+  const bool sums = limits.all_mass();
+  if (sums) Weights::fill(table);
   __syncthreads();
-  if (unit >= l.units) return;
+  if (unit >= (int)l.units) return;
+  float tops[kPieces];
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) {
+    tops[j] = x[j].top();
+    odd |= tops[j] != tops[j];
+  }
+  if (__any(odd)) {  // NaNs that a maximum of three takes over
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) tops[j] = x[j].top_of_numbers();
+  }
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
-    float m = x[j][0];
-#pragma unroll
-    for (int i = 1; i < kValues; ++i) m = fmaxf(m, x[j][i]);
-    m = lanes_max<kLanes>(fmaxf(m, -INFINITY));
-    const int64_t group = (base + j * 64 * kValues) / GROUP;
-    if (lane % kLanes == 0 && group < l.groups) l.group_top[row * l.groups + group] = m;
+    const float m = lanes_max<kLanes>(tops[j]);
+    const int group = (base + j * 64 * kValues) / GROUP;
+    if (lane % kLanes == 0 && group < (int)l.groups) l.group_top[row * l.groups + group] = m;
     top = fmaxf(top, m);
   }
-  if (!limits.all_mass()) return;
+  if (!sums) return;
   top = lanes_max<64>(top);
-  const Exp2 exp2_of{table};
-  const double high = top;
   double sum = 0.0;
   if (top > -INFINITY && top < INFINITY) {
+    const Weights weights(table, limits, top);
+    const Weights16 weights16(table, limits, top);
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j)
+    for (int j = 0; j < kPieces; ++j) {
+      // piece by piece: all values taken apart together, as for the maxima, would need too many registers
+      asm volatile("" : "+v"(x[j].w));
 #pragma unroll
       for (int i = 0; i < kValues; ++i) {
-        double power, factor;
-        exp2_of.parts(((double)x[j][i] - high) * limits.scale, power, factor);
-        sum = fma(power, factor, sum);
+        if constexpr (DT == kF32) {
+          double power, factor;
+          weights.parts(x[j][i], power, factor);
+          sum = fma(power, factor, sum);
+        } else {
+          weights16.add(x[j][i], sum);
+        }
       }
+      asm volatile("" : "+v"(sum));
+    }
     sum = of_lane(lanes_scan(sum), 63);
   }
   if (lane == 0) {
@@ -374,18 +468,12 @@ struct RowShared {
     float tops[kMostGroups];
     struct {
       uint64_t keys[kCandidates];  // in the vocabulary's order
-      union {
-        uint64_t sorted[kCandidates];  // the greatest first
-        double weights[kCandidates];   // in the vocabulary's order, 0 where one is not kept
-      };
+      uint64_t some[kCandidates];  // those around a cut
     };
   };
   union {
     uint16_t groups[kCandidates];
-    struct {
-      uint32_t count[kBins];
-      unsigned long long mass[kBins];
-    };
+    unsigned long long mass[kBins];
   };
   uint64_t table[kSteps];
   double unit[kMostUnits / kMostSlices];
@@ -393,7 +481,7 @@ struct RowShared {
   unsigned long long red_mass[kWaves];
   int red_count[kWaves];
   float red_low[kWaves], red_high[kWaves];
-  unsigned long long slice[kMostSlices];
+  unsigned long long slice[kMostSlices], slices[kMostSlices][kWaves];
   int first_item[kWaves], last_item[kWaves], bin, n;
   double first_before[kWaves], last_before[kWaves];
   unsigned long long before_mass;
@@ -416,11 +504,9 @@ struct Pick {
   const kv_elem<DT>* p;
   double mass_scale;
   float top;
-  double high, u;
+  double u;
 
-  __device__ __forceinline__ double weight(float x) const {
-    return Exp2{s.table}(((double)x - high) * limits.scale);
-  }
+  __device__ __forceinline__ double weight(float x) const { return Weights(s.table, limits, top)(x); }
   // A weight times 2^shift, rounded; the sum is below 2^52.
   __device__ __forceinline__ unsigned long long mass_of(double w) const {
     return (unsigned long long)__double_as_longlong(w * mass_scale + 0x1p52) & ((1ull << 52) - 1);
@@ -476,6 +562,83 @@ struct Pick {
     return item;
   }
 
+  // Greatest and least of the finite ones of lo and hi over the workgroup.
+  __device__ __forceinline__ void reduce_range(float& lo, float& hi) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    hi = lanes_max<64>(hi);
+    lo = -lanes_max<64>(-lo);
+    if (lane == 0) {
+      s.red_high[wave] = hi;
+      s.red_low[wave] = lo;
+    }
+    __syncthreads();
+    hi = lanes_max<16>(s.red_high[lane & 15]);
+    lo = -lanes_max<16>(-s.red_low[lane & 15]);
+  }
+
+  // The one of n keys in s.some at which the running sum, in the order, of ones or (by_mass) masses reaches the
+  // target; 0 if it never does.
+  __device__ __forceinline__ uint64_t place_of(int n, bool by_mass, unsigned long long target) const {
+    const int tid = threadIdx.x;
+    if (tid == 0) s.cut = 0;
+    if (n <= kCounted) {  // what is ahead of each, by comparing it with all: 4 to 16 threads a key
+      if (tid < n) s.mass[tid] = by_mass ? mass_of(weight(value_of(s.some[tid]))) : 1;
+      __syncthreads();
+      const int bits = n <= 64 ? 4 : n <= 128 ? 3 : 2, mine_at = tid >> bits, part = tid & ((1 << bits) - 1);
+      unsigned long long ahead = 0;
+      if (mine_at < n) {
+        const uint64_t key = s.some[mine_at];
+        for (int j = part; j < n; j += 1 << bits) ahead += s.some[j] > key ? s.mass[j] : 0;
+      }
+      ahead = group_sum(ahead, bits);
+      if (mine_at < n && part == 0 && ahead < target && ahead + s.mass[mine_at] >= target) s.cut = s.some[mine_at];
+    } else {
+      sort_keys(s.some, n);
+      const int i = 2 * tid;
+      unsigned long long m[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) m[j] = i + j >= n ? 0 : by_mass ? mass_of(weight(value_of(s.some[i + j]))) : 1;
+      const int j = bin_at(m[0], m[1], target);
+      if (tid == 0 && j >= 0) s.cut = s.some[j];
+    }
+    __syncthreads();
+    return s.cut;
+  }
+
+  // The same among the n keys in s.keys.
+  __device__ __forceinline__ uint64_t cut_of(int n, bool by_mass, unsigned long long target) const {
+    const int tid = threadIdx.x;
+    if (n <= kCounted) {
+      if (tid < n) s.some[tid] = s.keys[tid];
+      __syncthreads();
+      return place_of(n, by_mass, target);
+    }
+    // the bin that it is in, then those in the bin
+    float v[2], lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = tid + j * kThreads;
+      v[j] = i < n ? value_of(s.keys[i]) : 0.0f;
+      if (i < n) lo = fminf(lo, v[j]);
+      s.mass[i] = 0;
+    }
+    reduce_range(lo, hi);
+    const Steps steps(top, lo);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (tid + j * kThreads < n) atomicAdd(&s.mass[steps.of(v[j])], by_mass ? mass_of(weight(v[j])) : 1ull);
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    const int bin = bin_at(s.mass[2 * tid], s.mass[2 * tid + 1], target);
+    if (bin < 0) return 0;
+    const unsigned long long before = s.before_mass;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (tid + j * kThreads < n && steps.of(v[j]) == bin) s.some[atomicAdd(&s.n, 1)] = s.keys[tid + j * kThreads];
+    __syncthreads();
+    return place_of(s.n, by_mass, target - before);
+  }
+
   // The token within a unit: values from `cut` on, the least weight `low`.
   __device__ __forceinline__ void pick_in_unit(int64_t unit, double base, double target, uint64_t cut, double low) const {
     const int64_t first = unit * kUnit;
@@ -494,25 +657,12 @@ struct Pick {
     answer(first + pick_item(w[0], w[1], base, target, false, before));
   }
 
-  // Greatest and least of the finite ones of lo and hi over the workgroup.
-  __device__ __forceinline__ void reduce_range(float& lo, float& hi) const {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    hi = lanes_max<64>(hi);
-    lo = -lanes_max<64>(-lo);
-    if (lane == 0) {
-      s.red_high[wave] = hi;
-      s.red_low[wave] = lo;
-    }
-    __syncthreads();
-    hi = lanes_max<16>(s.red_high[lane & 15]);
-    lo = -lanes_max<16>(-s.red_low[lane & 15]);
-  }
-
   enum Found { kDone, kWide, kElse };
 
   __device__ __forceinline__ Found run(Wide& left) {
     const int tid = threadIdx.x;
-    Exp2::fill(s.table);
+    if (!limits.greedy && !limits.plain) return kElse;
+    Weights::fill(s.table);
     u = a.u[row] > 0.0f ? (double)a.u[row] : 0.0;
     float lo = INFINITY, hi = -INFINITY;
 
@@ -531,7 +681,6 @@ struct Pick {
       hi = fmaxf(t[0], t[1]);
       reduce_range(lo, hi);
       top = hi;
-      high = hi;
       if (top == -INFINITY) {
         answer(-1);
         return kDone;
@@ -560,7 +709,6 @@ struct Pick {
     }
     reduce_range(lo, hi);
     top = hi;
-    high = hi;
     if (top == -INFINITY) {
       answer(-1);
       return kDone;
@@ -576,30 +724,23 @@ struct Pick {
       least = top;
     } else {
       // min-p's tokens are a part of a nucleus or hold all of it, but top-p's sum after top-k is of all of top-k's
-      if (limits.low_on && !(limits.k_on && limits.p_on) && limits.scale > 0.0) {
+      if (limits.low_on && !(limits.k_on && limits.p_on)) {
         // a little below the least weight's value: what is between is left out by its weight
-        const double low = high + log2(limits.low) / limits.scale;
+        const double high = top, low = high + log2(limits.low) / limits.scale;
         least = (float)(low - 1e-6 * fabs(low) - 1e-6 * fabs(high));
       }
       target = (unsigned long long)fmax(ceil(limits.p * all * mass_scale), 1.0);
       if ((limits.k_on || limits.p_on) && a.vocab > kCandidates) {
         if (limits.k_on && limits.k > kCandidates) return kElse;
-        for (int i = tid; i < kBins; i += kThreads) {
-          s.count[i] = 0;
-          s.mass[i] = 0;
-        }
+        for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0;
         __syncthreads();
         for (int64_t g = tid; g < l.groups; g += kThreads) {
           const float t = s.tops[g];
-          if (t > -INFINITY) {
-            const int b = steps.of(t);
-            atomicAdd(&s.count[b], 1u);
-            if (!limits.k_on) atomicAdd(&s.mass[b], mass_of(weight(t)));
-          }
+          if (t > -INFINITY) atomicAdd(&s.mass[steps.of(t)], limits.k_on ? 1ull : mass_of(weight(t)));
         }
         __syncthreads();
         if (limits.k_on) {
-          limit = bin_at(s.count[2 * tid], s.count[2 * tid + 1], limits.k);
+          limit = bin_at(s.mass[2 * tid], s.mass[2 * tid + 1], limits.k);
           if (limit < 0) return kElse;
         } else {
           const int sure = bin_at(s.mass[2 * tid], s.mass[2 * tid + 1], target);
@@ -614,7 +755,7 @@ struct Pick {
       float bound = least;
       if (limits.p_on) {
         const double depth = log2((double)a.vocab / ((1.0 - limits.p) * all)) / limits.scale;
-        bound = (float)(high - fmax(depth, 0.0) * 1.0001 - 1e-6 * fabs(high));
+        bound = (float)((double)top - fmax(depth, 0.0) * 1.0001 - 1e-6 * fabs((double)top));
       }
       left = Wide{limits.p_on ? 1 : 2, top, bound, target};
     }
@@ -632,28 +773,42 @@ struct Pick {
     if (few) {
       for (; mine; mine &= mine - 1) s.groups[at++] = (uint16_t)(g0 + __builtin_ctz(mine));
       __syncthreads();
-      // their candidates, in order
-      for (int b0 = 0; b0 < groups; b0 += kThreads / kLanes) {
-        const int mine_at = b0 + tid / kLanes;
-        Piece<DT> x;
-        uint32_t yes = 0;
-        int64_t first = 0;
-        if (mine_at < groups) {
-          first = (int64_t)s.groups[mine_at] * GROUP + tid % kLanes * kValues;
-          x.load(p, first, a.vocab);
+      // their candidates, in order: four groups a lane group in a round
+      constexpr int kStep = kThreads / kLanes;
+      for (int b0 = 0; b0 < groups && few; b0 += 4 * kStep) {
+        Piece<DT> x[4];
+        uint32_t yes[4];
+        unsigned long long counts = 0;
 #pragma unroll
-          for (int i = 0; i < kValues; ++i) yes |= (uint32_t)wanted(x[i]) << i;
-        }
-        int more;
-        int to = n + block_scan((int)__popc(yes), s.red_count, more) - __popc(yes);
-        if (n + more > kCandidates) {
-          few = false;
-          break;
+        for (int j = 0; j < 4; ++j) {
+          const int mine_at = b0 + j * kStep + tid / kLanes;
+          yes[j] = 0;
+          if (mine_at < groups) x[j].load(p, s.groups[mine_at] * GROUP + tid % kLanes * kValues, (int)a.vocab);
         }
 #pragma unroll
-        for (int i = 0; i < kValues; ++i)
-          if (yes >> i & 1) s.keys[to++] = key_of(x[i], first + i);
-        n += more;
+        for (int j = 0; j < 4; ++j) {
+          const int mine_at = b0 + j * kStep + tid / kLanes;
+          if (mine_at < groups) {
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) yes[j] |= (uint32_t)wanted(x[j][i]) << i;
+          }
+          counts |= (unsigned long long)__popc(yes[j]) << (16 * j);
+        }
+        unsigned long long more;
+        const unsigned long long before = block_scan(counts, s.red_mass, more) - counts;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int count = (int)(more >> (16 * j)) & 0xffff;
+          few = few && n + count <= kCandidates;
+          if (few && yes[j]) {
+            int to = n + ((int)(before >> (16 * j)) & 0xffff);
+            const int64_t first = (int64_t)s.groups[b0 + j * kStep + tid / kLanes] * GROUP + tid % kLanes * kValues;
+#pragma unroll
+            for (int i = 0; i < kValues; ++i)
+              if (yes[j] >> i & 1) s.keys[to++] = key_of(x[j][i], first + i);
+          }
+          n += count;
+        }
       }
     }
     __syncthreads();
@@ -663,73 +818,30 @@ struct Pick {
     }
     if (!few) return rest;
 
+    uint64_t cut = 0;
     const int i = 2 * tid;
+    if (limits.k_on && n > limits.k) cut = cut_of(n, false, limits.k);
     double w[2] = {0.0, 0.0};
-    double share = u, before;
-    if (n <= kCounted) {
-      // every token's place in the order, and the mass before it, by comparing it with all: 4 to 16 threads each
-      if (tid < n) {
-        const double y = weight(value_of(s.keys[tid]));
-        s.weights[tid] = y >= limits.low ? y : 0.0;
-        s.mass[tid] = mass_of(y);
-      }
-      __syncthreads();
-      if (limits.k_on || limits.p_on) {
-        const int bits = n <= 64 ? 4 : n <= 128 ? 3 : 2, mine_at = tid >> bits;
-        uint32_t rank = 0;
-        unsigned long long ahead = 0, own = 0;
-        if (mine_at < n) {
-          const uint64_t key = s.keys[mine_at];
-          own = s.mass[mine_at];
-          for (int j = tid & ((1 << bits) - 1); j < n; j += 1 << bits) {
-            const bool first = s.keys[j] > key;
-            rank += first;
-            ahead += first ? s.mass[j] : 0;
-          }
-        }
-        rank = group_sum(rank, bits);
-        ahead = group_sum(ahead, bits);
-        bool kept = mine_at < n && (!limits.k_on || rank < limits.k);
-        if (limits.p_on) {
-          unsigned long long total;
-          block_scan<unsigned long long>(kept && (tid & ((1 << bits) - 1)) == 0 ? own : 0, s.red_mass, total);
-          if (limits.k_on) target = (unsigned long long)fmax(ceil(limits.p * (double)total), 1.0);
-          else if (total < target && !limits.low_on && a.vocab > kCandidates) return rest;  // not all of the nucleus
-          kept = kept && (ahead < target || rank == 0);
-        }
-        if (mine_at < n && !kept && (tid & ((1 << bits) - 1)) == 0) s.weights[mine_at] = 0.0;
-        __syncthreads();
-      }
-      if (i < n) w[0] = s.weights[i];
-      if (i + 1 < n) w[1] = s.weights[i + 1];
-    } else {
-      uint64_t cut = 0;
-      if (limits.k_on || limits.p_on) {
-        for (int j = tid; j < n; j += kThreads) s.sorted[j] = s.keys[j];
-        sort_keys(s.sorted, n);
-        const int kept = limits.k_on ? (int)min((int64_t)n, limits.k) : n;
-        cut = s.sorted[kept - 1];
-        if (limits.p_on) {
-          const unsigned long long m0 = i < kept ? mass_of(weight(value_of(s.sorted[i]))) : 0;
-          const unsigned long long m1 = i + 1 < kept ? mass_of(weight(value_of(s.sorted[i + 1]))) : 0;
-          if (limits.k_on) {
-            unsigned long long total;
-            block_scan<unsigned long long>(m0 + m1, s.red_mass, total);
-            target = (unsigned long long)fmax(ceil(limits.p * (double)total), 1.0);
-          }
-          const int j = bin_at(m0, m1, target);
-          if (j >= 0) cut = s.sorted[j];
-          else if (!limits.k_on && !limits.low_on && a.vocab > kCandidates) return rest;
-        }
-      }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (i + j < n && s.keys[i + j] >= cut) {
-          const double y = weight(value_of(s.keys[i + j]));
-          if (y >= limits.low) w[j] = y;
-        }
+    for (int j = 0; j < 2; ++j)
+      if (i + j < n && s.keys[i + j] >= cut) w[j] = weight(value_of(s.keys[i + j]));
+    if (limits.p_on) {
+      unsigned long long total;
+      block_scan<unsigned long long>(mass_of(w[0]) + mass_of(w[1]), s.red_mass, total);
+      if (limits.k_on) target = (unsigned long long)fmax(ceil(limits.p * (double)total), 1.0);
+      if (total >= target) {
+        cut = max(cut, cut_of(n, true, target));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (i + j < n && s.keys[i + j] < cut) w[j] = 0.0;
+      } else if (!limits.low_on && a.vocab > kCandidates) {
+        return rest;  // the candidates are not all of the nucleus
       }
     }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (w[j] < limits.low) w[j] = 0.0;
+    double share = u, before;
     answer(index_of(s.keys[pick_item(w[0], w[1], 0.0, share, true, before)]));
     return kDone;
   }
@@ -737,20 +849,26 @@ struct Pick {
   // A wide row from its slices' histograms; false: not decided here.
   __device__ __forceinline__ bool finish(const Wide& of) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Exp2::fill(s.table);
+    Weights::fill(s.table);
     u = a.u[row] > 0.0f ? (double)a.u[row] : 0.0;
     top = of.top;
-    high = of.top;
     const Steps steps(top, of.least);
     const unsigned long long* bins = l.bins + row * l.slices * kBins;
     int whole = kBins;  // bins before it are kept whole
     uint64_t cut = 0;
     int n = 0;
+    unsigned long long x[kMostSlices][2];
+#pragma unroll
+    for (int j = 0; j < kMostSlices; ++j) {
+      x[j][0] = j < l.slices ? bins[j * kBins + 2 * tid] : 0;
+      x[j][1] = j < l.slices ? bins[j * kBins + 2 * tid + 1] : 0;
+    }
     if (of.kind == 1) {
       unsigned long long x0 = 0, x1 = 0;
-      for (int j = 0; j < l.slices; ++j) {
-        x0 += bins[j * kBins + 2 * tid];
-        x1 += bins[j * kBins + 2 * tid + 1];
+#pragma unroll
+      for (int j = 0; j < kMostSlices; ++j) {
+        x0 += x[j][0];
+        x1 += x[j][1];
       }
       const int bin = bin_at(x0, x1, of.target);
       if (bin < 0) return false;
@@ -759,7 +877,7 @@ struct Pick {
       int last = bin;
       whole = bin;
       if (limits.low_on) {
-        const int low = steps.of((float)(high + log2(limits.low) / limits.scale));
+        const int low = steps.of((float)((double)top + log2(limits.low) / limits.scale));
         whole = min(bin, max(low - 1, 0));
         last = min(bin, low + 1);
       }
@@ -767,39 +885,43 @@ struct Pick {
       block_scan((2 * tid < whole ? x0 : 0) + (2 * tid + 1 < whole ? x1 : 0), s.red_mass, above);
       if (tid == 0) s.n = 0;
       __syncthreads();
-      for (int64_t unit = wave; unit < l.units; unit += kWaves) {
-        const int64_t base = unit * kUnit + lane * kValues;
-        Piece<DT> x[kPieces];
+      constexpr int kAhead = 2;  // units whose loads are under way together
+      for (int64_t unit = wave; unit < l.units; unit += kAhead * kWaves) {
+        Piece<DT> y[kAhead][kPieces];
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
+        for (int h = 0; h < kAhead; ++h) load_unit(y[h], p, (int)((unit + h * kWaves) * kUnit) + lane * kValues, (int)a.vocab);
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j)
+        for (int h = 0; h < kAhead; ++h)
 #pragma unroll
-          for (int i = 0; i < kValues; ++i) {
-            const int b = steps.of(x[j][i]);
-            if (b >= whole && b <= last && x[j][i] >= of.least) {
-              const int at = atomicAdd(&s.n, 1);
-              if (at < kCandidates) s.sorted[at] = key_of(x[j][i], base + j * 64 * kValues + i);
+          for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) {
+              const int b = steps.of(y[h][j][i]);
+              if (b >= whole && b <= last && y[h][j][i] >= of.least) {
+                const int at = atomicAdd(&s.n, 1);
+                if (at < kCandidates)
+                  s.some[at] = key_of(y[h][j][i], (unit + h * kWaves) * kUnit + (j * 64 + lane) * kValues + i);
+              }
             }
-          }
       }
       __syncthreads();
       n = s.n;
       if (n > kCandidates) return false;
-      sort_keys(s.sorted, n);
-      const int i = 2 * tid;
-      const int j = bin_at(i < n ? mass_of(weight(value_of(s.sorted[i]))) : 0,
-                           i + 1 < n ? mass_of(weight(value_of(s.sorted[i + 1]))) : 0,
-                           of.target > above ? of.target - above : 1);
-      if (j >= 0) cut = s.sorted[j];
-      else if (last == bin) return false;
+      cut = place_of(n, true, of.target > above ? of.target - above : 1);
+      if (cut == 0 && last == bin) return false;
     }
-    // the slices' kept masses, a wave each
+    // the slices' kept masses
+#pragma unroll
+    for (int j = 0; j < kMostSlices; ++j) {
+      unsigned long long sum = (2 * tid < whole ? x[j][0] : 0) + (2 * tid + 1 < whole ? x[j][1] : 0);
+      sum = lanes_scan(sum);
+      if (lane == 63) s.slices[j][wave] = sum;
+    }
+    __syncthreads();
     if (wave < l.slices) {
-      unsigned long long sum = 0;
-      for (int b = lane; b < whole; b += 64) sum += bins[wave * kBins + b];
+      unsigned long long sum = lane < kWaves ? s.slices[wave][lane] : 0;
       for (int j = lane; j < n; j += 64) {
-        const uint64_t key = s.sorted[j];
+        const uint64_t key = s.some[j];
         const double w = weight(value_of(key));
         if (key >= cut && w >= limits.low && index_of(key) / (kUnit * l.slice_units) == wave) sum += mass_of(w);
       }
@@ -822,19 +944,22 @@ struct Pick {
     }
     if (slice < 0) return false;
     // the units' in that slice
+    const Weights weights(s.table, limits, top);
+    const float cut_value = cut ? value_of(cut) : -INFINITY;
+    const int64_t cut_index = cut ? index_of(cut) : -1;
     const int64_t first = (int64_t)slice * l.slice_units, last = min(first + l.slice_units, l.units);
     for (int64_t unit = first + wave; unit < last; unit += kWaves) {
       const int64_t at = unit * kUnit + lane * kValues;
       Piece<DT> x[kPieces];
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j) x[j].load(p, at + j * 64 * kValues, a.vocab);
+      load_unit(x, p, (int)at, (int)a.vocab);
       double mass = 0.0;
 #pragma unroll
       for (int j = 0; j < kPieces; ++j)
 #pragma unroll
         for (int i = 0; i < kValues; ++i) {
-          const double w = weight(x[j][i]);
-          const bool kept = x[j][i] > -INFINITY && key_of(x[j][i], at + j * 64 * kValues + i) >= cut && w >= limits.low;
+          const float v = x[j][i];
+          const double w = weights(v);
+          const bool kept = (v > cut_value || (v == cut_value && at + j * 64 * kValues + i <= cut_index)) && w >= limits.low;
           mass += kept ? w : 0.0;
         }
       mass = of_lane(lanes_scan(mass), 63);
@@ -881,26 +1006,25 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(const Sample a, co
   if (of.kind != 1 && of.kind != 2) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int i = threadIdx.x; i < kBins; i += kSliceThreads) mass[i] = 0;
-  Exp2::fill(table);
+  Weights::fill(table);
   __syncthreads();
   const Limits limits(a, row);
-  const Exp2 exp2_of{table};
+  const Weights weights(table, limits, of.top);
   const Steps steps(of.top, of.least);
-  const double high = of.top, mass_scale = __hiloint2double((1023 + shift) << 20, 0);
+  const double mass_scale = __hiloint2double((1023 + shift) << 20, 0);
   const double low = of.kind == 2 ? limits.low : 0.0;
   const kv_elem<DT>* p = reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride;
   const int64_t last = min((int64_t)(slice + 1) * l.slice_units, l.units);
   for (int64_t unit = (int64_t)slice * l.slice_units + wave; unit < last; unit += kSliceThreads / 64) {
     const int64_t base = unit * kUnit + lane * kValues;
     Piece<DT> x[kPieces];
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) x[j].load(p, base + j * 64 * kValues, a.vocab);
+    load_unit(x, p, (int)base, (int)a.vocab);
 #pragma unroll
     for (int j = 0; j < kPieces; ++j)
 #pragma unroll
       for (int i = 0; i < kValues; ++i) {
         if (x[j][i] >= of.least) {
-          const double w = exp2_of(((double)x[j][i] - high) * limits.scale);
+          const double w = weights(x[j][i]);
           if (w >= low)
             atomicAdd(&mass[steps.of(x[j][i])],
                       (unsigned long long)__double_as_longlong(w * mass_scale + 0x1p52) & ((1ull << 52) - 1));
@@ -956,6 +1080,9 @@ int64_t most_rows(const Sample& a) {
   return std::min(a.rows, std::max<int64_t>(256, ((int64_t)1 << 25) / std::max<int64_t>(a.vocab, 1 << 14)));
 }
 
+// Whether scan_kernel and pick_kernel take the rows.
+bool in_kernels(const Sample& a) { return a.vocab >= kLeastVocab && a.vocab <= kMostVocab; }
+
 int unit_of(int dtype) { return dtype == kF32 ? unit_values<kF32>() : unit_values<kF16>(); }
 
 // Whether a row may keep more tokens than pick_kernel sorts, as far as the host can see.
@@ -1005,7 +1132,7 @@ void launch_groups(const Sample& a, const Left& l, int shift, hipStream_t stream
 
 template <int DT>
 hipError_t launch_rows(const Sample& a, const Left& l, int shift, hipStream_t stream) {
-  if (a.vocab > kMostVocab) select_kernel<DT><<<(unsigned)a.rows, kThreads, 0, stream>>>(a, shift);
+  if (!in_kernels(a)) select_kernel<DT><<<(unsigned)a.rows, kThreads, 0, stream>>>(a, shift);
   else if (l.group == 16) launch_groups<DT, 16>(a, l, shift, stream);
   else launch_groups<DT, 64>(a, l, shift, stream);
   return hipGetLastError();
@@ -1015,7 +1142,7 @@ hipError_t launch_rows(const Sample& a, const Left& l, int shift, hipStream_t st
 
 size_t sample_workspace(const Sample& a) {
   size_t bytes = 0;
-  if (a.rows > 0 && a.vocab <= kMostVocab) layout_of(a, nullptr, &bytes);
+  if (a.rows > 0 && in_kernels(a)) layout_of(a, nullptr, &bytes);
   return bytes;
 }
 
