@@ -40,6 +40,15 @@
 // workspace, and the second kernel joins them.  Weights are added by whoever knows
 // a unit's sum: the first kernel for whole units, the second, piece by piece, for
 // the others, from the scores that the first one left in the workspace.
+//
+// 4-bit pages: a wave's step is 4.3 KB (128 values), a quarter of bf16's, so the work per slot counts, and more waves
+// have to be under way: three a SIMD at 128 values.  Codes become bf16 with their scale in one instruction a pair
+// (the conversion looks at nothing but a scale's exponent, so its byte is rotated into place and no more; the product
+// that takes codes and scales as they are was 5e-5 of the largest sum off in 128 terms, too much).  The queries lie
+// in shared memory, read in every step; the addresses of codes and exponents come from one row number.  One sequence of
+// 400,001 slots, f16: 141 us with bf16's launch and two waves, 118 with output tiles two at a time, 106 with 512
+// pieces, 97 with fewer registers, three waves and 768 pieces: 4.5 TB/s.  64 of 512 to 8,192 with weights: 87 to 79 us.
+// Steps of 64 slots: 102 and 82 us.  f16 queries meet bf16 rows as two values of bf16, which hold all of their bits.
 //   Grid mode: a workgroup per piece of grid_chunk() tiles, as the tables' extent
 //   asks for.  The unit is the fast index: consecutive workgroups go round the 8
 //   XCDs, and later pieces exist for the long sequences only; with the piece as the
@@ -272,12 +281,17 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w, bool high) {
                                              : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
 }
 
-// 8 e2m1 codes, the first one lowest, times their scale: exact in bf16.
+// Two of 8 e2m1 codes, the first one lowest, times their scale: exact in bf16.
+__device__ __forceinline__ uint32_t widen_pair(uint32_t w, float scale, int pair) {
+  switch (pair) {
+    case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+    case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+    default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+  }
+}
 __device__ __forceinline__ u32x4 widen8(uint32_t w, float scale) {
-  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+  return u32x4{widen_pair(w, scale, 0), widen_pair(w, scale, 1), widen_pair(w, scale, 2), widen_pair(w, scale, 3)};
 }
 // The scale of an exponent byte; 255 is a NaN's place, and the conversions give NaN for it.
 __device__ __forceinline__ float block_scale(uint32_t e) { return __uint_as_float(e << 23); }
@@ -358,11 +372,15 @@ struct Wave {
 
   static constexpr int kVLoad = !EXACT && CT == kE4M3 ? (kVWords < 2 ? 1 : 2) : kVWords < 4 ? kVWords : 4;
 
-  u32x4 q[kQParts][kQWords / 4];
+  u32x4 q[k4 ? 1 : kQParts][k4 ? 1 : kQWords / 4];  // 4 bits: in shared memory
   u32x4 k[kTiles][kPieces];
   words<kVLoad> v[kSlots][kVWords / kVLoad];
   f32x4 k_scale[kTiles], v_scale[kTiles];  // e4m3: of this lane's slots
-  uint32_t k_block[kTiles][kPieces], v_block[kSlots];  // 4 bits: exponents, of this lane's pieces and values
+  // 4 bits: exponents, of this lane's k pieces, and of its slots' v rows: those of the lane's values, or
+  // (kRowWords dwords for four rows) of all
+  static constexpr int kRowWords = k4 && EXACT && DP <= 128 ? DP / 32 : 0;
+  uint32_t k_block[kTiles][kPieces], v_block[kSlots];
+  uint32_t v_words[kTiles][kRowWords > 0 ? kRowWords : 1];
   f32x4 acc[kValues];
   float m, l;  // m: of the query; l: of this lane's slots
 
@@ -376,23 +394,31 @@ struct Wave {
   }
 
   // Queries may start at any element: 16-byte loads of the type's alignment.
-  __device__ __forceinline__ void load_queries(const KvAttend& a, int64_t row_offset, bool there, int g) {
+  __device__ __forceinline__ void load_queries(const KvAttend& a, int64_t row_offset, bool there, int g,
+                                               u32x4 (*shared)[64]) {
     constexpr int kElem = QT == kF32 ? 4 : 2;
     typedef u32x4 __attribute__((aligned(2))) any4;
     const int dim = a.pages.dim;
+    // 4 bits: all waves have the same queries, and each brings a part of them
 #pragma unroll
     for (int w = 0; w < kQWords; w += 4) {
+      if (k4 && (w / 4) % 4 != (int)(threadIdx.x >> 6)) continue;
       const int d = q_value(w, g);
       u32x4 x = {0, 0, 0, 0};
       if (there && (EXACT || d < dim)) x = *reinterpret_cast<const any4*>(a.q.p + (row_offset + d) * kElem);
-      if constexpr (kQParts == 2) {  // 11 bits are 8 and 3
+      if constexpr (k4) {
+        u32x4 rest = {0, 0, 0, 0};
+        if constexpr (kQParts == 2) {  // 11 bits are 8 and 3
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = low_of<kF16>(x[i]), v = high_of<kF16>(x[i]);
-          const uint32_t h = pack2<kBF16>(u, v);
-          q[0][w / 4][i] = h;
-          q[1][w / 4][i] = pack2<kBF16>(u - low_of<kBF16>(h), v - high_of<kBF16>(h));
+          for (int i = 0; i < 4; ++i) {
+            const float u = low_of<kF16>(x[i]), v = high_of<kF16>(x[i]);
+            const uint32_t h = pack2<kBF16>(u, v);
+            x[i] = h;
+            rest[i] = pack2<kBF16>(u - low_of<kBF16>(h), v - high_of<kBF16>(h));
+          }
+          shared[kQWords / 4 + w / 4][threadIdx.x & 63] = rest;
         }
+        shared[w / 4][threadIdx.x & 63] = x;
       } else {
         q[0][w / 4] = x;
       }
@@ -434,6 +460,27 @@ struct Wave {
       if (EXACT || d < dim) e[i] = load_byte(blocks + d / 32);
     }
   }
+  static __device__ __forceinline__ void load_v_words(uint32_t (&w)[kRowWords > 0 ? kRowWords : 1], const uint8_t* blocks) {
+    typedef u32x4 __attribute__((aligned(1))) any4;
+    typedef words<2> __attribute__((aligned(1))) any2;
+    if constexpr (kRowWords == 4) {
+      const u32x4 x = *(const __attribute__((address_space(1))) any4*)(uintptr_t)blocks;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = x[i];
+    } else {
+      const words<2> x = *(const __attribute__((address_space(1))) any2*)(uintptr_t)blocks;
+      w[0] = x[0];
+      w[1] = x[1];
+    }
+  }
+  // The scale of a slot's values.  The conversions look at a scale's exponent alone, so the byte is rotated there
+  // and what is beside it stays.
+  __device__ __forceinline__ float v_scale_of(int slot, int c) const {
+    if constexpr (kRowWords == 0) return block_scale(v_block[slot]);
+    const uint32_t w = v_words[slot / 4][slot % 4 * kRowWords / 4];
+    const uint32_t byte = slot % 4 * kRowWords % 4 + c * kValues / 32;
+    return __uint_as_float(__builtin_amdgcn_alignbit(w, w, 8 * byte + 9));
+  }
   static __device__ __forceinline__ uint32_t load_v_block(const uint8_t* blocks, int c, int dim) {
     const int d = c * kValues;
     return load_byte(blocks + (EXACT || d < dim ? d / 32 : 0));
@@ -453,6 +500,27 @@ struct Wave {
     }
   }
 
+  // 4 bits: of all tiles of a step, each read of the queries for all.
+  __device__ __forceinline__ void scores4(f32x4 (&s)[kTiles], const u32x4 (*shared)[64]) const {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // read again in every step, and not kept in registers through the loop
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) s[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      u32x4 y[kQParts];
+#pragma unroll
+      for (int h = 0; h < kQParts; ++h) y[h] = shared[h * kSteps + i][lane];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        const int piece = i * 8 / kRun;
+        const u32x4 x = widen8(k[n][piece][i * 8 % kRun / 8], block_scale(k_block[n][piece]));
+#pragma unroll
+        for (int h = 0; h < kQParts; ++h) s[n] = mma<kBF16>(x, y[h], s[n]);
+      }
+    }
+  }
+
   __device__ __forceinline__ f32x4 scores(int tile) const {
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (QT == kF32) {
@@ -464,24 +532,20 @@ struct Wave {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         u32x4 x;
-        if constexpr (k4) {
-          const int piece = i * 8 / kRun;
-          x = widen8(k[tile][piece][i * 8 % kRun / 8], block_scale(k_block[tile][piece]));
-        } else if constexpr (CT == kE4M3) {
+        if constexpr (CT == kE4M3) {
           const uint32_t w0 = k[tile][i / 2][i % 2 * 2], w1 = k[tile][i / 2][i % 2 * 2 + 1];
           x = u32x4{widen2<QT>(w0, false), widen2<QT>(w0, true), widen2<QT>(w1, false), widen2<QT>(w1, true)};
         } else {
           x = k[tile][i];
         }
-#pragma unroll
-        for (int n = 0; n < kQParts; ++n) s = mma<k4 ? kBF16 : QT>(x, q[n][i], s);
+        s = mma<QT>(x, q[0][i], s);
       }
     }
     return s;
   }
 
   // acc += V^T P^T for the weights p of this lane's slots.
-  __device__ __forceinline__ void add_values(const float (&p)[kSlots]) {
+  __device__ __forceinline__ void add_values(const float (&p)[kSlots], int c) {
     if constexpr (QT == kF32) {
 #pragma unroll
       for (int j = 0; j < kValues; ++j)
@@ -502,14 +566,36 @@ struct Wave {
           part[n][i] = kCoded || n == 0 ? w : at_least_one(w, part[0][i]);
         }
       }
+      if constexpr (k4) {
+        // two output tiles at a time, so that few widened values are alive
+        float scale[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) scale[r] = v_scale_of(r, c);
+#pragma unroll
+        for (int j = 0; j < kValues; j += 2) {
+          uint32_t w[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) w[r] = widen_pair(v[r][j / 8 / kVLoad][j / 8 % kVLoad], scale[r], j / 2 % 4);
+          u32x4 x, y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+            y[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+          }
+#pragma unroll
+          for (int n = 0; n < kParts; ++n) {
+            acc[j] = mma<VT>(x, part[n], acc[j]);
+            acc[j + 1] = mma<VT>(y, part[n], acc[j + 1]);
+          }
+        }
+        return;
+      }
       uint32_t w[8][kValues / 2];
 #pragma unroll
       for (int r = 0; r < 8; ++r)
 #pragma unroll
         for (int i = 0; i < kValues / 2; ++i) {
-          if constexpr (k4)
-            w[r][i] = widen8(v[r][i / 4 / kVLoad][i / 4 % kVLoad], block_scale(v_block[r]))[i % 4];
-          else if constexpr (CT == kE4M3)
+          if constexpr (CT == kE4M3)
             w[r][i] = widen2<VT>(v[r][i / 2 / kVLoad][i / 2 % kVLoad], i & 1);
           else
             w[r][i] = v[r][i / kVLoad][i % kVLoad];
@@ -528,10 +614,13 @@ struct Wave {
 };
 
 // Waves of a SIMD (and workgroups of a CU) that the kernel is built for and stream mode fills.
-constexpr int waves_per_simd(int dp) { return dp == 64 ? 3 : dp == 128 ? 2 : 1; }
+constexpr int waves_per_simd(int ct, int dp) {
+  if (ct == kMXFP4) return dp == 64 ? 4 : dp == 128 ? 3 : 2;
+  return dp == 64 ? 3 : dp == 128 ? 2 : 1;
+}
 
 template <int QT, int CT, int DP, bool EXACT, bool ACC, bool GRID>
-__global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(const KvAttend a, const Plan p) {
+__global__ __launch_bounds__(256, waves_per_simd(CT, DP)) void kv_attend_kernel(const KvAttend a, const Plan p) {
   using W = Wave<QT, CT, DP, EXACT>;
   using T = kv_elem<QT>;
   constexpr int kWaves = 4, kStep = W::kStep, kValues = W::kValues;
@@ -540,7 +629,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
   __shared__ float wave_ml[kWaves][2][16];
   __shared__ float rows[kWaves][16 * kRow];
   __shared__ float all[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  __shared__ u32x4 queries[W::k4 ? W::kQParts * W::kSteps : 1][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = W::k4 ? uniform(tid >> 6) : tid >> 6, c = lane & 15, g = lane >> 4;
   const KvPages& pages = a.pages;
   const int dim = EXACT ? DP : pages.dim;
   const int row_bytes = kv_row_bytes(CT, dim), mask = pages.page - 1;
@@ -553,7 +643,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
     const int rows_here = min(16, p.group - query_tile * 16);
     const int64_t q_head = (int64_t)u.head * p.group + query_tile * 16 + c;
     const bool there = c < rows_here;
-    x.load_queries(a, u.seq * a.q.token_stride + q_head * a.q.head_stride, there, g);
+    x.load_queries(a, u.seq * a.q.token_stride + q_head * a.q.head_stride, there, g, queries);
+    if constexpr (W::k4) __syncthreads();
 #pragma unroll
     for (int j = 0; j < kValues; ++j) x.acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     x.m = -INFINITY;
@@ -583,10 +674,11 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
       return *reinterpret_cast<const f4*>(static_cast<const float*>(base) +
                                           ((int64_t)max(id, 0) * pages.heads + u.head) * pages.page + (t & mask));
     };
-    // 4 bits: the exponents of a slot's row
-    auto blocks_at = [&](const void* base, int id, int64_t t) {
-      return static_cast<const uint8_t*>(base) +
-             (((int64_t)max(id, 0) * pages.heads + u.head) * pages.page + (t & mask)) * (dim / 32);
+    // 4 bits: a row's number in the cache, for its codes and its exponents, from what all lanes have (the tile's first
+    // slot) and what is a lane's own.
+    auto row_number = [&](int id, int64_t tile_t, int in_tile) {
+      const uint32_t in_page = (uint32_t)(u.head * pages.page + ((int)tile_t & mask)) + (uint32_t)(in_tile & mask);
+      return (uint64_t)(uint32_t)max(id, 0) * (uint32_t)(pages.heads * pages.page) + in_page;
     };
     // Slots without a row read the first page's instead; their scores and values are dropped below.
     auto load_k = [&](int step) {
@@ -594,8 +686,13 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
 #pragma unroll
       for (int n = 0; n < W::kTiles; ++n) {
         const int id = __shfl(ids, (step & 15) * 4 + n * 2 + (c >> 3));
-        W::load_k(x.k[n], row_at(pages.k, id, t0 + n * 16 + c), g, dim);
-        if constexpr (W::k4) W::load_k_blocks(x.k_block[n], blocks_at(pages.k_scale, id, t0 + n * 16 + c), g, dim);
+        if constexpr (W::k4) {
+          const uint64_t row = row_number(id, t0 + n * 16, c);
+          W::load_k(x.k[n], pages.k + row * row_bytes, g, dim);
+          W::load_k_blocks(x.k_block[n], static_cast<const uint8_t*>(pages.k_scale) + row * (dim / 32), g, dim);
+        } else {
+          W::load_k(x.k[n], row_at(pages.k, id, t0 + n * 16 + c), g, dim);
+        }
         if constexpr (CT == kE4M3) {
           const int of = __shfl(ids, (step & 15) * 4 + n * 2 + (g >> 1));
           x.k_scale[n] = scale_at(pages.k_scale, of, t0 + n * 16 + g * 4);
@@ -608,14 +705,19 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
       for (int n = 0; n < W::kTiles; ++n) {
         const int id = __shfl(ids, (step & 15) * 4 + n * 2 + (g >> 1));
         const int64_t t = t0 + n * 16 + g * 4;
-        const uint8_t* row = row_at(pages.v, id, t);
+        const uint64_t number = W::k4 ? row_number(id, t0 + n * 16, g * 4) : 0;
+        const uint8_t* row = W::k4 ? pages.v + number * row_bytes : row_at(pages.v, id, t);
 #pragma unroll
         for (int r = 0; r < 4; ++r) W::load_v(x.v[n * 4 + r], row + r * row_bytes, c, dim);
         if constexpr (CT == kE4M3) x.v_scale[n] = scale_at(pages.v_scale, id, t);
         if constexpr (W::k4) {
-          const uint8_t* blocks = blocks_at(pages.v_scale, id, t);
+          const uint8_t* blocks = static_cast<const uint8_t*>(pages.v_scale) + number * (dim / 32);
+          if constexpr (W::kRowWords > 0) {
+            W::load_v_words(x.v_words[n], blocks);
+          } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x.v_block[n * 4 + r] = W::load_v_block(blocks + r * (dim / 32), c, dim);
+            for (int r = 0; r < 4; ++r) x.v_block[n * 4 + r] = W::load_v_block(blocks + r * (dim / 32), c, dim);
+          }
         }
       }
     };
@@ -629,8 +731,12 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
     auto advance = [&](int step, auto more) {
       const int64_t t0 = t_base + (int64_t)step * (kWaves * kStep);
       f32x4 s[W::kTiles];
+      if constexpr (W::k4) {
+        x.scores4(s, queries);
+      } else {
 #pragma unroll
-      for (int n = 0; n < W::kTiles; ++n) s[n] = x.scores(n);
+        for (int n = 0; n < W::kTiles; ++n) s[n] = x.scores(n);
+      }
       // the four page numbers of this step, -1 where a slot has no row
       const uint64_t absent = __ballot(ids < 0) >> ((step & 15) * 4);
       const bool full = t0 + kStep <= u.len && (absent & (kStep == 32 ? 15 : 3)) == 0;
@@ -651,7 +757,12 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
             const uint32_t keep = row ? 0xffffffffu : 0u;
             y[n * 4 + r] = row ? y[n * 4 + r] : -INFINITY;
             if constexpr (CT == kE4M3) x.v_scale[n][r] = row ? x.v_scale[n][r] : 0.0f;
-            if constexpr (W::k4) x.v_block[n * 4 + r] &= keep;
+            if constexpr (W::kRowWords > 0) {  // no NaN beside the codes, which become 0
+              const uint32_t bytes = W::kRowWords == 4 ? 0xffffffffu : 0xffffu << (16 * (r & 1));
+              x.v_words[n][r * W::kRowWords / 4] &= keep | ~bytes;
+            } else if constexpr (W::k4) {
+              x.v_block[n * 4 + r] &= keep;
+            }
 #pragma unroll
             for (int w = 0; w < W::kVWords / W::kVLoad; ++w) x.v[n * 4 + r][w] &= keep;
           }
@@ -687,20 +798,24 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
         x.l += w[i];
         if constexpr (CT == kE4M3) w[i] *= x.v_scale[i / 4][i % 4];
       }
-      x.add_values(w);
+      x.add_values(w, c);
       if constexpr (more) load_v(step + 1);
     };
     for (int step = 0; step + 1 < steps; ++step) advance(step, std::true_type());
     advance(steps - 1, std::false_type());
 
-    // the workgroup's waves: rows relative to the largest m
+    // the workgroup's waves: rows relative to the largest m.  4 bits: what only this needs is worked out here, and
+    // not held in registers through the loop above.
+    int end_tid = tid;
+    if constexpr (W::k4) asm volatile("" : "+v"(end_tid));
+    const int end_wave = W::k4 ? end_tid >> 6 : wave, end_c = W::k4 ? end_tid & 15 : c, end_g = W::k4 ? (end_tid >> 4) & 3 : g;
     const float l = query_sum(x.l);
-    if (g == 0) {
-      wave_ml[wave][0][c] = x.m;
-      wave_ml[wave][1][c] = l;
+    if (end_g == 0) {
+      wave_ml[end_wave][0][end_c] = x.m;
+      wave_ml[end_wave][1][end_c] = l;
     }
     const bool whole = u.first == 0 && u.last == u.tiles;
-    const int q = tid >> 4, r = tid & 15;  // a query, and the output rows r of the tiles
+    const int q = end_tid >> 4, r = end_tid & 15;  // a query, and the output rows r of the tiles
     const int64_t out_head = (int64_t)u.head * p.group + query_tile * 16 + q;
     const int64_t at = (int64_t)slot * p.query_tiles + query_tile;
 #pragma unroll
@@ -710,7 +825,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP)) void kv_attend_kernel(cons
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < kPass; ++j) rows[wave][c * kRow + (4 * g + i) * kPass + j] = x.acc[pass * kPass + j][i];
+          for (int j = 0; j < kPass; ++j) rows[end_wave][end_c * kRow + (4 * end_g + i) * kPass + j] = x.acc[pass * kPass + j][i];
       }
       __syncthreads();
       if (q < rows_here) {
@@ -960,7 +1075,7 @@ struct Layout {
 //   Whole units, one launch, up to 4 tiles (one piece 12.2 us, 32 pieces and a join 10.3 us for one
 //   sequence of 4,096 slots, but 34.9 against 43.4 us for 256 of 32 to 512), and up to 16 where
 //   there are units for all CUs (64 sequences of 125 to 2,000 slots: whole 33.9, pieces of 8 42.3).
-//   One sequence: 256 pieces, one a CU, are enough (200,001 slots: 144 us, stream 155, pieces of 16
+//   One sequence: 256 pieces, one a CU, are enough (768 of 4-bit pages; 200,001 slots: 144 us, stream 155, pieces of 16
 //   tiles 165; 16,384: 17.7, stream 23.6, 1 tile 22.0). Its tiles are shared by these pieces as its
 //   length asks for, which only the kernels know: its table may be far longer.
 //   Several may be much shorter than the longest: smaller pieces (7 of 33 to 30,011 slots, 2 key
@@ -969,11 +1084,11 @@ struct Layout {
 //   An empty workgroup costs 1.2 ns, so tables far longer than the sequences go to stream mode
 //   (64 sequences of up to 2,000 slots in tables of 131,072: stream 41 us, pieces of 12 tiles 91;
 //   in tables of 32,768: 42 and 44).
-int64_t grid_chunk(int64_t seqs, int64_t units, int64_t tiles, int tile) {
+int64_t grid_chunk(int64_t seqs, int64_t units, int64_t tiles, int tile, int ct) {
   const int64_t all = units * tiles, most = tile < 128 ? 8 : 12;
   int64_t chunk = std::min(most, (all + 1023) / 1024);
   if (tiles <= 4 || (tiles <= 16 && units >= 256)) chunk = tiles;
-  else if (seqs == 1) chunk = (all + 255) / 256;
+  else if (seqs == 1) chunk = ct == kMXFP4 ? (all + 767) / 768 : (all + 255) / 256;
   const int64_t pieces = (tiles + chunk - 1) / chunk;
   return pieces == 1 || units * pieces <= 8192 ? chunk : 0;
 }
@@ -990,12 +1105,12 @@ Layout layout_of(const KvAttend& a, void* workspace) {
   const int64_t units = a.seqs * a.pages.heads;
   r.units = (unsigned)units;
   const int dp = padded_dim(a.pages.dim);
-  const int64_t chunk = grid_chunk(a.seqs, units, tiles, p.tile);
+  const int64_t chunk = grid_chunk(a.seqs, units, tiles, p.tile, a.pages.dtype);
   r.grid = chunk > 0;
   p.chunk = a.seqs == 1 ? 0 : (int)chunk;
   p.pieces = r.grid ? (int)((tiles + chunk - 1) / chunk) : 0;
   // what the 256 CUs hold at once
-  p.workgroups = (int)std::min<int64_t>(256 * waves_per_simd(dp), units * tiles);
+  p.workgroups = (int)std::min<int64_t>(256 * waves_per_simd(a.pages.dtype, dp), units * tiles);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   auto take = [&](size_t n) {
     void* x = at + r.bytes;
