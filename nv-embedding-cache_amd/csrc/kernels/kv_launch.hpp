@@ -54,7 +54,7 @@ struct KvAppend {
   int32_t ends[4];  // the first pair past each axis
   const uint8_t* q_norm;  // [dim] of dtype, or null: no norm
   const uint8_t* k_norm;
-  double eps;
+  double eps, inverse_dim;
 };
 
 struct KvAttend {

@@ -213,6 +213,7 @@ void kv_append_norm_run(const nve_amd_kv_pages_t* pages, const nve_amd_kv_append
   a.q_norm = static_cast<const uint8_t*>(norm->q_weight);
   a.k_norm = static_cast<const uint8_t*>(norm->k_weight);
   a.eps = norm->eps;
+  a.inverse_dim = 1.0 / a.pages.dim;
   NVE_HIP(launch_kv_append(a, s));
 }
 
