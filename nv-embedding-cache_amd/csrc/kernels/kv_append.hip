@@ -9,8 +9,7 @@
 // behind them have 16 unrotated values.  A workgroup has whole tokens: it brings
 // their cosines and sines into shared memory once for all their heads, while the
 // first rows' loads are under way.
-// Several tokens a workgroup once there are 2,048 workgroups: 9,000 tokens into e4m3
-// 51 -> 42 us.  Measured: 16,001 f16 tokens of 32 query and 8 key heads of 128 values
+// Several tokens a workgroup: 9,000 tokens into e4m3 51 -> 42 us.  Measured: 16,001 f16 tokens of 32 query and 8 key heads of 128 values
 // 83 to 92 us (4.4 to 4.8 TB/s; a large copy 4.7); 9,000 bf16 tokens of 96 values
 // into e4m3 42 to 44 us (3.6 TB/s; 6 of 8 lanes a row work); a step of 64
 // tokens 4.8 us, the chain position, cosine, shared memory, store.
@@ -449,7 +448,7 @@ __global__ __launch_bounds__(64 * kRowsPerBlock) void kv_append_any_kernel(const
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-constexpr int64_t kEnough = 2048;  // workgroups
+constexpr int64_t kEnough = 640;  // workgroups
 constexpr int64_t kMostGroups = 0xffffffffu / kThreads;  // a launch has fewer than 2^32 threads
 static_assert(kThreads == 64 * kRowsPerBlock);
 
@@ -490,10 +489,16 @@ hipError_t launch(const KvAppend& a, hipStream_t stream) {
     const int need = (a.pages.dim + 15) / 16;
     while ((1 << p.lane_bits) < need) ++p.lane_bits;
     p.lanes = 1 << p.lane_bits;
-    // whole tokens: enough to fill the workgroup's threads, and more once there are workgroups for every CU
-    const int64_t fill = std::max(1, kThreads / (rows * p.lanes));
-    p.tokens = (int)std::max(fill, std::min<int64_t>(8 * fill, a.tokens / kEnough));
-    if (a.rot > 0) p.tokens = std::min(p.tokens, kMaxTable / a.rot);
+    // Whole tokens: enough to fill the workgroup's threads, and more, while there are workgroups for every CU, where
+    // their rows leave fewer threads idle in the last turn (12,001 tokens of 48 rows of 8 lanes: 1 token 77.5 us, 2
+    // 63.5, 5 67.3; 4,801 of 36 rows of 4 lanes, 64 f32 values: 1 26.2, 2 26.9, 5 24.5, 7 23.8).
+    const int64_t each = (int64_t)rows * p.lanes, fill = std::max<int64_t>(1, kThreads / each);
+    int64_t most_tokens = std::max(fill, std::min(8 * fill, a.tokens / kEnough));
+    if (a.rot > 0) most_tokens = std::min<int64_t>(most_tokens, kMaxTable / a.rot);
+    auto busy = [&](int64_t tokens) { return (double)(tokens * each) / ((tokens * each + kThreads - 1) / kThreads * kThreads); };
+    p.tokens = (int)std::min(fill, most_tokens);
+    for (int64_t t = p.tokens + 1; t <= most_tokens; ++t)
+      if (busy(t) > busy(p.tokens) + 0.03) p.tokens = (int)t;
     most = kMostGroups * p.tokens;
   } else {
     most = kMostGroups * kRowsPerBlock / rows;
