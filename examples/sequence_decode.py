@@ -2,11 +2,13 @@
 
 A small sequence model over the lookup layers: item embeddings from a table in
 HBM (NVEmbedding, GPULayer), a few attention blocks whose keys and values live
-in KVCache pages, and one new item per user and step.  Every user's cache holds
-at most about `budget` items: once it is a page over, the items that have
-received the least attention are evicted, except the first few and the latest.
+in KVCache pages, and one new item per user and step, the best one or one drawn
+from the likely ones.  Every user's cache holds at most about `budget` items: once
+it is a page over, the items that have received the least attention are evicted,
+except the first few and the latest.
 
   python examples/sequence_decode.py --users 16 --steps 64
+  python examples/sequence_decode.py --users 16 --steps 64 --mxfp4 --norms --temperature 0.8 --top-p 0.9
 """
 import argparse
 import os
@@ -23,6 +25,7 @@ if PKG not in sys.path:
 
 from pynve.torch.nve_kv import KVCache  # noqa: E402
 from pynve.torch.nve_layers import LayerType, NVEmbedding  # noqa: E402
+from pynve.torch.nve_sample import sample_tokens  # noqa: E402
 
 
 class SequenceDecoder:
@@ -30,7 +33,7 @@ class SequenceDecoder:
     `kv_heads` key heads over item rows of `width` values."""
 
     def __init__(self, items, users, width=256, layers=2, q_heads=8, kv_heads=2, budget=256, sinks=4, recent=32,
-                 page=16, longest=4096, dtype=torch.float16, cache_dtype=None, seed=0):
+                 page=16, longest=4096, dtype=torch.float16, cache_dtype=None, norms=False, seed=0):
         g = torch.Generator(device="cuda")
         g.manual_seed(seed)
         dim = width // q_heads
@@ -38,7 +41,10 @@ class SequenceDecoder:
         self.emb = NVEmbedding(items, width, dtype, LayerType.GPULayer, optimize_for_training=False)
         self.emb.weight.data.copy_(torch.randn((items, width), device="cuda", generator=g))
         self.blocks = [{"qkv": draw(width, (q_heads + 2 * kv_heads) * dim), "out": draw(q_heads * dim, width),
-                        "up": draw(width, 2 * width), "down": draw(2 * width, width)} for _ in range(layers)]
+                        "up": draw(width, 2 * width), "down": draw(2 * width, width),
+                        # the weights of the query and key heads' norms
+                        **({n: torch.ones(dim, device="cuda", dtype=dtype) for n in ("q_norm", "k_norm")} if norms else {})}
+                       for _ in range(layers)]
         self.q_heads, self.kv_heads, self.dim, self.dtype = q_heads, kv_heads, dim, dtype
         self.budget, self.sinks, self.recent, self.page = budget, sinks, recent, page
         # a sequence grows to a page over the budget before it is cut
@@ -63,7 +69,8 @@ class SequenceDecoder:
         for w, cache in zip(self.blocks, self.caches):
             qkv = F.layer_norm(x, x.shape[1:]) @ w["qkv"]
             q, k, v = qkv.view(len(items), -1, self.dim).split([self.q_heads, self.kv_heads, self.kv_heads], 1)
-            q = cache.append(k, v, slots, q=q, positions=at, cos_sin=self.cos_sin)
+            q = cache.append(k, v, slots, q=q, positions=at, cos_sin=self.cos_sin, q_norm=w.get("q_norm"),
+                             k_norm=w.get("k_norm"))
             x = x + cache.attend(q, self.tables, self.lengths).flatten(1) @ w["out"]
             x = x + F.gelu(F.layer_norm(x, x.shape[1:]) @ w["up"]) @ w["down"]
         self.length += 1
@@ -76,9 +83,11 @@ class SequenceDecoder:
         return x
 
     @torch.no_grad()
-    def next_items(self, hidden, candidates):
-        """The best of `candidates` (int64) for every user."""
-        return candidates[(hidden @ self.emb(candidates).t()).argmax(1)]
+    def next_items(self, hidden, candidates, u=None, **limits):
+        """The best of `candidates` (int64) for every user, or, with random numbers `u` (float32 [users]), one drawn
+        within sample_tokens' limits."""
+        scores = hidden @ self.emb(candidates).t()
+        return candidates[scores.argmax(1) if u is None else sample_tokens(scores, u, **limits)]
 
 
 def main(argv=None):
@@ -88,16 +97,24 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=400)
     ap.add_argument("--budget", type=int, default=256)
     ap.add_argument("--e4m3", action="store_true", help="keep keys and values in 8 bits")
+    ap.add_argument("--mxfp4", action="store_true", help="keep keys and values in 4 bits")
+    ap.add_argument("--norms", action="store_true", help="norm the query and key heads")
+    ap.add_argument("--temperature", type=float, default=0.0, help="draw items; 0 takes the best")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     a = ap.parse_args(argv)
-    model = SequenceDecoder(a.items, a.users, budget=a.budget, longest=a.steps + 1,
-                            cache_dtype=torch.float8_e4m3fn if a.e4m3 else None)
+    model = SequenceDecoder(a.items, a.users, budget=a.budget, longest=a.steps + 1, norms=a.norms,
+                            cache_dtype=torch.float4_e2m1fn_x2 if a.mxfp4 else torch.float8_e4m3fn if a.e4m3 else None)
+    limits = {"temperature": a.temperature, "top_k": a.top_k, "top_p": a.top_p, "min_p": a.min_p}
     candidates = torch.arange(0, a.items, max(1, a.items // 1000), device="cuda")
     items = torch.randint(0, a.items, (a.users,), device="cuda")
     model.step(items)
     torch.cuda.synchronize()
     start = time.perf_counter()
     for _ in range(a.steps - 1):
-        items = model.next_items(model.step(items), candidates)
+        u = torch.rand(a.users, device="cuda") if a.temperature > 0 else None
+        items = model.next_items(model.step(items), candidates, u, **(limits if u is not None else {}))
     torch.cuda.synchronize()
     spent = (time.perf_counter() - start) / max(1, a.steps - 1)
     print(f"{a.users} users, {a.steps} steps: {spent * 1e6:.0f} us a step, {model.length} of {model.seen} items kept, "
