@@ -23,12 +23,20 @@
 //   rest_kernel    those rows: the cut's bin is gathered and sorted, the slice that u falls into read
 //                  again; and what is left (a top-k of over 2,048 or of more than there are groups,
 //                  infinities, many equals at a wide cut), with sample_row() (sample_select.cuh)
-// Vocabularies of more than 2^19 and of less than 16 are sample_row()'s alone.  It is no function that pick_kernel calls: a
-// kernel with a stack took 20 us where one without took 6.
+// Vocabularies of more than 2^19 and of less than 16 are sample_row()'s alone.  sample_row() is either all of
+// what a kernel does or inlined: as a function that pick_kernel called it gave that kernel a stack, with which a
+// launch took 20 us and without which it took 6.  Where no row can be wide and the rows are no more than the
+// CUs, pick_kernel has it inlined and rest_kernel is not launched (one row of 128,256: 15.5 to 14.2 us).
+//
+// Measured, in us (bytes at the 4.8 TB/s of a large copy): 256 rows of 131,072 bf16 without limits 26 (14), of
+// which the scan 23: 8 instructions a value and not the bytes bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
+// rows, 63 (7): scan 11, pick 13, slices 11, rest 29, launches behind each other; one row, top-k 50, 14.2, two
+// launches.
 #include <math.h>
 
 #include <algorithm>
 #include <array>
+#include <type_traits>
 
 #include "../dtypes.hpp"
 #include "kv_common.cuh"
@@ -490,6 +498,9 @@ struct RowShared {
 
 union AnyShared {
   SelectShared select;
+  RowShared row;
+};
+struct RowSharedAlone {
   RowShared row;
 };
 
@@ -978,17 +989,22 @@ struct Pick {
   }
 };
 
-template <int DT, int GROUP>
+// ALONE: nothing is left for rest_kernel, which is not launched.
+template <int DT, int GROUP, bool ALONE>
 __global__ __launch_bounds__(kThreads) void pick_kernel(const Sample a, const Left l, const int shift) {
-  __shared__ RowShared s;
+  __shared__ std::conditional_t<ALONE, AnyShared, RowSharedAlone> s;
   const int64_t row = blockIdx.x;
   const Limits limits(a, row);
   using P = Pick<DT, GROUP>;
-  P pick{a, l, limits, s, row, reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride,
+  P pick{a, l, limits, s.row, row, reinterpret_cast<const kv_elem<DT>*>(a.logits) + row * a.row_stride,
          __hiloint2double((1023 + shift) << 20, 0)};
   Wide left{};
   const typename P::Found found = pick.run(left);
-  if (threadIdx.x == 0) {
+  if constexpr (ALONE) {
+    if (found == P::kDone) return;
+    __syncthreads();
+    sample_row<DT>(a, shift, row, s.select);
+  } else if (threadIdx.x == 0) {
     if (found == P::kDone) left.kind = 0;
     else if (found == P::kElse || l.slices == 0) left.kind = 3;
     l.wide[row] = left;
@@ -1128,7 +1144,12 @@ void launch_groups(const Sample& a, const Left& l, int shift, hipStream_t stream
   const unsigned n = (unsigned)a.rows;
   const int blocks = (int)((l.units + kScanThreads / 64 - 1) / (kScanThreads / 64));
   scan_kernel<DT, GROUP><<<n * blocks, kScanThreads, 0, stream>>>(a, l, blocks);
-  pick_kernel<DT, GROUP><<<n, kThreads, 0, stream>>>(a, l, shift);
+  // sample_row()'s registers leave one workgroup a CU; a launch without rows to do takes 1.5 us and more
+  if (l.slices == 0 && a.rows <= 256) {
+    pick_kernel<DT, GROUP, true><<<n, kThreads, 0, stream>>>(a, l, shift);
+    return;
+  }
+  pick_kernel<DT, GROUP, false><<<n, kThreads, 0, stream>>>(a, l, shift);
   if (l.slices > 0) slice_kernel<DT><<<n * l.slices, kSliceThreads, 0, stream>>>(a, l, shift);
   rest_kernel<DT><<<n, kThreads, 0, stream>>>(a, l, shift);
 }
