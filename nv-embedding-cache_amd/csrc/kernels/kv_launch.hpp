@@ -13,9 +13,8 @@
 
 namespace nve_amd {
 
-// Bytes of a head's row, and of its scales.
+// Bytes of a head's row.
 inline constexpr int kv_row_bytes(int dtype, int dim) { return dtype == kMXFP4 ? dim / 2 : dim * value_elem_bytes(dtype); }
-inline constexpr int kv_scale_bytes(int dtype, int dim) { return dtype == kMXFP4 ? dim / 32 : dtype == kE4M3 ? 4 : 0; }
 
 // The pages: k and v [num_pages, heads, page, dim] of dtype, the rest [num_pages, heads, page]
 // (kMXFP4: the scales are [num_pages, heads, page, dim / 32] bytes).

@@ -216,6 +216,23 @@ def test_strides_and_no_pages():
     assert (out == 0).all() and torch.isneginf(lse).all()
 
 
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_scales_at_any_byte(dim):
+    from pynve.torch import nve_kv
+
+    s = setup("f16", [300, 50], 4, 2, dim, 16, seed=8)
+    want = call(s, 0.1)
+    k, v, scales = pages(s)
+    for n in ("k_scale", "v_scale"):
+        x = scales[n].view(torch.uint8)
+        apart = torch.zeros(x.numel() + 3, dtype=torch.uint8, device="cuda")[3:].view(x.shape)
+        scales[n] = apart.copy_(x).view(torch.float8_e8m0fnu)
+        assert scales[n].data_ptr() % 4 == 3
+    w = cuda(s["weights"])
+    out = nve_kv.kv_attend(cuda(s["q"]), k, v, cuda(s["table"]), cuda(s["lengths"]), scale=0.1, weights=w, **scales)
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(w.cpu(), want[2])
+
+
 def test_max_length_bounds_the_lengths():
     s = setup("f16", [500, 700], 4, 2, 128, 16, seed=7)
     got = call(s, 0.1, max_length=400)

@@ -64,6 +64,23 @@ def test_vocabularies(dtype, vocab):
         check(x, rng.random(n), **limits)
 
 
+@pytest.mark.parametrize("vocab", [524287, 524288, 524289, 1000003])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_the_largest_vocabularies(dtype, vocab):
+    rng = np.random.default_rng(vocab)
+    x = logits_of(rng, 2, vocab, dtype=dtype)
+    for limits in ({}, {"top_k": 20, "top_p": 0.9}, {"top_p": 0.8}, {"min_p": 0.1}, {"temperature": 0.0}):
+        check(x, rng.random(2), **limits)
+
+
+@pytest.mark.parametrize("limits", [{}, {"top_k": 9}, {"top_p": 0.9}, {"top_p": 0.99, "min_p": 0.001}])
+@pytest.mark.parametrize("rows, vocab", [(2049, 2500), (4100, 40), (300, 140000)])
+def test_more_rows_than_a_launch(rows, vocab, limits):
+    """Past 2,048 rows, or 256 of a large vocabulary, the workspace is used again."""
+    rng = np.random.default_rng(rows)
+    check(logits_of(rng, rows, vocab, spread=0.5 if rows % 100 else 2.0, dtype="bf16"), rng.random(rows), **limits)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 7, 64, 300, 1025])
 def test_every_row_has_limits_of_its_own(rows):
     rng = np.random.default_rng(rows)
