@@ -1,20 +1,21 @@
-// kv_append.hip -- new tokens enter the paged key-value cache: rotary positions
-// on queries and keys, keys and values written to their slots.
+// kv_append.hip -- new tokens enter the paged key-value cache: norms of query and key
+// heads, rotary positions on them, keys and values written to their slots.
 //
-// Every value is read and written once, with 3 flops a rotated value: bound by
-// the bytes.  kv_append_kernel: a head row is a group of lanes (a power of two),
-// 16 values a lane.  A lane that rotates has 8 pairs, both values of each, so
-// that nothing crosses lanes but an e4m3 row's largest magnitude: values 8 j ..
-// and rot / 2 + 8 j .. of the row, or (pairs of neighbours) 16 j ..; the lanes
+// Every value is read and written once, with 3 flops a rotated value and 3 more under a
+// norm: bound by the bytes.  kv_append_kernel: a head row is a group of lanes (a power of
+// two), 16 values a lane.  A lane that rotates has 8 pairs, both values of each, so
+// that nothing crosses lanes but a norm's sum and a scaled row's largest magnitudes: values
+// 8 j .. and rot / 2 + 8 j .. of the row, or (pairs of neighbours) 16 j ..; the lanes
 // behind them have 16 unrotated values.  A workgroup has whole tokens: it brings
 // their cosines and sines into shared memory once for all their heads, while the
 // first rows' loads are under way.
-// Several tokens a workgroup: 9,000 tokens into e4m3 51 -> 42 us.  Measured: 16,001 f16 tokens of 32 query and 8 key heads of 128 values
-// 83 to 92 us (4.4 to 4.8 TB/s; a large copy 4.7); 9,000 bf16 tokens of 96 values
-// into e4m3 42 to 44 us (3.6 TB/s; 6 of 8 lanes a row work); a step of 64
-// tokens 4.8 us, the chain position, cosine, shared memory, store.
+// Measured: 16,001 f16 tokens of 32 query and 8 key heads of 128 values 83 us (4.8 TB/s; a
+// large copy 4.7 to 5.0); 12,001 of them with norms 63 us (4.8 TB/s); 9,000 bf16 tokens of 96 values
+// into e4m3 40 us (3.9 TB/s; 6 of 8 lanes a row work), of 128 values with norms into 4 bits 43 us
+// (4.5 TB/s); a step of 64 tokens 4.8 us, with norms 5.7: the chain position, cosine, shared memory, store.
 // kv_append_any_kernel, for rows that start off 16 bytes and for rotated widths
-// that are no multiple of 16: one value of a row per lane and step (409 us for the
+// that are no multiple of 16 (4-bit pages, pairs of halves: of 64, so that 32 values of a scale
+// are in neighbouring lanes): one value of a row per lane and step (409 us for the
 // 16,001 tokens above).
 #include <algorithm>
 
