@@ -7,8 +7,8 @@
 // at which the kept weights' running sum, in the vocabulary's order, exceeds u times their total.
 //
 // Weights are 64-bit: a token's probability may be 1e-6, and a sum in 32 bits would give some
-// tokens' share of the random numbers to their neighbours.  A vector instruction in 64 bits takes as
-// long here as one in 32.  Sums that pick a cut are integers (weights times 2^shift), so that the order
+// tokens' share of the random numbers to their neighbours.  A vector instruction in 64 bits takes
+// twice as long here as one in 32.  Sums that pick a cut are integers (weights times 2^shift), so that the order
 // of the LDS additions changes nothing.
 //
 // Bound: the logits' bytes, read once.
@@ -29,7 +29,7 @@
 // CUs, pick_kernel has it inlined and rest_kernel is not launched (one row of 128,256: 15.5 to 14.2 us).
 //
 // Measured, in us (bytes at the 4.8 TB/s of a large copy): 256 rows of 131,072 bf16 without limits 26 (14), of
-// which the scan 23: 8 instructions a value and not the bytes bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
+// which the scan 23: some 17 vector instructions a value, 3 of them in 64 bits, bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
 // rows, 63 (7): scan 11, pick 13, slices 11, rest 29, launches behind each other; one row, top-k 50, 14.2, two
 // launches.
 #include <math.h>
