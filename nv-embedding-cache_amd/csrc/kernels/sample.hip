@@ -26,7 +26,7 @@
 // Vocabularies of more than 2^19 and of less than 16 are sample_row()'s alone.  sample_row() is either all of
 // what a kernel does or inlined: as a function that pick_kernel called it gave that kernel a stack, with which a
 // launch took 20 us and without which it took 6.  Where no row can be wide and the rows are no more than the
-// CUs, pick_kernel has it inlined and rest_kernel is not launched (one row of 128,256: 15.5 to 14.2 us).
+// CUs, pick_kernel has it inlined and rest_kernel is not launched (one row of 50,021: 15.5 to 14.2 us).
 //
 // Measured, in us (bytes at the 4.8 TB/s of a large copy): 256 rows of 131,072 bf16 without limits 26 (14), of
 // which the scan 23: some 17 vector instructions a value, 3 of them in 64 bits, bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
