@@ -21,7 +21,7 @@
 //   slice_kernel   up to 8 workgroups for each row that pick_kernel found too wide (a flat nucleus, a low
 //                  min-p): histograms of mass.  Launched where the limits allow such rows
 //   rest_kernel    those rows: the cut's bin is gathered and sorted, the slice that u falls into read
-//                  again; and what is left (a top-k of over 2,048 or of more than there are groups,
+//                  again; and what is left (a top-k of nearly 2,048 and more, or of more than there are groups,
 //                  infinities, many equals at a wide cut), with sample_row() (sample_select.cuh)
 // Vocabularies of more than 2^19 and of less than 16 are sample_row()'s alone.  sample_row() is either all of
 // what a kernel does or inlined: as a function that pick_kernel called it gave that kernel a stack, with which a
@@ -789,40 +789,63 @@ struct Pick {
       __syncthreads();
       // their candidates, in order: four groups a lane group in a round
       constexpr int kStep = kThreads / kLanes;
-      for (int b0 = 0; b0 < groups && few; b0 += 4 * kStep) {
-        Piece<DT> x[4];
-        uint32_t yes[4];
-        unsigned long long counts = 0;
+      for (bool again = limits.k_on;; again = false) {
+        for (int b0 = 0; b0 < groups && few; b0 += 4 * kStep) {
+          Piece<DT> x[4];
+          uint32_t yes[4];
+          unsigned long long counts = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int mine_at = b0 + j * kStep + tid / kLanes;
-          yes[j] = 0;
-          if (mine_at < groups) x[j].load(p, s.groups[mine_at] * GROUP + tid % kLanes * kValues, (int)a.vocab);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int mine_at = b0 + j * kStep + tid / kLanes;
-          if (mine_at < groups) {
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) yes[j] |= (uint32_t)wanted(x[j][i]) << i;
+          for (int j = 0; j < 4; ++j) {
+            const int mine_at = b0 + j * kStep + tid / kLanes;
+            yes[j] = 0;
+            if (mine_at < groups) x[j].load(p, s.groups[mine_at] * GROUP + tid % kLanes * kValues, (int)a.vocab);
           }
-          counts |= (unsigned long long)__popc(yes[j]) << (16 * j);
-        }
-        unsigned long long more;
-        const unsigned long long before = block_scan(counts, s.red_mass, more) - counts;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int count = (int)(more >> (16 * j)) & 0xffff;
-          few = few && n + count <= kCandidates;
-          if (few && yes[j]) {
-            int to = n + ((int)(before >> (16 * j)) & 0xffff);
-            const int64_t first = (int64_t)s.groups[b0 + j * kStep + tid / kLanes] * GROUP + tid % kLanes * kValues;
+          for (int j = 0; j < 4; ++j) {
+            const int mine_at = b0 + j * kStep + tid / kLanes;
+            if (mine_at < groups) {
 #pragma unroll
-            for (int i = 0; i < kValues; ++i)
-              if (yes[j] >> i & 1) s.keys[to++] = key_of(x[j][i], first + i);
+              for (int i = 0; i < kValues; ++i) yes[j] |= (uint32_t)wanted(x[j][i]) << i;
+            }
+            counts |= (unsigned long long)__popc(yes[j]) << (16 * j);
           }
-          n += count;
+          unsigned long long more;
+          const unsigned long long before = block_scan(counts, s.red_mass, more) - counts;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int count = (int)(more >> (16 * j)) & 0xffff;
+            few = few && n + count <= kCandidates;
+            if (few && yes[j]) {
+              int to = n + ((int)(before >> (16 * j)) & 0xffff);
+              const int64_t first = (int64_t)s.groups[b0 + j * kStep + tid / kLanes] * GROUP + tid % kLanes * kValues;
+#pragma unroll
+              for (int i = 0; i < kValues; ++i)
+                if (yes[j] >> i & 1) s.keys[to++] = key_of(x[j][i], first + i);
+            }
+            n += count;
+          }
         }
+        if (few || !again) break;
+        // Too many for top-k: groups above the k-th maximum hold more tokens above it.  The step that the k-th token
+        // itself is in leaves few more than k (64 rows of 32,003 f16, top-k 2,000: 102 us by sample_row(), so 29; of
+        // 128,256 f32 327 and 64).
+        __syncthreads();
+        auto* counts = reinterpret_cast<unsigned long long*>(s.some);
+        static_assert(sizeof(s.some) == kBins * sizeof(unsigned long long));
+        for (int i = tid; i < kBins; i += kThreads) counts[i] = 0;
+        __syncthreads();
+        for (int b0 = tid / kLanes; b0 < groups; b0 += kStep) {
+          Piece<DT> x;
+          x.load(p, s.groups[b0] * GROUP + tid % kLanes * kValues, (int)a.vocab);
+#pragma unroll
+          for (int i = 0; i < kValues; ++i)
+            if (wanted(x[i])) atomicAdd(&counts[steps.of(x[i])], 1ull);
+        }
+        __syncthreads();
+        limit = bin_at(counts[2 * tid], counts[2 * tid + 1], limits.k);
+        if (limit < 0) return kElse;
+        n = 0;
+        few = true;
       }
     }
     __syncthreads();

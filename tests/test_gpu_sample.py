@@ -105,6 +105,18 @@ def test_equal_logits_go_by_their_index(dtype, levels):
             check(x, np.arange(16) / 16, **limits)  # on the borders of the shares
 
 
+@pytest.mark.parametrize("k", [900, 1500, 1999, 2048, 2049])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [5003, 32003, 70001])
+def test_many_of_top_k(vocab, dtype, k):
+    """As many as the groups whose maxima they are looked for by."""
+    rng = np.random.default_rng(vocab + k)
+    x = logits_of(rng, 8, vocab, dtype=dtype)
+    x[4:, ::2] = -math.inf
+    for limits in ({}, {"top_p": 0.97}, {"min_p": 1e-4}):
+        check(x, rng.random(8), top_k=k, **limits)
+
+
 @pytest.mark.parametrize("spread", [0.01, 0.3, 1.0])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_flat_rows_have_wide_nuclei(dtype, spread):
