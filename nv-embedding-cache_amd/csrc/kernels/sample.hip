@@ -30,7 +30,7 @@
 //
 // Measured, in us (bytes at the 4.8 TB/s of a large copy): 256 rows of 131,072 bf16 without limits 26 (14), of
 // which the scan 23: some 17 vector instructions a value, 3 of them in 64 bits, bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
-// rows, 63 (7): scan 11, pick 13, slices 11, rest 29, launches behind each other; one row, top-k 50, 14.2, two
+// rows, 63 to 70 (7): scan 11, pick 13, slices 11, rest 28, launches behind each other; one row, top-k 50, 14.2, two
 // launches.
 #include <math.h>
 
@@ -394,6 +394,13 @@ struct Steps {
     scale = width > 0.0f ? fminf((kBins - 0.1f) / width, 3e38f) : 3e38f;
   }
   __device__ __forceinline__ int of(float x) const { return (int)fminf((high - x) * scale, kBins - 1.0f); }
+  // Values above all and below all of bin b's: a bin's width and 2^-20 away, more than any rounding; or NaN.
+  __device__ __forceinline__ float above(int b) const { return away((float)(b - 1), 0x1p-20f); }
+  __device__ __forceinline__ float below(int b) const { return b == kBins - 1 ? -INFINITY : away((float)(b + 2), -0x1p-20f); }
+  __device__ __forceinline__ float away(float bins, float more) const {
+    const float edge = high - bins / scale;
+    return edge + (fabsf(high) + fabsf(edge)) * more;
+  }
 };
 
 // ---------------------------------------------------------------------------
@@ -484,7 +491,7 @@ struct RowShared {
     unsigned long long mass[kBins];
   };
   uint64_t table[kSteps];
-  double unit[kMostUnits / kMostSlices];
+  double part[kMostUnits / kMostSlices * kPieces];
   double red_sum[kWaves];
   unsigned long long red_mass[kWaves];
   int red_count[kWaves];
@@ -650,15 +657,14 @@ struct Pick {
     return place_of(s.n, by_mass, target - before);
   }
 
-  // The token within a unit: values from `cut` on, the least weight `low`.
-  __device__ __forceinline__ void pick_in_unit(int64_t unit, double base, double target, uint64_t cut, double low) const {
-    const int64_t first = unit * kUnit;
+  // The token among `size` values from `first` on, 2,048 at most: those from `cut` on, the least weight `low`.
+  __device__ __forceinline__ void pick_in(int64_t first, int size, double base, double target, uint64_t cut, double low) const {
     double w[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int64_t at = first + 2 * threadIdx.x + i;
       w[i] = 0.0;
-      if (2 * threadIdx.x + i < kUnit && at < a.vocab) {
+      if (2 * (int)threadIdx.x + i < size && at < a.vocab) {
         const float x = (float)p[at];
         const double y = weight(x);
         if (x > -INFINITY && key_of(x, at) >= cut && y >= low) w[i] = y;
@@ -703,7 +709,7 @@ struct Pick {
       if (!limits.p_on) {
         double target = u, before;
         const int unit = pick_item(m[0], m[1], 0.0, target, true, before);
-        pick_in_unit(unit, before, target, 0, 0.0);
+        pick_in((int64_t)unit * kUnit, kUnit, before, target, 0, 0.0);
         return kDone;
       }
       block_scan(m[0] + m[1], s.red_sum, all);
@@ -922,15 +928,23 @@ struct Pick {
       block_scan((2 * tid < whole ? x0 : 0) + (2 * tid + 1 < whole ? x1 : 0), s.red_mass, above);
       if (tid == 0) s.n = 0;
       __syncthreads();
+      // two comparisons before the bin, which takes some more instructions (a NaN above passes); with the runs below in
+      // place of units 100 rows of 32,003 f16 took 49.6 us a call, 52.8 without, 64 of 128,256 f32 67.5 and 68.6
+      const float above_all = steps.above(whole), below_all = fmaxf(steps.below(last), of.least);
       constexpr int kAhead = 2;  // units whose loads are under way together
       for (int64_t unit = wave; unit < l.units; unit += kAhead * kWaves) {
         Piece<DT> y[kAhead][kPieces];
 #pragma unroll
         for (int h = 0; h < kAhead; ++h) load_unit(y[h], p, (int)((unit + h * kWaves) * kUnit) + lane * kValues, (int)a.vocab);
 #pragma unroll
-        for (int h = 0; h < kAhead; ++h)
+        for (int h = 0; h < kAhead; ++h) {
+          if (unit + h * kWaves >= l.units) break;
 #pragma unroll
-          for (int j = 0; j < kPieces; ++j)
+          for (int j = 0; j < kPieces; ++j) {
+            bool some = false;
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) some |= (int)!(y[h][j][i] > above_all) & (int)(y[h][j][i] >= below_all);
+            if (!some) continue;
 #pragma unroll
             for (int i = 0; i < kValues; ++i) {
               const int b = steps.of(y[h][j][i]);
@@ -940,6 +954,8 @@ struct Pick {
                   s.some[at] = key_of(y[h][j][i], (unit + h * kWaves) * kUnit + (j * 64 + lane) * kValues + i);
               }
             }
+          }
+        }
       }
       __syncthreads();
       n = s.n;
@@ -980,34 +996,39 @@ struct Pick {
       if ((double)sum / mass_scale > target) break;
     }
     if (slice < 0) return false;
-    // the units' in that slice
+    // the runs' of a wave's piece in that slice
     const Weights weights(s.table, limits, top);
     const float cut_value = cut ? value_of(cut) : -INFINITY;
     const int64_t cut_index = cut ? index_of(cut) : -1;
     const int64_t first = (int64_t)slice * l.slice_units, last = min(first + l.slice_units, l.units);
-    for (int64_t unit = first + wave; unit < last; unit += kWaves) {
-      const int64_t at = unit * kUnit + lane * kValues;
-      Piece<DT> x[kPieces];
-      load_unit(x, p, (int)at, (int)a.vocab);
-      double mass = 0.0;
+    constexpr int kPart = 64 * kValues;
+    const int64_t part0 = first * kPieces, count = (last - first) * kPieces;
+    for (int at0 = wave; at0 < count; at0 += 4 * kWaves) {
+      Piece<DT> x[4];
 #pragma unroll
-      for (int j = 0; j < kPieces; ++j)
+      for (int j = 0; j < 4; ++j) x[j].load(p, (int)(part0 + at0 + j * kWaves) * kPart + lane * kValues, (int)a.vocab);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (at0 + j * kWaves >= count) break;
+        const int64_t at = (part0 + at0 + j * kWaves) * kPart + lane * kValues;
+        double mass = 0.0;
 #pragma unroll
         for (int i = 0; i < kValues; ++i) {
           const float v = x[j][i];
           const double w = weights(v);
-          const bool kept = (v > cut_value || (v == cut_value && at + j * 64 * kValues + i <= cut_index)) && w >= limits.low;
+          const bool kept = (v > cut_value || (v == cut_value && at + i <= cut_index)) && w >= limits.low;
           mass += kept ? w : 0.0;
         }
-      mass = of_lane(lanes_scan(mass), 63);
-      if (lane == 0) s.unit[unit - first] = mass;
+        mass = of_lane(lanes_scan(mass), 63);
+        if (lane == 0) s.part[at0 + j * kWaves] = mass;
+      }
     }
     __syncthreads();
-    const int i = 2 * tid, count = (int)(last - first);
+    const int i = 2 * tid;
     double to = target;
     double before;
-    const int unit = pick_item(i < count ? s.unit[i] : 0.0, i + 1 < count ? s.unit[i + 1] : 0.0, base, to, false, before);
-    pick_in_unit(first + unit, before, to, cut, limits.low);
+    const int part = pick_item(i < count ? s.part[i] : 0.0, i + 1 < count ? s.part[i + 1] : 0.0, base, to, false, before);
+    pick_in((part0 + part) * kPart, kPart, before, to, cut, limits.low);
     return true;
   }
 };
