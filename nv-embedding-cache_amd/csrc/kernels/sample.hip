@@ -228,11 +228,13 @@ struct Piece {
     if constexpr (DT == kBF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i / 2] >> (i & 1 ? 16 : 0)));
   }
-  // The greatest value; a NaN where the instruction makes one of the NaNs among them.
+  // The greatest value, or a NaN where there is one among them: this instruction passes on every NaN.  (A maximum of
+  // three as max(max(a, b), c) drops a and b where one of them is a signalling NaN, which leaves max(a, b) a quiet one.)
   __device__ __forceinline__ float top() const {
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kValues; i += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(m) : "v"((*this)[i]), "v"((*this)[i + 1]));
+    for (int i = 0; i < kValues; i += 2)
+      asm("v_maximum3_f32 %0, %0, %1, %2" : "+v"(m) : "v"((*this)[i]), "v"((*this)[i + 1]));
     return m;
   }
   // The same of what is no NaN.
@@ -386,14 +388,17 @@ __device__ __forceinline__ void sort_keys(uint64_t* keys, int n) {
   __syncthreads();
 }
 
-// kBins bins of one width from `high` down; the last one has all that is below, and what is no number.
+// kBins bins of one width from `high` down; the first one has all that is above (and what is no number), the last one
+// all that is below.  A width past f32 leaves a scale that keeps the order.
 struct Steps {
   float high, scale;
   __device__ __forceinline__ Steps(float high, float low) : high(high) {
     const float width = high - low;
-    scale = width > 0.0f ? fminf((kBins - 0.1f) / width, 3e38f) : 3e38f;
+    scale = width > 0.0f ? fminf(fmaxf((kBins - 0.1f) / width, 1e-36f), 3e38f) : 3e38f;
   }
-  __device__ __forceinline__ int of(float x) const { return (int)fminf((high - x) * scale, kBins - 1.0f); }
+  __device__ __forceinline__ int of(float x) const {
+    return (int)__builtin_amdgcn_fmed3f((high - x) * scale, 0.0f, kBins - 1.0f);
+  }
   // Values above all and below all of bin b's: a bin's width and 2^-20 away, more than any rounding; or NaN.
   __device__ __forceinline__ float above(int b) const { return away((float)(b - 1), 0x1p-20f); }
   __device__ __forceinline__ float below(int b) const { return b == kBins - 1 ? -INFINITY : away((float)(b + 2), -0x1p-20f); }
@@ -433,7 +438,7 @@ __global__ __launch_bounds__(kScanThreads, 7) void scan_kernel(const Sample a, c
     tops[j] = x[j].top();
     odd |= tops[j] != tops[j];
   }
-  if (__any(odd)) {  // NaNs that a maximum of three takes over
+  if (__any(odd)) {  // NaNs
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) tops[j] = x[j].top_of_numbers();
   }

@@ -142,6 +142,50 @@ def test_masked_rows(dtype):
             assert (got[::5] == -1).all() and (got[1::5] >= 0).all()
 
 
+def set_bits(x, at, bits):
+    """Puts the bit pattern `bits` at x[at]."""
+    kind, size = {4: (torch.int32, 32), 2: (torch.int16, 16)}[x.element_size()]
+    x.view(kind)[at] = bits - (1 << size) if bits >> (size - 1) else bits
+
+
+# signalling, signalling with its sign set, quiet
+NANS = {"f32": (0x7F800001, 0xFFA00000, 0x7FC00000), "f16": (0x7C01, 0xFD00, 0x7E00), "bf16": (0x7F81, 0xFFA0, 0x7FC0)}
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [3007, 66003])
+def test_no_nan_hides_what_is_beside_it(vocab, dtype, kind):
+    """A NaN at every place of 16 neighbours, the row's largest logit at every other one: in the row's first
+    neighbours, in its last ones and between."""
+    rng = np.random.default_rng(vocab)
+    pairs = [(m, n) for m in range(16) for n in range(16) if m != n]
+    x = logits_of(rng, len(pairs), vocab, dtype=dtype)
+    most = int(x.float().max()) + 2
+    for r, (m, n) in enumerate(pairs):
+        first = [0, vocab // 3 // 16 * 16, (vocab - 1) // 16 * 16 - 16][r % 3]
+        x[r, first + m] = float(most)
+        set_bits(x, (r, first + n), NANS[dtype][kind])
+    u = rng.random(len(pairs))
+    best = [[0, vocab // 3 // 16 * 16, (vocab - 1) // 16 * 16 - 16][r % 3] + m for r, (m, _) in enumerate(pairs)]
+    assert check(x, u, temperature=0.0).tolist() == best and check(x, u, top_k=1).tolist() == best
+    for limits in ({"top_k": 3}, {"top_p": 0.5}) + (({}, {"top_p": 0.9}, {"min_p": 0.1}) if vocab < 4000 else ()):
+        check(x, u, **limits)
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_rows_of_nans_but_for_a_few(dtype, kind):
+    rng = np.random.default_rng(14)
+    x = logits_of(rng, 32, 9001, dtype=dtype)
+    for r in range(32):
+        off = torch.from_numpy(rng.permutation(9001)[[0, 1, 2, 40][r % 4]:])
+        set_bits(x, (r, off), NANS[dtype][kind])
+    for limits in ({}, {"top_k": 2}, {"top_p": 0.6}, {"min_p": 0.1}, {"temperature": 0.0}):
+        got = check(x, rng.random(32), **limits)
+        assert (got[::4] == -1).all() and (got[1::4] >= 0).all()
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_infinite_and_extreme_logits(dtype):
     rng = np.random.default_rng(7)
