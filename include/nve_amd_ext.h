@@ -363,7 +363,7 @@ NVE_C_API nve_status_t nve_amd_kv_evict(const nve_amd_kv_pages_t* pages,
  * vocabulary's order, at which the sum of the kept w_j, j <= i, exceeds u times
  * their sum.  temperature 0: the first of the largest logits.  Exponentials and
  * sums are 64-bit; in the sum over a whole row of 16-bit logits a weight is within
- * 2^-34 of its value.  temperatures, top_ks, top_ps and min_ps (device, [num_rows])
+ * 2^-31 of its value.  temperatures, top_ks, top_ps and min_ps (device, [num_rows])
  * hold a limit for each row; NULL: the one value beside it counts for all.  In
  * device memory a temperature that is not above 0 counts as 0, a top_k below 1
  * as 0, a top_p or min_p that is no number as none, one outside [0, 1] as the

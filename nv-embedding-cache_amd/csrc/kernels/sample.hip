@@ -29,7 +29,7 @@
 // CUs, pick_kernel has it inlined and rest_kernel is not launched (one row of 50,021: 15.5 to 14.2 us).
 //
 // Measured, in us (bytes at the 4.8 TB/s of a large copy): 256 rows of 131,072 bf16 without limits 26 (14), of
-// which the scan 23: some 17 vector instructions a value, 3 of them in 64 bits, bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
+// which the scan 23: some 15 vector instructions a value, 3 of them in 64 bits, bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
 // rows, 63 to 70 (7): scan 11, pick 13, slices 11, rest 28, launches behind each other; one row, top-k 50, 14.2, two
 // launches.
 #include <math.h>
@@ -81,7 +81,7 @@ struct Limits {
   bool greedy, k_on, p_on, low_on;
   bool plain;  // the temperature leaves everything in f32's range
   int64_t k;
-  double p, low, scale;  // scale: log2(e) / T
+  double p, low, scale, inverse;  // scale: log2(e) / T; inverse: of that
   __device__ __forceinline__ Limits(const Sample& a, int64_t row) {
     const float t = a.temperature ? a.temperature[row] : a.temperature_all;
     const float pf = a.top_p ? a.top_p[row] : a.top_p_all;
@@ -95,6 +95,7 @@ struct Limits {
     low = low_on ? fmin((double)lf, 1.0) : 0.0;
     plain = t >= 1e-30f && t <= 1e30f;
     scale = greedy ? 0.0 : 1.4426950408889634 / (double)t;
+    inverse = (double)t * 0.6931471805599453;
   }
   __device__ __forceinline__ bool all_mass() const { return !greedy && plain && !k_on && (p_on || !low_on); }
 };
@@ -102,7 +103,8 @@ struct Limits {
 // ---------------------------------------------------------------------------
 // 2^z in 64 bits
 // ---------------------------------------------------------------------------
-constexpr int kSteps = 256;  // of the table
+constexpr int kStepBits = 8;
+constexpr int kSteps = 1 << kStepBits;  // of the table
 
 // 2^(j / kSteps) from the exponential's series, with j taken off the exponent's field again, so that
 // adding the whole exponent (in units of 1 / kSteps) to the high word gives the power.
@@ -127,37 +129,46 @@ constexpr std::array<uint64_t, kSteps> make_powers() {
       }
     }
     if (rest >= 0.5L) ++bits;
-    t[j] = (bits | (uint64_t)1023 << 52) - ((uint64_t)j << (52 - 8));
+    t[j] = (bits | (uint64_t)1023 << 52) - ((uint64_t)j << (52 - kStepBits));
   }
   return t;
 }
 __constant__ const std::array<uint64_t, kSteps> kPowers = make_powers();
-static_assert(kSteps == 1 << 8);
 
-// Weights 2^((x - high) scale) for x <= high: n, the exponent in steps of 1 / 256, the table, and the series up
+// A table's power with n, in steps, added to its exponent.
+__device__ __forceinline__ double raised(uint64_t power, int n) {
+  return __hiloint2double((int)(power >> 32) + (n << (20 - kStepBits)), (int)power);
+}
+
+// 2^(steps / kSteps) as a power and the factor that completes it: n, the whole steps, the table, and the series up
 // to the third power for the rest, |r| <= 1/2 of a step, whose next term is (ln 2 / 512)^4 / 24 = 1.4e-13.
-// Less than 2^-1000 is 0 (parts(): 2^-1000, nothing beside a sum of 1 and more).
+// near: steps plus 0x1.8p52, which rounds to a whole number; rest: steps plus what it is given, rounded once.
+template <typename REST>
+__device__ __forceinline__ void power_parts(const uint64_t* table, double near, REST rest, double& power, double& factor) {
+  constexpr double k1 = 0.6931471805599453 / kSteps, k2 = k1 * k1 / 2, k3 = k1 * k1 * k1 / 6;
+  const int n = (int)__double_as_longlong(near);
+  const double r = rest(0x1.8p52 - near);
+  double y;  // the compiler would copy k2 for every use
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(r), "s"(k3), "v"(k2));
+  factor = fma(r, fma(r, y, k1), 1.0);
+  power = raised(table[n & (kSteps - 1)], n);
+}
+
+// Weights 2^((x - high) scale) for x <= high.  Less than 2^-1000 is 0 (parts(): 2^-1000, nothing beside a sum of 1
+// and more).
 struct Weights {
   const uint64_t* table;
   double high, scale;  // of a step
   double least;        // x - high: what is below has no weight
   __device__ __forceinline__ Weights(const uint64_t* table, const Limits& limits, float high)
-      : table(table), high(high), scale(limits.scale * kSteps), least(-1000.0 / limits.scale) {}
+      : table(table), high(high), scale(limits.scale * kSteps), least(-1000.0 * limits.inverse) {}
   static __device__ __forceinline__ void fill(uint64_t* t) {
     if (threadIdx.x < kSteps) t[threadIdx.x] = kPowers[threadIdx.x];
   }
   // The power and the factor that completes it; a NaN counts as nothing.
   __device__ __forceinline__ void parts(float x, double& power, double& factor) const {
-    constexpr double k1 = 0.6931471805599453 / kSteps, k2 = k1 * k1 / 2, k3 = k1 * k1 * k1 / 6;
     const double d = __builtin_fmax((double)x - high, least);
-    const double t = fma(d, scale, 0x1.8p52);  // rounds to a whole number of steps
-    const int n = (int)__double_as_longlong(t);
-    const double r = fma(d, scale, 0x1.8p52 - t);
-    double y;  // the compiler would copy k2 for every use
-    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(r), "s"(k3), "v"(k2));
-    factor = fma(r, fma(r, y, k1), 1.0);
-    const uint64_t p = table[n & (kSteps - 1)];
-    power = __hiloint2double((int)(p >> 32) + (n << 12), (int)p);
+    power_parts(table, fma(d, scale, 0x1.8p52), [&](double more) { return fma(d, scale, more); }, power, factor);
   }
   __device__ __forceinline__ double operator()(float x) const {
     double power, factor;
@@ -166,28 +177,44 @@ struct Weights {
   }
 };
 
-// Adds weights of 16-bit logits to a sum, with what is small in 32 bits, as 64 take twice as long: the difference
-// to the maximum (exact where it is not 2^16 times x, 2^13 for f16, and its 2^-25 else), its product with the scale in
-// two parts, and the series without its 1, at most 2^-10 and 2^-24 of that off.  So a weight is 2^-34 off at most,
-// and a sum of thousands far less; the maximum's is exactly 1.
+// Adds weights of 16-bit logits, none of them a NaN, to a sum, with what is small in 32 bits, as 64 take twice as long.
+// x scale, not (x - high) scale, is taken apart: a difference in 32 bits is 2^-25 of itself off where x is far smaller
+// than high.  Whole powers of two of high go with the rounding, and the rest of them is one factor of the sum.
+// A weight is within 2^-31 = 4.7e-10 of its value.  In steps, z = x scale < 2^19, with the scale in two floats: what is left
+// of z behind its whole steps, r < 0.532, rounds twice, 2^-26 and 2^-25, and misses 2^-29 of z: 1.3e-10 of the weight.
+// The series without its 1 has 3/16 of its third power, as a multiple of r, with the first: with the constants'
+// rounding 1.3e-10 off; it rounds by 0.532 2^-33 and 2^-34, 1.2e-10.  (1,024 steps, 2^-33: 256 rows of 131,072
+// bf16 in 32.6 us in place of 29.6.)
 struct Weights16 {
   const uint64_t* table;
-  float high, scale, scale_rest, least;
+  float scale, scale_rest, least;
+  float near;  // rounds to a whole number of steps, and takes high's whole powers of two off
+  double factor;
+  static __device__ __forceinline__ bool fits(const Limits& limits, float high) {
+    return fabs((double)high) * limits.scale <= 1024.0;
+  }
   __device__ __forceinline__ Weights16(const uint64_t* table, const Limits& limits, float high)
-      : table(table), high(high), scale((float)(limits.scale * kSteps)),
-        scale_rest((float)(limits.scale * kSteps - (double)scale)), least((float)(-1000.0 / limits.scale)) {}
+      : table(table), scale((float)(limits.scale * kSteps)), scale_rest((float)(limits.scale * kSteps - (double)scale)),
+        least((float)((double)high - 1000.0 * limits.inverse)) {
+    const double powers = rint((double)high * limits.scale);
+    near = 0x1.8p23f - (float)powers * kSteps;  // exact
+    const double steps = fma((double)high, -limits.scale, powers) * kSteps;
+    double power, rest;
+    power_parts(table, steps + 0x1.8p52, [&](double more) { return steps + more; }, power, rest);
+    factor = power * rest;
+  }
+  // The sum is to be multiplied by the factor.
   __device__ __forceinline__ void add(float x, double& sum) const {
     constexpr double k = 0.6931471805599453 / kSteps;
-    constexpr float k1 = (float)k, k2 = (float)(k * k / 2), k3 = (float)(k * k * k / 6);
-    const float d = __builtin_fmaxf(x - high, least);
-    const float t = fmaf(d, scale, 0x1.8p23f);  // rounds to a whole number of steps
-    const float m = t - 0x1.8p23f;
+    constexpr float k1 = (float)(k + 3.0 / 16 * (k * k * k / 6)), k2 = (float)(k * k / 2);
+    float y;  // fmaxf() would first make NaNs quiet
+    asm("v_max_f32 %0, %1, %2" : "=v"(y) : "v"(x), "v"(least));
+    const float t = fmaf(y, scale, near);
+    const float r = fmaf(y, scale_rest, fmaf(y, scale, near - t));
+    const float more = r * fmaf(r, k2, k1);
     const int n = __float_as_int(t) - __float_as_int(0x1.8p23f);
-    const float r = fmaf(d, scale_rest, fmaf(d, scale, -m));
-    const float y = r * fmaf(r, fmaf(r, k3, k2), k1);
-    const uint64_t p = table[n & (kSteps - 1)];
-    const double power = __hiloint2double((int)(p >> 32) + (n << 12), (int)p);
-    sum = fma(power, (double)y, sum + power);
+    const double power = raised(table[n & (kSteps - 1)], n);
+    sum = fma(power, (double)more, sum + power);
   }
 };
 
@@ -438,7 +465,8 @@ __global__ __launch_bounds__(kScanThreads, 7) void scan_kernel(const Sample a, c
     tops[j] = x[j].top();
     odd |= tops[j] != tops[j];
   }
-  if (__any(odd)) {  // NaNs
+  const bool nans = __any(odd);
+  if (nans) {
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) tops[j] = x[j].top_of_numbers();
   }
@@ -454,25 +482,34 @@ __global__ __launch_bounds__(kScanThreads, 7) void scan_kernel(const Sample a, c
   top = lanes_max<64>(top);
   double sum = 0.0;
   if (top > -INFINITY && top < INFINITY) {
-    const Weights weights(table, limits, top);
-    const Weights16 weights16(table, limits, top);
+    // piece by piece: all values taken apart together, as for the maxima, would need too many registers
+    auto add = [&](auto one) {
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      // piece by piece: all values taken apart together, as for the maxima, would need too many registers
-      asm volatile("" : "+v"(x[j].w));
+      for (int j = 0; j < kPieces; ++j) {
+        asm volatile("" : "+v"(x[j].w));
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) {
-        if constexpr (DT == kF32) {
-          double power, factor;
-          weights.parts(x[j][i], power, factor);
-          sum = fma(power, factor, sum);
-        } else {
-          weights16.add(x[j][i], sum);
-        }
+        for (int i = 0; i < kValues; ++i) one(x[j][i]);
+        asm volatile("" : "+v"(sum));
       }
-      asm volatile("" : "+v"(sum));
+      sum = of_lane(lanes_scan(sum), 63);
+    };
+    auto exact = [&] {
+      const Weights weights(table, limits, top);
+      add([&](float v) {
+        double power, factor;
+        weights.parts(v, power, factor);
+        sum = fma(power, factor, sum);
+      });
+    };
+    if constexpr (DT == kF32) {
+      exact();
+    } else if (!nans && __builtin_amdgcn_readfirstlane(Weights16::fits(limits, top))) {
+      const Weights16 weights(table, limits, top);
+      add([&](float v) { weights.add(v, sum); });
+      sum *= weights.factor;
+    } else {
+      exact();
     }
-    sum = of_lane(lanes_scan(sum), 63);
   }
   if (lane == 0) {
     l.unit_top[row * l.units + unit] = top;

@@ -26,7 +26,7 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     `min_p`.  The token is the first index, in the vocabulary's order, at which the
     running sum of the kept w exceeds u times their sum.  A temperature of 0 takes
     the first of the largest logits.  Exponentials and sums are 64-bit; in the sum over
-    a whole row of 16-bit logits a weight is within 2^-34 of its value.
+    a whole row of 16-bit logits a weight is within 2^-31 of its value.
 
     Each limit is a number or a tensor [rows] (float32; top_k int32) on the logits'
     GPU, where a temperature that is not above 0 counts as 0, a top_k below 1 as 0 and

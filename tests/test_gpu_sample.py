@@ -351,3 +351,43 @@ def test_refusals():
         run(logits=x.clone().requires_grad_())
     with torch.no_grad():
         run(logits=x.clone().requires_grad_())
+
+
+def check_shares(row, temperature, u):
+    """The tokens that `u` draws from `row`, all of whose tokens are kept: a weight may be 2^-31 of itself off, so the
+    sums before and up to a token, and u times the total, by as much of the total each; 64-bit sums and series by
+    far less than the 2^-41 that are left for them."""
+    from pynve.torch.nve_sample import sample_tokens
+
+    got = sample_tokens(row.cuda().expand(len(u), -1), cuda(u), temperature=temperature).cpu().numpy()
+    x = row.double().numpy().astype(np.longdouble)
+    w = np.exp((x - x.max()) / np.longdouble(np.float32(temperature)))
+    after = np.cumsum(w)
+    target, room = u.astype(np.longdouble) * after[-1], after[-1] * (2.0**-30 + 2.0**-41)
+    assert (w[got] > 0).all()
+    low, high = after[got] - w[got] - target, target - after[got]
+    assert (low <= room).all() and (high <= room).all(), (float(low.max() / after[-1]), float(high.max() / after[-1]))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("high, small, temperature", [(6.0, 1.93e-5, 1.0), (12.0, 1.93e-5, 0.7), (60.0, 3e-4, 30.0),
+                                                      (16.0, 0.011, 1.0), (-3.0, -3.01, 0.01), (700.0, 1.0, 1.0),
+                                                      (5000.0, 4990.0, 2.0), (0.0, -1e-3, 1e-4)])
+def test_sums_over_16_bit_rows(dtype, high, small, temperature):
+    """Logits far smaller than the largest, one of which every 2,048 of the row's first half have."""
+    n = 1 << 17
+    x = torch.full((n,), small)
+    x[:n // 2:2048] = high
+    check_shares(x.to(TYPES[dtype]), temperature, ((np.arange(4096) + 0.5) / 4096).astype(np.float32))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("temperature", [1e-6, 0.01, 0.3, 1.0, 7.0, 1000.0])
+def test_16_bit_rows_at_any_temperature(dtype, temperature):
+    """Magnitudes from 2^-14 to 2^6 of both signs beside a few large logits, units of both kinds."""
+    rng = np.random.default_rng(15)
+    x = rng.choice([-1.0, 1.0], size=40961) * 2.0 ** rng.uniform(-14, 6, size=40961)
+    x[rng.integers(0, 40961, size=30)] = 64.0
+    x[20000:24000] = rng.normal(0, 1e-3, size=4000)
+    u = np.sort(rng.random(4000)).astype(np.float32)
+    check_shares(torch.from_numpy(x).to(TYPES[dtype]), temperature, u)
