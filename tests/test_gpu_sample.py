@@ -81,6 +81,16 @@ def test_more_rows_than_a_launch(rows, vocab, limits):
     check(logits_of(rng, rows, vocab, spread=0.5 if rows % 100 else 2.0, dtype="bf16"), rng.random(rows), **limits)
 
 
+@pytest.mark.parametrize("limits", [{"top_p": 0.9}, {"top_p": 0.97, "min_p": 0.05}, {"min_p": 0.3}])
+@pytest.mark.parametrize("rows", [257, 400, 700, 1100])
+def test_many_wide_rows(rows, limits):
+    """Rows with wide nuclei by fewer and fewer slices."""
+    rng = np.random.default_rng(rows)
+    for dtype in ("f32", "bf16"):
+        x = torch.from_numpy(rng.normal(0, 0.7, size=(rows, 16387)).astype(np.float32)).to(TYPES[dtype])
+        check(x, rng.random(rows), **limits)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 7, 64, 300, 1025])
 def test_every_row_has_limits_of_its_own(rows):
     rng = np.random.default_rng(rows)

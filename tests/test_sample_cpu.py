@@ -47,6 +47,18 @@ def test_null_struct_and_workspace():
             assert "orkspace" in _lib.last_error()
 
 
+@pytest.mark.parametrize("rows", [1, 64, 256, 300, 1024, 2048, 5000, 1 << 20])
+@pytest.mark.parametrize("vocab", [16, 2049, 16384, 32003, 65536, 65537, 131072, 1 << 19, 1 << 30])
+@pytest.mark.parametrize("dtype", [_lib.DT_F32, _lib.DT_F16, _lib.DT_BF16])
+def test_workspace_is_bounded(dtype, vocab, rows):
+    """2^27 logits at once at most, 4 bytes for 64 of them (2^25, for 16), 12 for 1,024, and 2,048 histograms of 16 KiB."""
+    n = ctypes.c_uint64()
+    c = _lib.Sample(num_rows=rows, vocab_size=vocab, dtype=dtype, logits=FAKE, row_stride=vocab, u=FAKE, temperature=1.0,
+                    top_p=0.9, tokens=FAKE)
+    _lib.call("nve_amd_sample_workspace_size", ctypes.byref(c), ctypes.byref(n))
+    assert n.value <= (8 << 20) + (12 << 17) + (32 << 20) + (1 << 20)
+
+
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
 def test_struct_layout(tmp_path):
     fields = [f[0] for f in _lib.Sample._fields_]
