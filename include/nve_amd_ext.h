@@ -274,7 +274,8 @@ NVE_C_API nve_status_t nve_amd_kv_append(const nve_amd_kv_pages_t* pages,
  * row x of head_dim values becomes (x[d] * r) * weight[d], both products f32,
  * with r = 1 / sqrt(mean of x[d]^2 + eps), the mean and r in 64 bits and r then
  * rounded to f32.  Weights: [head_dim] of the call's dtype; a NULL weight leaves
- * those heads without a norm.  eps is finite and not negative. */
+ * those heads without a norm.  eps is finite and not negative; with 0 a row of
+ * zeros becomes NaN. */
 typedef struct {
   const void* q_weight;
   const void* k_weight;

@@ -60,7 +60,7 @@ def kv_append(k, v, k_pages, v_pages, slots, *, q=None, positions=None, cos_sin=
 
     With `q_norm` or `k_norm` ([D] of the rows' type) the query or key heads are
     normalised first: x / sqrt(mean(x ** 2) + eps) * norm, head by head (the mean
-    in 64 bits, the products float32).
+    in 64 bits, the products float32; with an eps of 0 a row of zeros becomes NaN).
 
     4-bit pages: 32 values share a scale, the least power of two of which no
     magnitude is over 7 times; a value becomes the nearest of 0, .5, 1, 1.5, 2, 3, 4

@@ -166,6 +166,36 @@ def test_zero_tiny_and_large_rows(dtype, cache, norms, eps):
     run(dtype, cache, 41, 4, 2, 64, 16, 64, seed=2, edit=edit, norms=norms, eps=eps)
 
 
+@pytest.mark.parametrize("rot", [64, 24])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_zero_rows_without_eps_in_8_bits(dtype, rot):
+    """A row of zeros has no norm where eps is 0: NaN, with a NaN for its scale.  The rows beside it are as ever."""
+    from pynve.torch import nve_kv
+
+    rng = np.random.default_rng(10)
+    dt, n = R.TORCH[dtype], 23
+    q, k, v = (torch.from_numpy(rng.normal(0, 1, size=(n, h, 64)).astype(np.float32)).to(dt) for h in (4, 2, 2))
+    for x in (q, k, v):
+        x[::3] = 0
+    k[1, 0] = 0
+    weight = {x: torch.from_numpy(np.exp(rng.normal(0, 0.5, size=64)).astype(np.float32)).to(dt) for x in "qk"}
+    cs, pos = table_of(50, rot), rng.integers(0, 50, size=(1, n)).astype(np.int32)
+    cache = nve_kv.KVCache(3, 2, 64, dtype=torch.float8_e4m3fn)
+    out = cache.append(k.cuda(), v.cuda(), torch.arange(n).cuda(), q=q.cuda(), positions=torch.from_numpy(pos[0]).cuda(),
+                       cos_sin=torch.from_numpy(cs).cuda(), q_norm=weight["q"].cuda(), k_norm=weight["k"].cuda(), eps=0.0)
+    rows = [R.rotate(torch.from_numpy(R4.norm(x, w, 0.0)), pos, cs, [rot // 2], False)
+            for x, w in ((q, weight["q"]), (k, weight["k"]))] + [v.float().numpy()]
+    assert same(out.cpu(), torch.from_numpy(rows[0]).to(dt))
+    at = np.arange(n)
+    for pages, scales, r in ((cache.k, cache.k_scale, rows[1]), (cache.v, cache.v_scale, rows[2])):
+        got, scale = pages.cpu()[at // 16, :, at % 16].float(), scales.cpu()[at // 16, :, at % 16]
+        none = torch.from_numpy(np.isnan(r).any(-1))
+        codes, want = R.quantize(np.nan_to_num(r))
+        assert torch.equal(torch.isnan(scale), none) and torch.isnan(got[none]).all()
+        assert torch.equal(scale[~none], want[~none]) and torch.equal(got[~none], codes[~none].float())
+    assert torch.isnan(cache.k_scale.cpu()[0, :, 0]).all() and not torch.isnan(cache.v_scale).any()
+
+
 @pytest.mark.parametrize("dtype,cache", MX)
 @pytest.mark.parametrize("rot", [0, 32, 64])
 def test_values_on_the_borders_of_codes_and_scales(dtype, cache, rot):
