@@ -41,6 +41,17 @@
 // a unit's sum: the first kernel for whole units, the second, piece by piece, for
 // the others, from the scores that the first one left in the workspace.
 //
+//   Grid mode: a workgroup per piece of grid_chunk() tiles, as the tables' extent
+//   asks for.  The unit is the fast index: consecutive workgroups go round the 8
+//   XCDs, and later pieces exist for the long sequences only; with the piece as the
+//   fast index (4 a unit) the first pieces met on two XCDs (64 sequences of 512 to
+//   8,192 slots: 273 us, units first 183).
+//   Stream mode, for tables far longer than their sequences: the machine's resident
+//   workgroups share all tiles there are, units laid end to end, in equal runs.
+// Two waves a SIMD at 128 values of 8 to 32 bits (one at 256, three at 64): k and v rows of the
+// next step are in flight meanwhile, 32 KiB a workgroup.  Three were slower (one sequence
+// of 200,001 slots: 170 us, two 146).
+//
 // 4-bit pages: a wave's step is 4.3 KB (128 values), a quarter of bf16's, so the work per slot counts, and more waves
 // have to be under way: three a SIMD at 128 values.  Codes become bf16 with their scale in one instruction a pair
 // (the conversion looks at nothing but a scale's exponent, so its byte is rotated into place and no more; the product
@@ -49,16 +60,10 @@
 // 400,001 slots, f16: 141 us with bf16's launch and two waves, 118 with output tiles two at a time, 106 with 512
 // pieces, 97 with fewer registers, three waves and 768 pieces: 4.5 TB/s.  64 of 512 to 8,192 with weights: 87 to 79 us.
 // Steps of 64 slots: 102 and 82 us.  f16 queries meet bf16 rows as two values of bf16, which hold all of their bits.
-//   Grid mode: a workgroup per piece of grid_chunk() tiles, as the tables' extent
-//   asks for.  The unit is the fast index: consecutive workgroups go round the 8
-//   XCDs, and later pieces exist for the long sequences only; with the piece as the
-//   fast index (4 a unit) the first pieces met on two XCDs (64 sequences of 512 to
-//   8,192 slots: 273 us, units first 183).
-//   Stream mode, for tables far longer than their sequences: the machine's resident
-//   workgroups share all tiles there are, units laid end to end, in equal runs.
-// Two waves a SIMD at 128 values (one at 256, three at 64): k and v rows of the next
-// step are in flight meanwhile, 32 KiB a workgroup.  Three were slower (one sequence
-// of 200,001 slots: 170 us, two 146).
+// The other widths (200,001 slots, bf16): 64 values 66 us with two, three or four waves, four taken, although with weights
+// two take 51 us and three or four 70, as stream mode is slower with two (64 sequences of up to 2,000 slots: 28.5, four 25);
+// four spill up to 12 registers in the kernels with weights, three of 32 values take 83 us for 64 of 512 to 8,192
+// with weights, four 72.  256 values: two waves 93 us, one 110.
 //
 // Measured (bf16 / f16, 128 values, pages of 16): one sequence of 200,001 slots, 8 key
 // heads: 144 us, 5.7 TB/s of the pages' bytes (a large copy moves 4.7 TB/s, read and
@@ -1075,9 +1080,11 @@ struct Layout {
 //   Whole units, one launch, up to 4 tiles (one piece 12.2 us, 32 pieces and a join 10.3 us for one
 //   sequence of 4,096 slots, but 34.9 against 43.4 us for 256 of 32 to 512), and up to 16 where
 //   there are units for all CUs (64 sequences of 125 to 2,000 slots: whole 33.9, pieces of 8 42.3).
-//   One sequence: 256 pieces, one a CU, are enough (768 of 4-bit pages; 200,001 slots: 144 us, stream 155, pieces of 16
+//   One sequence: 256 pieces, one a CU, are enough (200,001 slots: 144 us, stream 155, pieces of 16
 //   tiles 165; 16,384: 17.7, stream 23.6, 1 tile 22.0). Its tiles are shared by these pieces as its
 //   length asks for, which only the kernels know: its table may be far longer.
+//   4-bit pages: 768 (200,001 slots of 8 key heads, 64 values: 66 us, 1,024 pieces 59; of one head 41 and 54; 16,000 of
+//   8 heads 12.3 and 14.7; 256 values: 93, 512 pieces 89; of one head 51 and 41; 16,000 slots 19 and 19).
 //   Several may be much shorter than the longest: smaller pieces (7 of 33 to 30,011 slots, 2 key
 //   heads: pieces of 4 tiles 22 us, 8 29, stream 35; 64 of 512 to 8,192: 8 tiles 180, 16 188, stream 186).
 //   In f32 (64-slot tiles) 8 is the most: 48 sequences of up to 2,000 slots 30.5 us, 12 32.2.

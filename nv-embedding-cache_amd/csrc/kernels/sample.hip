@@ -18,8 +18,9 @@
 //                  read again.  Few tokens are kept: k maxima above a value are k tokens above it, and
 //                  maxima whose weights sum to p of all are a nucleus, so only groups with a maximum
 //                  above such a value are read again, and their values above it sorted
-//   slice_kernel   up to 8 workgroups, fewer where there are many rows, for each row that pick_kernel found too wide (a flat nucleus, a low
-//                  min-p): histograms of mass.  Launched where the limits allow such rows
+//   slice_kernel   up to 8 workgroups (fewer where there are many rows) for each row that pick_kernel found
+//                  too wide (a flat nucleus, a low min-p): histograms of mass.  Launched where the limits
+//                  allow such rows
 //   rest_kernel    those rows: the cut's bin is gathered and sorted, the slice that u falls into read
 //                  again; and what is left (a top-k of nearly 2,048 and more, or of more than there are groups,
 //                  infinities, many equals at a wide cut), with sample_row() (sample_select.cuh)
@@ -29,8 +30,8 @@
 // CUs, pick_kernel has it inlined and rest_kernel is not launched (one row of 50,021: 15.5 to 14.2 us).
 //
 // Measured, in us (bytes at the 4.8 TB/s of a large copy): 256 rows of 131,072 bf16 without limits 26 (14), of
-// which the scan 23: some 15 vector instructions a value, 3 of them in 64 bits, bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
-// rows, 63 to 70 (7): scan 11, pick 13, slices 11, rest 28, launches behind each other; one row, top-k 50, 14.2, two
+// which the scan 22.5: some 15 vector instructions a value, 3 of them in 64 bits, bound it; 64 rows of 128,256 f32, top-p 0.95 of flat
+// rows, 66 to 70 (7): scan 11, pick 13, slices 11, rest 28, launches behind each other; one row, top-k 50, 14.2, two
 // launches.
 #include <math.h>
 
@@ -570,7 +571,7 @@ struct Pick {
   double u;
 
   __device__ __forceinline__ double weight(float x) const { return Weights(s.table, limits, top)(x); }
-  // A weight times 2^shift, rounded; the sum is below 2^52.
+  // A weight, 1 at most, times 2^shift, 2^51 at most, rounded by adding 2^52; those of a row sum to less than 2^62.
   __device__ __forceinline__ unsigned long long mass_of(double w) const {
     return (unsigned long long)__double_as_longlong(w * mass_scale + 0x1p52) & ((1ull << 52) - 1);
   }

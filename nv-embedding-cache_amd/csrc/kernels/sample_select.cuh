@@ -49,7 +49,7 @@ struct Row {
     if (top == INFINITY || x == -INFINITY) return 0.0;
     return exp(((double)x - (double)top) * inverse);
   }
-  // A weight times 2^shift, rounded; the sum is below 2^52.
+  // A weight, 1 at most, times 2^shift, 2^51 at most, rounded by adding 2^52; those of a row sum to less than 2^62.
   __device__ __forceinline__ unsigned long long mass(float x) const {
     const double w = weight(x) * mass_scale + 0x1p52;
     return (unsigned long long)__double_as_longlong(w) & ((1ull << 52) - 1);
