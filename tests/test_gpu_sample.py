@@ -401,3 +401,26 @@ def test_16_bit_rows_at_any_temperature(dtype, temperature):
     x[20000:24000] = rng.normal(0, 1e-3, size=4000)
     u = np.sort(rng.random(4000)).astype(np.float32)
     check_shares(torch.from_numpy(x).to(TYPES[dtype]), temperature, u)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("temperature", [1e-30, 1e-3, 0.05, 30.0, 1e6, 1e30, math.inf])
+def test_extreme_temperatures_of_16_bit_rows(dtype, temperature):
+    rng = np.random.default_rng(16)
+    x = logits_of(rng, 12, 20011, dtype=dtype)
+    x[4:8, ::2] = torch.from_numpy(rng.normal(0, 1e-4, size=(4, 10006)).astype(np.float32)).to(x.dtype)
+    x[8:, ::3] = -math.inf
+    x[10] -= x[10].max()
+    for limits in ({}, {"top_k": 30}, {"top_p": 0.6}, {"min_p": 0.3}):
+        check(x, rng.random(12), temperature=temperature, **limits)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("high", [709.0, 711.0, -709.0, -711.0, 0.0])
+def test_16_bit_rows_where_the_sums_change(dtype, high):
+    """Largest logits on both sides of 1,024 octaves, and weights down to nothing."""
+    rng = np.random.default_rng(17)
+    x = torch.from_numpy(high - rng.exponential(3.0, size=30011)).to(TYPES[dtype])
+    x[::7] = high - 900.0
+    x[5] = high
+    check_shares(x, 1.0, np.sort(rng.random(2000)).astype(np.float32))
